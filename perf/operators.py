@@ -391,7 +391,9 @@ def run(state):
                                            state["committed"], max_accepted=case["keep"])
         return {"nodes": kept.nodes, "count": kept.num_accepted, "tokens": kept.tokens,
                 "lengths": kept.committed_lengths, "rows": kept.last_rows}
-    framework.compact_draft_kv(state["layers"], state["table"], state["committed"], state["path"], state["kept"])
+    if "mover" not in state:  # made once for the caches of a program's layers
+        state["mover"] = framework.DraftKVCompactor(state["layers"])
+    state["mover"](state["table"], state["committed"], state["path"], state["kept"])
     return _bits(state["caches"])
 
 
