@@ -53,6 +53,10 @@ extern "C" {
 #define MVB_STATUS_POSITION_PAST_TABLE 4 /* position past its request's block ids: slot -1 */
 #define MVB_STATUS_INCONSISTENT_COUNTS 8 /* counts disagree with the sizes: padding only */
 #define MVB_STATUS_WAIT_TIMEOUT 16       /* a kernel's bounded wait ran out: its rows are undefined */
+#define MVB_STATUS_BAD_PARENT 32         /* a drafted node's parent is no earlier node: taken as a root */
+
+/* Most drafted nodes of one request (64 per word of an ancestor mask). */
+#define MVB_MAX_TREE_NODES 1024
 
 /* Visibility specs of mvb_build_metadata (attention/spec.py). */
 #define MVB_SPEC_FULL 0           /* FullAttentionSpec: start 0                          */
@@ -368,6 +372,115 @@ MVB_API int mvb_build_metadata(const int32_t* num_computed_tokens,
                                int64_t* context_lengths, int64_t* block_table,
                                int64_t* slot_mapping, int64_t* sampling_rows, int32_t* status,
                                void* stream);
+
+/*
+ * Draft trees (speculative decoding): one step verifies, per request, a tree
+ * of drafted tokens.  No counterpart in the reference project, whose decode
+ * step takes one token per request.
+ *
+ * Request r owns nodes query_start_locations[r] .. [r+1] of the flattened
+ * batch.  parents[t] is the index inside the request of node t's parent, an
+ * earlier node, or -1 for a root; a parent that is neither sets
+ * MVB_STATUS_BAD_PARENT and counts as -1.  Node 0 is the request's pending
+ * token (sampled last, its K/V not yet in the cache).  With C =
+ * committed_lengths[r] tokens in the cache, node i is cached at logical
+ * position C + i and has the sequence position C + depth(i).
+ *
+ * mvb_build_draft_tree writes one step's metadata on the device from those
+ * arrays: positions, context_starts (by spec_kind / spec_param, MVB_SPEC_*),
+ * slot_mapping [num_tokens], context_lengths [num_requests] = C + nodes, and
+ * ancestor_mask [num_tokens, mask_words]: bit j % 64 of word j / 64 of node
+ * i's row says that node j is i or an ancestor of i, at a position that i's
+ * window reaches.  Rows that no request owns get 0, 0, -1 and no bit.  A node
+ * past the block table gets slot -1 and sets MVB_STATUS_POSITION_PAST_TABLE;
+ * a request with more than 64 * mask_words nodes, or whose rows or lengths do
+ * not fit, gets padding rows, context length 0 and
+ * MVB_STATUS_INCONSISTENT_COUNTS.  1 <= mask_words <= MVB_MAX_TREE_NODES / 64.
+ */
+MVB_API int mvb_build_draft_tree(const int64_t* parents, const int64_t* query_start_locations,
+                                 const int64_t* committed_lengths, const int64_t* block_table,
+                                 int64_t block_table_row_stride, int64_t block_table_width,
+                                 int64_t num_tokens, int64_t num_requests, int32_t block_size,
+                                 int32_t spec_kind, int64_t spec_param, int32_t mask_words,
+                                 int64_t* positions, int64_t* context_starts,
+                                 int64_t* context_lengths, int64_t* slot_mapping,
+                                 int64_t* ancestor_mask, int32_t* status, void* stream);
+
+/*
+ * Attention of draft trees over the paged cache (no cache write).
+ *
+ * As mvb_paged_attention, but the last nodes(r) = query_start_locations[r+1]
+ * - query_start_locations[r] of a request's context_lengths[r] cached
+ * positions are its drafted nodes.  Node t sees the committed positions
+ *   max(ctx_start[first node of r], ctx_start[t]) .. C - 1
+ * and the drafted nodes whose bit is set in ancestor_mask [num_tokens,
+ * mask_words] (contiguous; bits at or past nodes(r) are ignored).  What a row
+ * does not see does not reach it, infinities and NaN among it.  A row that
+ * sees no key, and rows that no request owns, are written as 0.  A missing
+ * page hides its keys and sets MVB_STATUS_BLOCK_OUT_OF_RANGE.  Requests with
+ * more nodes than mask bits, or a context shorter than their nodes, get 0.
+ * head_dim <= 256.  The workspace (mvb_tree_attention_workspace_size, 256-byte
+ * aligned, no initialisation) belongs to the call until it has run: calls
+ * that may overlap need one each.
+ */
+MVB_API size_t mvb_tree_attention_workspace_size(int64_t max_num_tokens, int64_t max_num_requests,
+                                                 int32_t num_q_heads, int32_t num_kv_heads,
+                                                 int32_t head_dim);
+MVB_API int mvb_tree_attention(const void* query, int64_t query_token_stride,
+                               int64_t query_head_stride, void* output, const void* kv_cache,
+                               int64_t num_blocks, int32_t block_size, int32_t num_kv_heads,
+                               int32_t head_dim, const int64_t* query_context_starts,
+                               const int64_t* query_start_locations,
+                               const int64_t* context_lengths, const int64_t* block_table,
+                               int64_t block_table_row_stride, int64_t block_table_width,
+                               const int64_t* ancestor_mask, int32_t mask_words,
+                               int64_t num_tokens, int64_t num_requests, int32_t num_q_heads,
+                               float scale, int32_t dtype, void* workspace, size_t workspace_bytes,
+                               int32_t* status, void* stream);
+
+/*
+ * The path of each draft tree that the target model keeps.
+ *
+ * target_tokens[t] is the token the target chose at node t (mvb_sample over
+ * every node's logits).  From node 0, which is always kept, the walk goes to
+ * the child whose draft token is the target's token (the lowest index among
+ * equals) until there is none or max_accepted nodes are kept.  Every token
+ * given out was drawn by the target after the tokens before it, so the output
+ * has the target's distribution whatever the draft.  Outputs per request, for
+ * k kept nodes: nodes [num_requests, max_accepted] (indexes inside the
+ * request, -1 behind k), num_accepted = k, tokens [num_requests,
+ * max_accepted] (the target's token at each kept node, -1 behind k),
+ * new_lengths = committed_lengths + k, last_rows = row of the last kept node
+ * (-1 when k = 0: a request without nodes).  1 <= max_accepted <=
+ * MVB_MAX_TREE_NODES.  A request whose rows do not fit keeps nothing and sets
+ * MVB_STATUS_INCONSISTENT_COUNTS.
+ */
+MVB_API int mvb_accept_draft_tree(const int64_t* draft_tokens, const int64_t* target_tokens,
+                                  const int64_t* parents, const int64_t* query_start_locations,
+                                  const int64_t* committed_lengths, int64_t num_tokens,
+                                  int64_t num_requests, int32_t max_accepted, int64_t* nodes,
+                                  int64_t* num_accepted, int64_t* tokens, int64_t* new_lengths,
+                                  int64_t* last_rows, int32_t* status, void* stream);
+
+/*
+ * Moves the kept nodes' K/V rows behind the committed ones, in place and bit
+ * for bit: for every layer cache, plane and k < num_accepted[r], the row at
+ * logical position C + nodes[r, k] goes to C + k.  layer_caches is a host
+ * array of num_layers device pointers, each a kv_cache of these sizes.
+ * nodes[r] must increase (as mvb_accept_draft_tree writes them); a request
+ * whose entries do not, or whose positions or pages are out of range, is left
+ * as it was in every layer and sets a status bit
+ * (MVB_STATUS_INCONSISTENT_COUNTS, _POSITION_PAST_TABLE,
+ * _BLOCK_OUT_OF_RANGE).  No position moved into or from may lie on a page
+ * that two requests of the call share.
+ */
+MVB_API int mvb_compact_draft_kv(void* const* layer_caches, int32_t num_layers, int64_t num_blocks,
+                                 int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+                                 int32_t dtype, const int64_t* block_table,
+                                 int64_t block_table_row_stride, int64_t block_table_width,
+                                 const int64_t* committed_lengths, const int64_t* nodes,
+                                 const int64_t* num_accepted, int64_t num_requests,
+                                 int32_t max_accepted, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -28,6 +28,9 @@ MVB_STATUS_BLOCK_OUT_OF_RANGE = 2
 MVB_STATUS_POSITION_PAST_TABLE = 4
 MVB_STATUS_INCONSISTENT_COUNTS = 8
 MVB_STATUS_WAIT_TIMEOUT = 16
+MVB_STATUS_BAD_PARENT = 32
+
+MVB_MAX_TREE_NODES = 1024
 
 MVB_SPEC_FULL = 0
 MVB_SPEC_SLIDING_WINDOW = 1
@@ -104,6 +107,38 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _I64, _I64, _I64, _I64,  # request / token capacity, table width / stride
             _I32, _I64, _I32, _I64,  # block size, null block, spec kind / param
             _P, _P, _P, _P, _P, _P, _P, _P,  # outputs
+            _P, _P,  # status, stream
+        ],
+    ),
+    "mvb_build_draft_tree": (
+        ctypes.c_int,
+        [
+            _P, _P, _P, _P, _I64, _I64,  # parents, start locations, lengths, table, stride / width
+            _I64, _I64, _I32, _I32, _I64, _I32,  # T, R, block size, spec kind / param, mask words
+            _P, _P, _P, _P, _P,  # outputs
+            _P, _P,  # status, stream
+        ],
+    ),
+    "mvb_tree_attention_workspace_size": (_SZ, [_I64, _I64, _I32, _I32, _I32]),
+    "mvb_tree_attention": (
+        ctypes.c_int,
+        [
+            _P, _I64, _I64, _P,  # query, token stride, head stride, output
+            _P, _I64, _I32, _I32, _I32,  # cache, num_blocks, block_size, Hkv, D
+            _P, _P, _P, _P, _I64, _I64,  # metadata, table stride/width
+            _P, _I32, _I64, _I64, _I32, _F32, _I32,  # mask, words, T, R, Hq, scale, dtype
+            _P, _SZ, _P, _P,  # workspace, bytes, status, stream
+        ],
+    ),
+    "mvb_accept_draft_tree": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _P, _I64, _I64, _I32, _P, _P, _P, _P, _P, _P, _P],
+    ),
+    "mvb_compact_draft_kv": (
+        ctypes.c_int,
+        [
+            _P, _I32, _I64, _I32, _I32, _I32, _I32,  # layer pointers, layers, NB, bs, Hkv, D, dtype
+            _P, _I64, _I64, _P, _P, _P, _I64, _I32,  # table, stride / width, lengths, nodes, kept, R, max
             _P, _P,  # status, stream
         ],
     ),

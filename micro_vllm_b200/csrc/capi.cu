@@ -355,4 +355,185 @@ int mvb_build_metadata(const int32_t* num_computed_tokens, const int32_t* num_sc
   return launch_build_metadata(a);
 }
 
+int mvb_build_draft_tree(const int64_t* parents, const int64_t* query_start_locations,
+                         const int64_t* committed_lengths, const int64_t* block_table,
+                         int64_t block_table_row_stride, int64_t block_table_width,
+                         int64_t num_tokens, int64_t num_requests, int32_t block_size,
+                         int32_t spec_kind, int64_t spec_param, int32_t mask_words,
+                         int64_t* positions, int64_t* context_starts, int64_t* context_lengths,
+                         int64_t* slot_mapping, int64_t* ancestor_mask, int32_t* status,
+                         void* stream) {
+  if (num_tokens < 0 || num_requests < 0 || block_size <= 0 || block_table_width < 0 ||
+      mask_words < 1 || mask_words > kMaxTreeNodes / 64)
+    return MVB_ERR_INVALID_ARGUMENT;
+  if (spec_kind != MVB_SPEC_FULL && spec_kind != MVB_SPEC_SLIDING_WINDOW &&
+      spec_kind != MVB_SPEC_CHUNKED_LOCAL)
+    return MVB_ERR_INVALID_ARGUMENT;
+  if (spec_kind != MVB_SPEC_FULL && spec_param <= 0) return MVB_ERR_INVALID_ARGUMENT;
+  if (num_requests >= 0x7fffffff) return MVB_ERR_UNSUPPORTED_SHAPE;
+  if (num_tokens == 0 && num_requests == 0) return MVB_OK;
+  if (num_tokens > 0 && (!parents || !positions || !context_starts || !slot_mapping || !ancestor_mask))
+    return MVB_ERR_INVALID_ARGUMENT;
+  if (num_requests > 0 && (!query_start_locations || !committed_lengths || !context_lengths ||
+                           (block_table_width > 0 && !block_table)))
+    return MVB_ERR_INVALID_ARGUMENT;
+  DraftTreeArgs a;
+  a.parents = parents;
+  a.qsl = query_start_locations;
+  a.committed = committed_lengths;
+  a.block_table = block_table;
+  a.table_stride = block_table_row_stride;
+  a.table_width = block_table_width;
+  a.num_tokens = num_tokens;
+  a.num_requests = num_requests;
+  a.block_size = block_size;
+  a.spec_kind = spec_kind;
+  a.spec_param = spec_param;
+  a.mask_words = mask_words;
+  a.positions = positions;
+  a.context_starts = context_starts;
+  a.context_lengths = context_lengths;
+  a.slot_mapping = slot_mapping;
+  a.ancestor_mask = ancestor_mask;
+  a.status = status;
+  a.stream = static_cast<cudaStream_t>(stream);
+  return launch_build_draft_tree(a);
+}
+
+size_t mvb_tree_attention_workspace_size(int64_t max_num_tokens, int64_t max_num_requests,
+                                         int32_t num_q_heads, int32_t num_kv_heads,
+                                         int32_t head_dim) {
+  if (max_num_tokens < 0 || max_num_requests < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      head_dim <= 0)
+    return 0;
+  return 256;
+}
+
+int mvb_tree_attention(const void* query, int64_t query_token_stride, int64_t query_head_stride,
+                       void* output, const void* kv_cache, int64_t num_blocks, int32_t block_size,
+                       int32_t num_kv_heads, int32_t head_dim, const int64_t* query_context_starts,
+                       const int64_t* query_start_locations, const int64_t* context_lengths,
+                       const int64_t* block_table, int64_t block_table_row_stride,
+                       int64_t block_table_width, const int64_t* ancestor_mask, int32_t mask_words,
+                       int64_t num_tokens, int64_t num_requests, int32_t num_q_heads, float scale,
+                       int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* status,
+                       void* stream) {
+  if (elem_bytes_of(dtype) == 0) return MVB_ERR_UNSUPPORTED_DTYPE;
+  if (num_tokens < 0 || num_requests < 0 || num_blocks < 0 || block_size <= 0 ||
+      num_kv_heads <= 0 || head_dim <= 0 || num_q_heads <= 0 || block_table_width < 0 ||
+      mask_words < 1 || mask_words > kMaxTreeNodes / 64)
+    return MVB_ERR_INVALID_ARGUMENT;
+  if (num_q_heads % num_kv_heads != 0) return MVB_ERR_UNSUPPORTED_SHAPE;
+  if (num_tokens == 0) return MVB_OK;
+  if (!query || !output || !kv_cache || !query_context_starts || !ancestor_mask ||
+      !query_start_locations ||
+      (num_requests > 0 && (!context_lengths || (block_table_width > 0 && !block_table))))
+    return MVB_ERR_INVALID_ARGUMENT;
+  TreeProblem p{};
+  p.query = query;
+  p.q_st = query_token_stride;
+  p.q_sh = query_head_stride;
+  p.out = output;
+  p.cache = kv_cache;
+  p.num_blocks = num_blocks;
+  p.block_size = block_size;
+  p.num_kv_heads = num_kv_heads;
+  p.head_dim = head_dim;
+  p.qpos = nullptr;  // the mask says what a node sees
+  p.qstart = query_context_starts;
+  p.qsl = query_start_locations;
+  p.ctx_len = context_lengths;
+  p.table = block_table;
+  p.table_stride = block_table_row_stride;
+  p.table_width = block_table_width;
+  p.mask = ancestor_mask;
+  p.mask_words = mask_words;
+  p.num_tokens = num_tokens;
+  p.num_requests = num_requests;
+  p.num_q_heads = num_q_heads;
+  p.scale = scale;
+  p.dtype = dtype;
+  p.workspace = workspace;
+  p.workspace_bytes = workspace_bytes;
+  p.status = status;
+  p.stream = static_cast<cudaStream_t>(stream);
+  return launch_tree_attention_generic(p);
+}
+
+int mvb_accept_draft_tree(const int64_t* draft_tokens, const int64_t* target_tokens,
+                          const int64_t* parents, const int64_t* query_start_locations,
+                          const int64_t* committed_lengths, int64_t num_tokens,
+                          int64_t num_requests, int32_t max_accepted, int64_t* nodes,
+                          int64_t* num_accepted, int64_t* tokens, int64_t* new_lengths,
+                          int64_t* last_rows, int32_t* status, void* stream) {
+  if (num_tokens < 0 || num_requests < 0 || max_accepted < 1 || max_accepted > kMaxTreeNodes)
+    return MVB_ERR_INVALID_ARGUMENT;
+  if (num_requests >= 0x7fffffff) return MVB_ERR_UNSUPPORTED_SHAPE;
+  if (num_requests == 0) return MVB_OK;
+  if (!query_start_locations || !committed_lengths || !nodes || !num_accepted || !tokens ||
+      !new_lengths || !last_rows || (num_tokens > 0 && (!draft_tokens || !target_tokens || !parents)))
+    return MVB_ERR_INVALID_ARGUMENT;
+  AcceptArgs a;
+  a.draft_tokens = draft_tokens;
+  a.target_tokens = target_tokens;
+  a.parents = parents;
+  a.qsl = query_start_locations;
+  a.committed = committed_lengths;
+  a.num_tokens = num_tokens;
+  a.num_requests = num_requests;
+  a.max_accepted = max_accepted;
+  a.nodes = nodes;
+  a.num_accepted = num_accepted;
+  a.tokens = tokens;
+  a.new_lengths = new_lengths;
+  a.last_rows = last_rows;
+  a.status = status;
+  a.stream = static_cast<cudaStream_t>(stream);
+  return launch_accept_draft_tree(a);
+}
+
+int mvb_compact_draft_kv(void* const* layer_caches, int32_t num_layers, int64_t num_blocks,
+                         int32_t block_size, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
+                         const int64_t* block_table, int64_t block_table_row_stride,
+                         int64_t block_table_width, const int64_t* committed_lengths,
+                         const int64_t* nodes, const int64_t* num_accepted, int64_t num_requests,
+                         int32_t max_accepted, int32_t* status, void* stream) {
+  const int eb = elem_bytes_of(dtype);
+  if (eb == 0) return MVB_ERR_UNSUPPORTED_DTYPE;
+  if (num_layers < 0 || num_blocks < 0 || block_size <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+      block_table_width < 0 || num_requests < 0 || max_accepted < 1 || max_accepted > kMaxTreeNodes)
+    return MVB_ERR_INVALID_ARGUMENT;
+  if (num_requests >= 0x7fffffff) return MVB_ERR_UNSUPPORTED_SHAPE;
+  if (num_layers == 0 || num_requests == 0) return MVB_OK;
+  if (!layer_caches || !committed_lengths || !nodes || !num_accepted ||
+      (block_table_width > 0 && !block_table))
+    return MVB_ERR_INVALID_ARGUMENT;
+  for (int32_t i = 0; i < num_layers; ++i)
+    if (!layer_caches[i] || ((uintptr_t)layer_caches[i] % eb) != 0) return MVB_ERR_INVALID_ARGUMENT;
+  for (int32_t first = 0; first < num_layers; first += kMaxCompactLayers) {
+    CompactArgs a;
+    a.num_layers = num_layers - first < kMaxCompactLayers ? num_layers - first : kMaxCompactLayers;
+    bool aligned16 = true;
+    for (int32_t i = 0; i < a.num_layers; ++i) {
+      a.layers[i] = layer_caches[first + i];
+      aligned16 = aligned16 && ((uintptr_t)a.layers[i] % 16) == 0;
+    }
+    a.max_accepted = max_accepted;
+    a.num_blocks = num_blocks;
+    a.block_size = block_size;
+    a.block_table = block_table;
+    a.table_stride = block_table_row_stride;
+    a.table_width = block_table_width;
+    a.committed = committed_lengths;
+    a.nodes = nodes;
+    a.num_accepted = num_accepted;
+    a.num_requests = num_requests;
+    a.status = status;
+    a.stream = static_cast<cudaStream_t>(stream);
+    const int rc = launch_compact_draft_kv(a, (int64_t)num_kv_heads * head_dim * eb, aligned16);
+    if (rc != MVB_OK) return rc;
+  }
+  return MVB_OK;
+}
+
 }  // extern "C"

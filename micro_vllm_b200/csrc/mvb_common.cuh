@@ -58,6 +58,26 @@ __device__ __forceinline__ int64_t find_request(const int64_t* __restrict__ qsl,
   return r;
 }
 
+// The keys of draft-tree request r: committed positions [lo, committed), then
+// drafted nodes [committed, hi).  False for a request that owns no node, or
+// whose ranges or lengths do not fit together (its rows are written as 0).
+struct TreeExtent {
+  int64_t qs, qe, lo, committed, hi;
+};
+template <typename Problem>
+__device__ __forceinline__ bool tree_extent(const Problem& p, int64_t r, TreeExtent& e) {
+  e.qs = __ldg(p.qsl + r);
+  e.qe = __ldg(p.qsl + r + 1);
+  e.hi = __ldg(p.ctx_len + r);
+  const int64_t n = e.qe - e.qs;
+  if (n <= 0 || e.qs < 0 || e.qe > p.num_tokens || n > 64 * (int64_t)p.mask_words || e.hi < n ||
+      e.hi > ((int64_t)1 << 30))
+    return false;
+  e.committed = e.hi - n;
+  e.lo = min(max(__ldg(p.qstart + e.qs), (int64_t)0), e.committed);
+  return true;
+}
+
 // Programmatic dependent launch (sm_90+): a kernel launched with
 // programmatic stream serialization may start while the kernel before it in
 // the stream still runs; grid_dependency_wait() returns once that kernel has

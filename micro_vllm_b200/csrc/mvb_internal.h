@@ -196,6 +196,53 @@ struct MetadataArgs {
 constexpr int64_t kMaxMetadataRequests = 16384;  // shared-memory offsets of every request
 int launch_build_metadata(const MetadataArgs& a);
 
+// Draft trees: the most nodes a request may have (mask words x 64).
+constexpr int kMaxTreeNodes = 1024;
+// Layers one KV-move launch takes (their cache pointers are kernel arguments).
+constexpr int kMaxCompactLayers = 64;
+
+struct DraftTreeArgs {
+  const int64_t *parents, *qsl, *committed, *block_table;
+  int64_t table_stride, table_width, num_tokens, num_requests;
+  int64_t block_size;
+  int32_t spec_kind;
+  int64_t spec_param;
+  int32_t mask_words;
+  int64_t *positions, *context_starts, *context_lengths, *slot_mapping, *ancestor_mask;
+  int32_t* status;
+  cudaStream_t stream;
+};
+int launch_build_draft_tree(const DraftTreeArgs& a);
+
+struct AcceptArgs {
+  const int64_t *draft_tokens, *target_tokens, *parents, *qsl, *committed;
+  int64_t num_tokens, num_requests;
+  int32_t max_accepted;
+  int64_t *nodes, *num_accepted, *tokens, *new_lengths, *last_rows;
+  int32_t* status;
+  cudaStream_t stream;
+};
+int launch_accept_draft_tree(const AcceptArgs& a);
+
+struct CompactArgs {
+  void* layers[kMaxCompactLayers];
+  int32_t num_layers, max_accepted;
+  int64_t num_blocks, block_size, row_vecs;
+  const int64_t *block_table, *committed, *nodes, *num_accepted;
+  int64_t table_stride, table_width, num_requests;
+  int32_t* status;
+  cudaStream_t stream;
+};
+int launch_compact_draft_kv(CompactArgs a, int64_t row_bytes, bool aligned16);
+
+// One draft-tree attention call: a request's last (qsl[r+1] - qsl[r]) cached
+// positions are its drafted nodes, masked by `mask` [token, mask_words].
+struct TreeProblem : AttentionProblem {
+  const int64_t* mask;
+  int32_t mask_words;
+};
+int launch_tree_attention_generic(const TreeProblem& p);
+
 int launch_plan(const AttentionProblem& p, const WorkspaceLayout& w, int32_t group,
                 int32_t decode_ctas, int32_t prefill_block_q);
 int launch_paged_decode(const AttentionProblem& p, const WorkspaceLayout& w, int32_t grid,

@@ -16,6 +16,7 @@ from abc import ABC, abstractmethod
 import torch
 
 from micro_vllm_b200 import _lib
+from micro_vllm_b200.draft_tree import on_device
 
 OPERATOR_NAME = "b200_paged"
 
@@ -223,6 +224,93 @@ class B200PagedAttentionOperator(AttentionOperator):
             torch.cuda.current_stream(device).cuda_stream,
         )
         _lib.check(rc, "b200_paged attention")
+        return output
+
+    # -- draft trees -------------------------------------------------------
+    def forward_tree(self, query, key, value, layer_kv_cache, tree) -> torch.Tensor:
+        """The KV write of a draft-tree step's nodes, then ``attend_tree``."""
+
+        for t in (query, key, value, layer_kv_cache):
+            if t.device.type != "cuda":
+                raise RuntimeError("b200_paged attention requires CUDA tensors")
+        if query.dim() != 3 or layer_kv_cache.dim() != 5:
+            raise ValueError("expected query [T,H,D] and layer_kv_cache [2,NB,bs,Hkv,D]")
+        if not (key.dtype == value.dtype == layer_kv_cache.dtype == query.dtype):
+            raise ValueError("query, key, value and layer_kv_cache must share one dtype")
+        if key.shape != (query.shape[0], layer_kv_cache.shape[3], query.shape[2]) or value.shape != key.shape:
+            raise ValueError("key/value must be [num_tokens, num_kv_heads, head_dim]")
+        if key.device != query.device or value.device != query.device:
+            raise ValueError("query, key, value and layer_kv_cache must be on one device")
+        self._check_tree(query, layer_kv_cache, tree)
+        with on_device(query.device):
+            write_kv_cache(key, value, layer_kv_cache, tree.attention)
+        return self.attend_tree(query, layer_kv_cache, tree)
+
+    def _check_tree(self, query, layer_kv_cache, tree) -> int:
+        """Checks that the cache and the tree fit the query; the MVB_DTYPE_*."""
+
+        if query.device.type != "cuda" or layer_kv_cache.device.type != "cuda":
+            raise RuntimeError("b200_paged attention requires CUDA tensors")
+        dtype = _DTYPES.get(query.dtype)
+        if dtype is None or layer_kv_cache.dtype != query.dtype:
+            raise ValueError("query and layer_kv_cache must share a float16/bfloat16/float32 dtype")
+        if query.dim() != 3 or layer_kv_cache.dim() != 5 or not layer_kv_cache.is_contiguous():
+            raise ValueError("expected query [T,H,D] and a contiguous layer_kv_cache [2,NB,bs,Hkv,D]")
+        planes, _, block_size, num_kv_heads, head_dim = layer_kv_cache.shape
+        if planes != 2 or head_dim != query.shape[2] or block_size != tree.attention.block_size:
+            raise ValueError("layer_kv_cache does not match the query / metadata")
+        if num_kv_heads == 0 or query.shape[1] % num_kv_heads != 0:
+            raise ValueError("num_q_heads must be a multiple of num_kv_heads")
+        if layer_kv_cache.device != query.device:
+            raise ValueError("query and layer_kv_cache must be on one device")
+        mask = tree.ancestor_mask
+        if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != query.shape[0] \
+                or not 1 <= mask.shape[1] <= _lib.MVB_MAX_TREE_NODES // 64 or mask.device != query.device:
+            raise ValueError("ancestor_mask must be torch.int64 [num_tokens, words] on the query's device")
+        return dtype
+
+    def attend_tree(self, query, layer_kv_cache, tree) -> torch.Tensor:
+        """Attention of draft trees (``build_draft_tree``) over a cache that
+        holds their keys and values: each node sees its request's committed
+        positions (inside its window) and its own ancestors.  A row that sees
+        nothing is 0.  The workspace is allocated per call from the caching
+        allocator, so calls on several streams, and several captured graphs,
+        have one each."""
+
+        dtype = self._check_tree(query, layer_kv_cache, tree)
+        num_tokens, num_q_heads, head_dim = query.shape
+        _, num_blocks, block_size, num_kv_heads, _ = layer_kv_cache.shape
+        device = query.device
+        if query.stride(2) != 1:
+            query = query.contiguous()
+        md, mask = tree.attention, tree.ancestor_mask
+        if not mask.is_contiguous():
+            mask = mask.contiguous()
+        md_start = _meta(md.query_context_start_positions, device, "query_context_start_positions")
+        md_qsl = _meta(md.query_start_locations, device, "query_start_locations")
+        md_ctx = _meta(md.context_lengths, device, "context_lengths")
+        table = md.block_table
+        num_requests = md_ctx.numel()
+        if table.dtype != torch.int64 or table.device != device or table.dim() != 2 or table.shape[0] != num_requests:
+            raise ValueError("metadata.block_table must be torch.int64 [num_requests, width] on the query's device")
+        if md_start.numel() != num_tokens or md_qsl.numel() != num_requests + 1:
+            raise ValueError("metadata does not match the query")
+        if table.shape[1] > 1 and table.stride(1) != 1:
+            table = table.contiguous()
+        output = torch.empty((num_tokens, num_q_heads, head_dim), dtype=query.dtype, device=device)
+        nbytes = self._lib.mvb_tree_attention_workspace_size(num_tokens, num_requests, num_q_heads, num_kv_heads, head_dim)
+        with on_device(device):
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            rc = self._lib.mvb_tree_attention(
+                query.data_ptr(), query.stride(0), query.stride(1), output.data_ptr(),
+                layer_kv_cache.data_ptr(), num_blocks, block_size, num_kv_heads, head_dim,
+                md_start.data_ptr(), md_qsl.data_ptr(), md_ctx.data_ptr(),
+                table.data_ptr(), table.stride(0), table.shape[1], mask.data_ptr(), mask.shape[1],
+                num_tokens, num_requests, num_q_heads, 1.0 / math.sqrt(head_dim), dtype,
+                workspace.data_ptr(), nbytes, self._state(device).status.data_ptr(),
+                torch.cuda.current_stream(device).cuda_stream,
+            )
+        _lib.check(rc, "b200_paged tree attention")
         return output
 
 
