@@ -406,7 +406,7 @@ size_t mvb_tree_attention_workspace_size(int64_t max_num_tokens, int64_t max_num
   if (max_num_tokens < 0 || max_num_requests < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
       head_dim <= 0)
     return 0;
-  return 256;
+  return head_dim == 128 ? tree_workspace_bytes() : 256;
 }
 
 int mvb_tree_attention(const void* query, int64_t query_token_stride, int64_t query_head_stride,
@@ -457,7 +457,7 @@ int mvb_tree_attention(const void* query, int64_t query_token_stride, int64_t qu
   p.workspace_bytes = workspace_bytes;
   p.status = status;
   p.stream = static_cast<cudaStream_t>(stream);
-  return launch_tree_attention_generic(p);
+  return tree_tc_supported(p) ? launch_tree_attention(p) : launch_tree_attention_generic(p);
 }
 
 int mvb_accept_draft_tree(const int64_t* draft_tokens, const int64_t* target_tokens,

@@ -242,6 +242,12 @@ struct TreeProblem : AttentionProblem {
   int32_t mask_words;
 };
 int launch_tree_attention_generic(const TreeProblem& p);
+// The tensor-core kernel: CTAs at most (one per SM; they size its workspace),
+// what it takes, and its launch.
+constexpr int kMaxTreeCtas = 160;
+size_t tree_workspace_bytes();
+bool tree_tc_supported(const TreeProblem& p);
+int launch_tree_attention(const TreeProblem& p);
 
 int launch_plan(const AttentionProblem& p, const WorkspaceLayout& w, int32_t group,
                 int32_t decode_ctas, int32_t prefill_block_q);

@@ -1,0 +1,1217 @@
+// Attention of draft trees over the paged cache on the 5th-generation tensor
+// cores (tcgen05 + TMEM), head_dim 128, fp16/bf16.
+//
+// Mathematics.  Row (node t, query head) of request r sees the committed keys
+// max(ctx_start[first], ctx_start[t]) .. C - 1 and the drafted keys C + j
+// whose ancestor bit j is set.  Softmax is the online form: a reference m, a
+// sum l and an unnormalised O, each in fp32, so segments of the key axis
+// merge exactly.
+//
+// What bounds it.  A tree of n nodes reads every committed K/V row once per
+// KV head for n x G query rows: below about 240 rows (the machine's balance
+// of bf16 operations and bytes) the time is the HBM read.
+//
+// Split.  An item is (request, KV head, up to two 128-row query tiles); its
+// key axis is cut into 128-key tiles.  All tiles of all items lie on one cost
+// axis (kTileCost per tile, kItemCost per item), of which each CTA takes an
+// equal share, so the bytes are balanced whatever the lengths, and one long
+// request spreads over the whole GPU.  Every CTA sums the costs itself from
+// the metadata (a few KB): no planning launch, no host round trip.  An item
+// cut by share borders leaves fp32 partials (at most a head and a tail per
+// CTA), which the merge launch behind joins in a fixed order.
+//
+// Inside a CTA (12 warps, roles without a block-wide barrier between items):
+//   warp 11   scheduler: describes the next item in a 2-slot ring, loads its Q
+//   warps 8, 10  TMA producers of K (2 stages) and V (3 stages)
+//   warp 9    MMA issuer
+//   warps 0-3, 4-7  softmax of stream 0 and 1, one thread per row
+// The two streams each own S/P and O columns in TMEM.  With two query tiles
+// (more than 128 rows) a stream is a query tile and both read every K/V tile.
+// With one, both streams hold the same query tile and take the even and the
+// odd key tiles: one stream's softmax runs under the other's MMAs, which a
+// single tile could not overlap, and the streams' (m, l, O) merge in the
+// epilogue, each warpgroup normalising half of the columns.
+//
+// Rows of V that a query row does not see but another row does (other
+// branches, window edges) may hold infinities or NaN, and 0 x NaN would reach
+// O.  The V producer replaces the non-finite elements of those rows by 0 in
+// shared memory; where it found any, the epilogue adds the seen ones back.
+// Every mbarrier wait is bounded; a timeout sets kStatusWaitTimeout.
+#include <math.h>
+
+#include <mutex>
+#include <type_traits>
+
+#include "mvb_common.cuh"
+#include "mvb_internal.h"
+#include "ptx_sm100.cuh"
+
+namespace mvb {
+namespace {
+
+using namespace sm100;
+
+constexpr int kRows = 128;                 // MMA M: rows of one query tile
+constexpr int kKeys = 128;                 // keys per KV tile
+constexpr int kHalf = kRows * 128;         // [128 rows][64 elements] swizzled: 16 KiB
+constexpr int kTileBytes = 2 * kHalf;      // [128][128] 16-bit
+constexpr int kKStages = 2, kVStages = 3, kQStages = 2;
+constexpr int kOffQ = 0;
+constexpr int kOffK = kQStages * kTileBytes;
+constexpr int kOffV = kOffK + kKStages * kTileBytes;
+constexpr int kSmemBytes = kOffV + kVStages * kTileBytes;  // 224 KiB of the SM's 227
+constexpr int kThreads = 384;
+constexpr int kKProdWarp = 8, kMmaWarp = 9, kSchedWarp = 11;  // warp 10: V producer
+constexpr int kItemSlots = 2;
+constexpr int kItemReaders = 11;
+constexpr int kFlagSlots = 8;  // items whose V flag may still be read: V runs at most 3 tiles ahead
+// Register split (setmaxnreg): 2 x 128 x 200 + 128 x 96 <= 384 x 168.
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 200, kOtherRegs = 96;
+static_assert(2 * 128 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs,
+              "register split must fit the launch's registers");
+constexpr uint32_t kTmemCols = 512;
+__device__ __forceinline__ uint32_t col_s(int x) { return 128u * (uint32_t)x; }
+__device__ __forceinline__ uint32_t col_o(int x) { return 256u + 128u * (uint32_t)x; }
+constexpr float kRescaleLog2 = 8.f;
+
+// Cost axis: a KV tile of an item with one or two query tiles, an item's
+// fixed part, and the least share of a CTA.
+constexpr int kTileCost1 = 4, kTileCost2 = 6, kItemCost = 4, kMinShare = 8;
+
+constexpr int kPartRows = 2 * kRows;  // rows of one partial
+
+enum Bar : int {
+  kQFull = 0,
+  kQEmpty = kQFull + kQStages,
+  kKFull = kQEmpty + kQStages,
+  kKEmpty = kKFull + kKStages,
+  kVFull = kKEmpty + kKStages,
+  kVEmpty = kVFull + kVStages,
+  kVReady = kVEmpty + kVStages,
+  kSFull = kVReady + kVStages,   // +stream
+  kPFull = kSFull + 2,           // +stream
+  kPvDone = kPFull + 2,          // +stream
+  kMl = kPvDone + 2,             // +stream: its (m, l) are in shared memory
+  kORead = kMl + 2,              // +stream: the other warpgroup has read its O
+  kItemFull = kORead + 2,
+  kItemEmpty = kItemFull + kItemSlots,
+  kFinal = kItemEmpty + kItemSlots,
+  kNumBars = kFinal + 1,
+};
+
+struct ItemDesc {
+  int64_t q0, qe;       // first token of the item, end of the request's tokens
+  int32_t r, h;         // request (-1: no more items), KV head
+  int32_t n;            // KV tiles of this segment
+  int32_t kbase;        // first key of the segment's first tile
+  int32_t kv_lo, kv_hi; // keys any row may see: [kv_lo, kv_hi)
+  int32_t committed;    // C: first drafted key
+  int32_t lo_all;       // every row of the item sees committed keys from here
+  int32_t two;          // two query tiles
+  int32_t slot;         // partial slot, or -1: the whole item is this segment
+  int32_t first, last;  // the segment holds the request's first / last tile
+};
+
+// What the merge needs of the item that a CTA starts and does not finish.
+struct CutRecord {
+  int64_t q0, qe, cost0;  // first token, end of tokens, place on the cost axis
+  int64_t share;
+  int32_t h, tiles, tile_cost, valid;
+};
+
+struct TreeParams {
+  char* out;
+  int32_t num_q_heads, num_kv_heads, group, block_q, block_size, bs_shift, box_rows, boxes;
+  int64_t num_blocks, num_slots;
+  const int64_t *qstart, *qsl, *ctx_len, *table;
+  int64_t table_stride, table_width;
+  const int64_t* mask;
+  int32_t mask_words;
+  int64_t num_tokens, num_requests;
+  float scale_log2;
+  float4* part_o;    // [CTA][2][32 column chunks][kPartRows]
+  float2* part_ml;   // [CTA][2][kPartRows]
+  CutRecord* cuts;   // [CTA]
+  const char* cache;
+  int32_t* status;
+};
+
+__device__ __forceinline__ int64_t page_of(const TreeParams& p, const int64_t* trow, int64_t pos) {
+  const int64_t lb = p.bs_shift >= 0 ? (pos >> p.bs_shift) : pos / p.block_size;
+  if (pos < 0 || lb >= p.table_width) return -1;
+  const int64_t blk = __ldg(trow + lb);
+  return (blk >= 0 && blk < p.num_blocks) ? blk : -1;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// Bit 15 / 31 of the result: that 16-bit element's exponent is all ones.
+template <typename T>
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t v) {
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  return ((v & 0x7fff7fffu) + (kBf16 ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+}
+
+// A request's place on the cost axis.
+struct RequestCost {
+  int32_t pairs, tiles, kbase;
+  int64_t full, last, head;  // cost of an item with two query tiles, of the last item, of a KV head
+};
+__device__ __forceinline__ RequestCost cost_of(const TreeParams& p, const TreeExtent& e) {
+  RequestCost c;
+  const int32_t n = (int32_t)(e.qe - e.qs), two = 2 * p.block_q;
+  c.pairs = (n + two - 1) / two;
+  c.kbase = (int32_t)e.lo & ~(p.box_rows - 1);
+  c.tiles = ((int32_t)e.hi - c.kbase + kKeys - 1) / kKeys;
+  c.full = kItemCost + (int64_t)c.tiles * kTileCost2;
+  const bool one = n - (c.pairs - 1) * two <= p.block_q;
+  c.last = one ? kItemCost + (int64_t)c.tiles * kTileCost1 : c.full;
+  c.head = (c.pairs - 1) * c.full + c.last;
+  return c;
+}
+// First tile of an item at or behind cost position x (item at cost0).
+__host__ __device__ __forceinline__ int32_t tile_at(int64_t x, int64_t cost0, int32_t tile_cost,
+                                                    int32_t tiles) {
+  const int64_t d = x - cost0 - kItemCost;
+  const int64_t j = d <= 0 ? 0 : (d + tile_cost - 1) / tile_cost;
+  return (int32_t)(j < tiles ? j : tiles);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    tree_attention_kernel(const __grid_constant__ CUtensorMap qmap,
+                          const __grid_constant__ CUtensorMap kvmap, const TreeParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ __align__(8) uint64_t bars[kNumBars];
+  __shared__ __align__(16) ItemDesc items[kItemSlots];
+  __shared__ float2 ml_sh[2][kRows];
+  __shared__ int64_t warp_sum_sh[kThreads / 32];
+  __shared__ int64_t start_prefix_sh;
+  __shared__ int32_t start_request_sh;
+  __shared__ int32_t bad_v_sh[kFlagSlots];
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ int32_t abort_sh;
+  __shared__ int32_t last_issued[2];
+  __shared__ int32_t q_issued;
+
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  allow_dependent_launch();  // the merge waits for this grid's end before it reads
+
+  // ---- this CTA's share of the cost axis ----
+  const int64_t per = (p.num_requests + kThreads - 1) / kThreads;
+  const int64_t r_lo = min(tid * per, p.num_requests), r_hi = min(r_lo + per, p.num_requests);
+  int64_t mine = 0;
+  for (int64_t r = r_lo; r < r_hi; ++r) {
+    TreeExtent e;
+    if (tree_extent(p, r, e)) mine += cost_of(p, e).head * p.num_kv_heads;
+  }
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += u;
+  }
+  if (lane == 31) warp_sum_sh[warp] = incl;
+  if (tid == 0) p.cuts[blockIdx.x].valid = 0;
+  __syncthreads();
+  int64_t before = incl - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    const int64_t v = warp_sum_sh[w];
+    if (w < warp) before += v;
+    total += v;
+  }
+  const int64_t share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kMinShare);
+  const int64_t my_lo = blockIdx.x * share, my_hi = min(my_lo + share, total);
+  if (my_lo >= total) return;
+  if (before <= my_lo && my_lo < before + mine) {
+    int64_t r = r_lo, at = before;
+    for (;; ++r) {
+      TreeExtent e;
+      const int64_t c = tree_extent(p, r, e) ? cost_of(p, e).head * p.num_kv_heads : 0;
+      if (my_lo < at + c) break;
+      at += c;
+    }
+    start_request_sh = (int32_t)r;
+    start_prefix_sh = at;
+  }
+
+  const uint32_t sb = smem_addr(smem);
+  if ((sb & 1023u) != 0) {  // the swizzle needs the declared alignment
+    if (tid == 0 && p.status != nullptr) atomicOr(p.status, kStatusWaitTimeout);
+    return;
+  }
+  const uint32_t bar0 = smem_addr(&bars[0]);
+  auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
+  volatile int32_t* abort_flag = &abort_sh;
+
+  if (tid == 0) {
+    for (int i = 0; i < kNumBars; ++i) {
+      const bool four = (i >= kPFull && i < kPFull + 2) || (i >= kMl && i < kORead + 2);
+      const bool readers = i >= kItemEmpty && i < kItemEmpty + kItemSlots;
+      mbar_init(bar(i), readers ? kItemReaders : four ? 4 : 1);
+    }
+    mbar_init_fence();
+    abort_sh = 0;
+    last_issued[0] = last_issued[1] = -1;
+    q_issued = 0;
+  }
+  if (warp == kMmaWarp) tmem_alloc(smem_addr(&tmem_base_sh), kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_sh;
+
+  auto take_item = [&](uint32_t i, ItemDesc& d) -> bool {
+    const uint32_t slot = i % kItemSlots;
+    if (!__all_sync(0xffffffffu, mbar_wait(bar(kItemFull + slot), (i / kItemSlots) & 1)))
+      return false;
+    d = items[slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(kItemEmpty + slot));
+    return true;
+  };
+  // KV tiles of stream x in an item of n tiles: all of them for a query tile
+  // of its own, else every other one.
+  auto stream_tiles = [](const ItemDesc& d, int x) { return d.two ? d.n : (d.n + 1 - x) >> 1; };
+  // Running counts (identical in every role): KV tiles of this CTA, tiles per
+  // stream, Q tiles, items with one query tile.
+  uint32_t kvc = 0, tc0 = 0, tc1 = 0, qc = 0, mc = 0;
+  auto advance = [&](const ItemDesc& d) {
+    kvc += (uint32_t)d.n;
+    tc0 += (uint32_t)stream_tiles(d, 0);
+    tc1 += (uint32_t)stream_tiles(d, 1);
+    qc += d.two ? 2 : 1;
+    mc += d.two ? 0 : 1;
+  };
+  auto fail = [&]() {
+    if (lane == 0) atomicOr(&abort_sh, 1);
+  };
+  auto kslot = [](uint32_t c) { return c % kKStages; };
+  auto kphase = [](uint32_t c) { return (c / kKStages) & 1; };
+  auto vslot = [](uint32_t c) { return c % kVStages; };
+  auto vphase = [](uint32_t c) { return (c / kVStages) & 1; };
+
+  if (warp >= kKProdWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
+    if (warp == kSchedWarp) {
+      // ---------------------------------------------------- scheduler
+      const uint32_t q_bytes = (uint32_t)(p.group * p.block_q) * 128u * 2u;
+      int64_t r = start_request_sh, at = start_prefix_sh;  // request and its cost position
+      int64_t batch = r;                                   // lane l holds request batch + l
+      TreeExtent mine_e;
+      bool mine_ok = batch + lane < p.num_requests && tree_extent(p, batch + lane, mine_e);
+      int32_t h = 0, pair = 0;
+      int64_t cost0 = at;  // of item (r, h, pair)
+      bool fresh = true;   // the request's figures are not yet read
+      TreeExtent e{};
+      RequestCost rc{};
+      CutRecord cut{};
+      bool ok = true;
+      for (uint32_t i = 0; ok; ++i) {
+        // The next item with tiles in this share.
+        ItemDesc d;
+        d.r = -1;
+        while (*abort_flag == 0) {
+          if (fresh) {
+            if (cost0 >= my_hi || r >= p.num_requests) break;
+            if (r >= batch + 32) {
+              batch = r;
+              mine_ok = batch + lane < p.num_requests && tree_extent(p, batch + lane, mine_e);
+            }
+            const int src = (int)(r - batch);
+            if (!__shfl_sync(0xffffffffu, mine_ok ? 1 : 0, src)) {
+              ++r;
+              continue;
+            }
+            e.qs = __shfl_sync(0xffffffffu, mine_e.qs, src);
+            e.qe = __shfl_sync(0xffffffffu, mine_e.qe, src);
+            e.lo = __shfl_sync(0xffffffffu, mine_e.lo, src);
+            e.committed = __shfl_sync(0xffffffffu, mine_e.committed, src);
+            e.hi = __shfl_sync(0xffffffffu, mine_e.hi, src);
+            rc = cost_of(p, e);
+            h = pair = 0;
+            if (cost0 < my_lo) {  // the share begins inside this request
+              const int64_t in = my_lo - cost0;
+              h = (int32_t)(in / rc.head);
+              pair = (int32_t)min((in - h * rc.head) / rc.full, (int64_t)(rc.pairs - 1));
+              cost0 += h * rc.head + pair * rc.full;
+            }
+            fresh = false;
+          }
+          if (cost0 >= my_hi) break;
+          const bool last_pair = pair == rc.pairs - 1;
+          const int64_t cost = last_pair ? rc.last : rc.full;
+          d.q0 = e.qs + (int64_t)pair * 2 * p.block_q;
+          d.two = d.q0 + p.block_q < e.qe ? 1 : 0;
+          const int32_t tile_cost = d.two ? kTileCost2 : kTileCost1;
+          const int32_t j0 = tile_at(my_lo, cost0, tile_cost, rc.tiles);
+          const int32_t j1 = tile_at(my_hi, cost0, tile_cost, rc.tiles);
+          const bool some = j1 > j0;
+          if (some) {
+            d.r = (int32_t)r;
+            d.h = h;
+            d.qe = e.qe;
+            d.n = j1 - j0;
+            d.kbase = rc.kbase + j0 * kKeys;
+            d.kv_lo = (int32_t)e.lo;
+            d.kv_hi = (int32_t)e.hi;
+            d.committed = (int32_t)e.committed;
+            d.first = j0 == 0;
+            d.last = j1 == rc.tiles;
+            d.slot = d.first && d.last ? -1 : d.first ? 1 : 0;
+            if (d.first && !d.last) cut = {d.q0, e.qe, cost0, share, h, rc.tiles, tile_cost, 1};
+          }
+          cost0 += cost;
+          if (!last_pair) {
+            ++pair;
+          } else {
+            pair = 0;
+            if (++h == p.num_kv_heads) {
+              ++r;
+              fresh = true;
+            }
+          }
+          if (some) break;
+        }
+        if (d.r >= 0) {
+          // Committed keys that every row of the item sees start here.
+          int32_t hi_start = d.kv_lo;
+          const int64_t tend = min(d.q0 + 2 * (int64_t)p.block_q, d.qe);
+          for (int64_t t = d.q0 + lane; t < tend; t += 32)
+            hi_start = max(hi_start, (int32_t)min(max(__ldg(p.qstart + t), (int64_t)0), (int64_t)d.committed));
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1)
+            hi_start = max(hi_start, __shfl_xor_sync(0xffffffffu, hi_start, o));
+          d.lo_all = hi_start;
+        }
+        const uint32_t slot = i % kItemSlots;
+        if (!__all_sync(0xffffffffu,
+                        mbar_wait(bar(kItemEmpty + slot), ((i / kItemSlots) & 1) ^ 1))) {
+          fail();
+          break;
+        }
+        if (lane == 0) {
+          items[slot] = d;
+          mbar_arrive(bar(kItemFull + slot));
+        }
+        __syncwarp();
+        if (d.r < 0) break;
+        if (lane == 0) {
+          const int qn = d.two ? 2 : 1;
+          for (int t = 0; ok && t < qn; ++t) {
+            const uint32_t c = qc + (uint32_t)t, qs = c % kQStages;
+            if (!mbar_wait(bar(kQEmpty + qs), ((c / kQStages) & 1) ^ 1)) {
+              ok = false;
+              break;
+            }
+            mbar_expect_tx(bar(kQFull + qs), q_bytes);
+            const int32_t qy = d.h * p.group, qz = (int32_t)(d.q0 + (int64_t)t * p.block_q);
+            tma_load_3d(sb + kOffQ + qs * kTileBytes, &qmap, 0, qy, qz, bar(kQFull + qs));
+            tma_load_3d(sb + kOffQ + qs * kTileBytes + kHalf, &qmap, 64, qy, qz, bar(kQFull + qs));
+            q_issued = (int32_t)c + 1;
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        if (!ok) fail();
+        advance(d);
+      }
+      if (lane == 0 && cut.valid) p.cuts[blockIdx.x] = cut;
+    } else if (warp == kMmaWarp) {
+      // ---------------------------------------------------- MMA issuer
+      if (lane == 0) {
+        const uint32_t idesc_qk = f16_idesc(kBf16, false, kRows, kKeys);
+        const uint32_t idesc_pv = f16_idesc(kBf16, true, kRows, 128);
+        const uint64_t dq0 = sw128_desc(sb + kOffQ, 16, 1024);
+        const uint64_t dk0 = sw128_desc(sb + kOffK, 16, 1024);
+        const uint64_t dv0 = sw128_desc(sb + kOffV, kHalf, 1024);
+        auto issue_s = [&](int x, uint32_t qs, uint32_t stage) {
+          const uint64_t dq = dq0 + (uint64_t)((qs * kTileBytes) >> 4);
+          const uint64_t dk = dk0 + (uint64_t)((stage * kTileBytes) >> 4);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t step = (uint32_t)((k >> 2) * (kHalf >> 4) + 2 * (k & 3));
+            umma_f16(tmem + col_s(x), dq + step, dk + step, idesc_qk, k > 0);
+          }
+          umma_commit(bar(kSFull + x));
+        };
+        auto issue_pv = [&](int x, uint32_t stage, bool acc) {
+          const uint64_t dv = dv0 + (uint64_t)((stage * kTileBytes) >> 4);
+#pragma unroll
+          for (int part = 0; part < (kBf16 ? 2 : 1); ++part) {  // P_hi (+ P_lo in bf16)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint32_t pcol = 32 * (k >> 1) + 8 * (k & 1) + 16 * part;
+              umma_f16_ts(tmem + col_o(x), tmem + col_s(x) + pcol, dv + (uint64_t)(k * (2048 >> 4)),
+                          idesc_pv, acc || k > 0 || part > 0);
+            }
+          }
+          umma_commit(bar(kPvDone + x));
+        };
+        bool ok = true;
+        for (uint32_t i = 0; ok; ++i) {
+          const uint32_t slot = i % kItemSlots;
+          if (!mbar_wait(bar(kItemFull + slot), (i / kItemSlots) & 1)) {
+            ok = false;
+            break;
+          }
+          const ItemDesc d = items[slot];
+          mbar_arrive(bar(kItemEmpty + slot));
+          if (d.r < 0 || *abort_flag != 0) break;
+          const int n = d.n;
+          const uint32_t qs0 = qc % kQStages, qs1 = (qc + 1) % kQStages;
+          ok = mbar_wait(bar(kQFull + qs0), (qc / kQStages) & 1) &&
+               mbar_wait(bar(kKFull + kslot(kvc)), kphase(kvc));
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(0, qs0, kslot(kvc));
+          if (d.two) {
+            ok = mbar_wait(bar(kQFull + qs1), ((qc + 1) / kQStages) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            issue_s(1, qs1, kslot(kvc));
+            umma_commit(bar(kKEmpty + kslot(kvc)));
+            if (n == 1) {
+              umma_commit(bar(kQEmpty + qs0));
+              umma_commit(bar(kQEmpty + qs1));
+            }
+            for (int j = 0; ok && j < n; ++j) {
+              const uint32_t c = kvc + j;
+              for (int x = 0; x < 2; ++x) {
+                ok = mbar_wait(bar(kPFull + x), ((x == 0 ? tc0 : tc1) + j) & 1) &&
+                     (x == 1 || mbar_wait(bar(kVReady + vslot(c)), vphase(c)));
+                if (!ok) break;
+                tc_fence_after();
+                issue_pv(x, vslot(c), j > 0);
+                if (x == 1) umma_commit(bar(kVEmpty + vslot(c)));
+                if (j + 1 < n) {
+                  if (x == 0) {
+                    ok = mbar_wait(bar(kKFull + kslot(c + 1)), kphase(c + 1));
+                    if (!ok) break;
+                    tc_fence_after();
+                  }
+                  issue_s(x, x == 0 ? qs0 : qs1, kslot(c + 1));
+                  if (x == 1) umma_commit(bar(kKEmpty + kslot(c + 1)));
+                  if (j + 2 == n) umma_commit(bar(kQEmpty + (x == 0 ? qs0 : qs1)));
+                }
+              }
+            }
+          } else {
+            umma_commit(bar(kKEmpty + kslot(kvc)));
+            if (n > 1) {
+              ok = mbar_wait(bar(kKFull + kslot(kvc + 1)), kphase(kvc + 1));
+              if (!ok) break;
+              tc_fence_after();
+              issue_s(1, qs0, kslot(kvc + 1));
+              umma_commit(bar(kKEmpty + kslot(kvc + 1)));
+            }
+            if (n <= 2) umma_commit(bar(kQEmpty + qs0));
+            for (int j = 0; ok && j < n; ++j) {
+              const uint32_t c = kvc + j;
+              const int x = j & 1;
+              ok = mbar_wait(bar(kPFull + x), ((x == 0 ? tc0 : tc1) + (j >> 1)) & 1) &&
+                   mbar_wait(bar(kVReady + vslot(c)), vphase(c));
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv(x, vslot(c), j > 1);
+              umma_commit(bar(kVEmpty + vslot(c)));
+              if (j + 2 < n) {
+                ok = mbar_wait(bar(kKFull + kslot(c + 2)), kphase(c + 2));
+                if (!ok) break;
+                tc_fence_after();
+                issue_s(x, qs0, kslot(c + 2));
+                umma_commit(bar(kKEmpty + kslot(c + 2)));
+                if (j + 3 == n) umma_commit(bar(kQEmpty + qs0));
+              }
+            }
+          }
+          if (!ok) break;
+          advance(d);
+        }
+        if (!ok) atomicOr(&abort_sh, 1);
+      }
+      __syncwarp();
+    } else {
+      // ---------------------------------------------------- producers
+      const bool is_k = warp == kKProdWarp;
+      for (uint32_t i = 0;; ++i) {
+        ItemDesc d;
+        if (!take_item(i, d)) {
+          fail();
+          break;
+        }
+        if (d.r < 0 || *abort_flag != 0) break;
+        const int64_t* trow = p.table + (int64_t)d.r * p.table_stride;
+        bool ok = true;
+        uint32_t bad_v = 0;  // this lane replaced a non-finite element
+        for (int j = 0; ok && j < d.n; ++j) {
+          const uint32_t c = kvc + j;
+          const uint32_t s = is_k ? kslot(c) : vslot(c);
+          const uint32_t full = bar((is_k ? kKFull : kVFull) + s);
+          const int32_t k0 = d.kbase + j * kKeys;
+          const int64_t pos = (int64_t)k0 + p.box_rows * lane;
+          int64_t blk = -1;
+          if (lane < p.boxes) blk = page_of(p, trow, pos);
+          if (!__all_sync(0xffffffffu, mbar_wait(bar((is_k ? kKEmpty : kVEmpty) + s),
+                                                 (is_k ? kphase(c) : vphase(c)) ^ 1))) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) {
+            last_issued[is_k ? 0 : 1] = (int32_t)c;
+            mbar_expect_tx(full, kTileBytes);
+          }
+          __syncwarp();
+          if (lane < p.boxes) {
+            // Missing pages load page 0; the softmax masks their keys.
+            const int64_t page = blk >= 0 ? blk : 0;
+            const int64_t off = p.bs_shift >= 0 ? (pos & (p.block_size - 1)) : pos % p.block_size;
+            const int32_t y = (int32_t)(page * p.block_size + off) + (is_k ? 0 : (int32_t)p.num_slots);
+            const uint32_t dst = sb + (is_k ? kOffK : kOffV) + s * kTileBytes + lane * p.box_rows * 128;
+            tma_load_2d(dst, &kvmap, d.h * 128, y, full);
+            tma_load_2d(dst + kHalf, &kvmap, d.h * 128 + 64, y, full);
+            if (is_k && blk < 0 && pos < d.kv_hi && pos + p.box_rows > d.kv_lo && p.status != nullptr)
+              atomicOr(p.status, MVB_STATUS_BLOCK_OUT_OF_RANGE);
+          }
+          if (is_k) continue;
+          // Rows that some query row does not see: behind the last key,
+          // before the first, on missing pages (all zeroed), and those that
+          // only some rows see (their non-finite elements).
+          const uint32_t boxes_ok = __ballot_sync(0xffffffffu, lane < p.boxes && blk >= 0);
+          const bool all_pages = boxes_ok == (1u << p.boxes) - 1u;
+          const bool last = j == d.n - 1;
+          if (k0 < d.lo_all || k0 + kKeys > d.committed || k0 < d.kv_lo || !all_pages) {
+            if (!__all_sync(0xffffffffu, mbar_wait(full, vphase(c)))) {
+              ok = false;
+              break;
+            }
+            uint8_t* vt = smem + kOffV + s * kTileBytes;
+#pragma unroll 4
+            for (int it = 0; it < 32; ++it) {
+              const int row = 4 * it + (lane >> 3);
+              const int32_t key = k0 + row;
+              uint4* cell = reinterpret_cast<uint4*>(vt + row * 128 + (lane & 7) * 16);
+              if (key < d.kv_lo || key >= d.kv_hi || !((boxes_ok >> (row / p.box_rows)) & 1u)) {
+                cell[0] = make_uint4(0, 0, 0, 0);
+                cell[kHalf / 16] = make_uint4(0, 0, 0, 0);
+              } else if (key < d.lo_all || key >= d.committed) {
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                  uint4 v = cell[hf * (kHalf / 16)];
+                  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+                  uint32_t any = 0;
+#pragma unroll
+                  for (int q = 0; q < 4; ++q) {
+                    const uint32_t b = nonfinite2<T>(w[q]);
+                    any |= b;
+                    w[q] &= ~((b >> 15) * 0xffffu);
+                  }
+                  if (any) {
+                    cell[hf * (kHalf / 16)] = v;
+                    bad_v = 1;
+                  }
+                }
+              }
+            }
+            fence_proxy_async();  // visible to the P.V MMAs
+            if (last) bad_v = __any_sync(0xffffffffu, bad_v) ? 1 : 0;
+            if (last && lane == 0) bad_v_sh[i % kFlagSlots] = (int32_t)bad_v;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(kVReady + s));
+          } else {
+            if (last) bad_v = __any_sync(0xffffffffu, bad_v) ? 1 : 0;
+            if (lane == 0) {
+              if (last) bad_v_sh[i % kFlagSlots] = (int32_t)bad_v;
+              if (!mbar_wait(full, vphase(c))) ok = false;
+              mbar_arrive(bar(kVReady + s));
+            }
+          }
+          ok = __all_sync(0xffffffffu, ok);
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          fail();
+          break;
+        }
+        advance(d);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
+    // ------------------------------------------------ softmax / epilogue of stream x
+    const int x = warp >> 2;
+    const int row = 32 * (warp & 3) + lane;  // TMEM lane of this thread
+    const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t s_cols = tmem + lane_base + col_s(x);
+    const uint32_t o_cols = tmem + lane_base + col_o(x);
+    for (uint32_t i = 0;; ++i) {
+      ItemDesc d;
+      if (!take_item(i, d)) {
+        fail();
+        break;
+      }
+      if (d.r < 0 || *abort_flag != 0) break;
+      const int64_t* trow = p.table + (int64_t)d.r * p.table_stride;
+      bool ok = true;
+      const int qt = d.two ? x : 0;  // query tile of this stream
+      const int64_t tok = d.q0 + (int64_t)qt * p.block_q + row / p.group;
+      const bool row_valid = row < p.group * p.block_q && tok < d.qe;
+      const bool warp_valid = __any_sync(0xffffffffu, row_valid);
+      const int32_t lo_q =
+          row_valid ? (int32_t)min(max((int64_t)d.kv_lo, __ldg(p.qstart + tok)), (int64_t)d.committed) : 0;
+      const uint64_t* mrow =
+          reinterpret_cast<const uint64_t*>(p.mask) + (row_valid ? tok * p.mask_words : 0);
+      const int nx = stream_tiles(d, x), step = d.two ? 1 : 2, first = d.two ? 0 : x;
+      const uint32_t tcx = x == 0 ? tc0 : tc1;
+      // The row's keys among 32 from position k0 (32-aligned in the tile).
+      auto seen32 = [&](int32_t k) -> uint32_t {
+        if (!row_valid) return 0u;
+        const int32_t a = min(max(lo_q - k, 0), 32), b = min(max(d.committed - k, 0), 32);
+        const uint32_t below_a = a >= 32 ? ~0u : (1u << a) - 1u, below_b = b >= 32 ? ~0u : (1u << b) - 1u;
+        uint32_t bits = below_b & ~below_a;
+        const int32_t j = k - d.committed, nodes = d.kv_hi - d.committed;  // first node of the 32
+        if (j > -32 && j < nodes) {
+          uint32_t tree;
+          if (j <= 0) {
+            tree = (uint32_t)(__ldg(mrow) << (-j));
+          } else {
+            const int w = j >> 6, sh = j & 63;
+            uint64_t v = __ldg(mrow + w) >> sh;
+            if (sh > 32 && w + 1 < p.mask_words) v |= __ldg(mrow + w + 1) << (64 - sh);
+            tree = (uint32_t)v;
+          }
+          if (nodes - j < 32) tree &= (1u << (nodes - j)) - 1u;
+          bits |= tree;
+        }
+        return bits;
+      };
+      float m_ref = -INFINITY, l = 0.f;
+      int64_t blk_next = -1;
+      if (lane < p.boxes && nx > 0)
+        blk_next = page_of(p, trow, (int64_t)d.kbase + first * kKeys + p.box_rows * lane);
+      for (int jj = 0; jj < nx; ++jj) {
+        const int32_t k0 = d.kbase + (first + jj * step) * kKeys;
+        const uint32_t pok = __ballot_sync(0xffffffffu, blk_next >= 0);
+        blk_next = -1;
+        if (lane < p.boxes && jj + 1 < nx)
+          blk_next = page_of(p, trow, (int64_t)k0 + step * kKeys + p.box_rows * lane);
+        const bool all_pages = pok == (1u << p.boxes) - 1u;
+        // Does every row of this warp see every key of the tile?
+        const bool whole = all_pages && k0 >= d.lo_all && k0 + kKeys <= d.committed;
+        uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+        if (!whole && warp_valid) {
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) {
+            vis[ch] = seen32(k0 + 32 * ch);
+            if (!all_pages) {
+              uint32_t pages = 0;
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+                if ((pok >> ((32 * ch + 16 * u) / p.box_rows)) & 1u) pages |= 0xffffu << (16 * u);
+              vis[ch] &= pages;
+            }
+          }
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(kSFull + x), (tcx + jj) & 1))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (warp_valid) {
+          uint32_t sc[4][32];
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) tmem_ld32_raw(s_cols + 32 * ch, sc[ch]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) reg_fence(sc[ch]);
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < kKeys; e += 2)
+              mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], __uint_as_float(sc[e >> 5][e & 31]),
+                                       __uint_as_float(sc[e >> 5][(e & 31) + 1]));
+          } else {
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float va = (vis[ch] >> e) & 1u ? __uint_as_float(sc[ch][e]) : -INFINITY;
+                const float vb = (vis[ch] >> (e + 1)) & 1u ? __uint_as_float(sc[ch][e + 1]) : -INFINITY;
+                sc[ch][e] = __float_as_uint(va);
+                sc[ch][e + 1] = __float_as_uint(vb);
+                mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], va, vb);
+              }
+            }
+          }
+          const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+          // The reference moves only when a score exceeds it by 2^8: O / l is
+          // exact whatever it is, and P <= 2^8 stays well inside fp16 / bf16.
+          float corr = 1.f;
+          if (tmax > m_ref + kRescaleLog2) {
+            corr = ex2(m_ref - tmax);  // 0 when m_ref is -inf
+            l *= corr;
+            m_ref = tmax;
+          }
+          // O holds P.V of the stream's tile before, complete because this S
+          // (issued behind it) is.
+          if (jj >= 1 && __any_sync(0xffffffffu, corr != 1.f)) {
+#pragma unroll 1
+            for (int ch = 0; ch < 8; ++ch) {
+              uint32_t o[16];
+              tmem_ld16_raw(o_cols + 16 * ch, o);
+              tmem_wait_ld();
+              reg_fence(o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+              tmem_st16(o_cols + 16 * ch, o);
+            }
+          }
+          // P = 2^(s*scale - m), over S as packed 16-bit pairs: keys
+          // 32ch..+31 in columns 32ch..+15, the bf16 remainder (P - bf16(P),
+          // which keeps 16 bits of P in the second product) in 32ch+16..+31.
+          const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+          const uint64_t scale2 = f32x2_pack(p.scale_log2, p.scale_log2);
+          const uint64_t negmu2 = f32x2_pack(-mu, -mu);
+          uint64_t ps2[2] = {f32x2_pack(0.f, 0.f), f32x2_pack(0.f, 0.f)};
+#pragma unroll
+          for (int ch = 0; ch < 4; ++ch) {
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+              uint32_t hi[8], lo[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const int k = 16 * hh + 2 * e;
+                float xa, xb;
+                f32x2_unpack(f32x2_fma(f32x2_pack(__uint_as_float(sc[ch][k]),
+                                                  __uint_as_float(sc[ch][k + 1])),
+                                       scale2, negmu2),
+                             xa, xb);
+                const float pa = ex2(xa), pb = ex2(xb);
+                ps2[e & 1] = f32x2_add(ps2[e & 1], f32x2_pack(pa, pb));
+                hi[e] = pack2<T>(pa, pb);
+                if constexpr (kBf16) {
+                  const float2 hf =
+                      __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&hi[e]));
+                  lo[e] = pack2<T>(pa - hf.x, pb - hf.y);
+                }
+              }
+              tmem_st8(s_cols + 32 * ch + 8 * hh, hi);
+              if constexpr (kBf16) tmem_st8(s_cols + 32 * ch + 16 + 8 * hh, lo);
+            }
+          }
+          tmem_wait_st();
+          float s0, s1, s2, s3;
+          f32x2_unpack(ps2[0], s0, s1);
+          f32x2_unpack(ps2[1], s2, s3);
+          l += (s0 + s1) + (s2 + s3);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kPFull + x));
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        fail();
+        break;
+      }
+
+      // ---- epilogue ----
+      // The non-finite values that this row sees among the replaced ones:
+      // columns [c0, c0 + 64) of the rows that only some query rows see.
+      // 32 columns at a time, which keeps them and the sums in registers.
+      const int64_t orow = tok * p.num_q_heads + (int64_t)d.h * p.group + row % p.group;
+      const int64_t part = (int64_t)blockIdx.x * 2 + d.slot;
+      const int part_row = qt * kRows + row;
+      // The non-finite values that this row sees among the replaced ones.
+      auto add_nonfinite = [&](float (&o)[32], int c0) {
+        const int32_t seg_end = min(d.kbase + d.n * kKeys, d.kv_hi);
+        for (int32_t k = max(d.kbase, d.kv_lo); k < seg_end; ++k) {
+          if (k >= d.lo_all && k < d.committed) {
+            k = d.committed - 1;
+            continue;
+          }
+          if (!(seen32(k) & 1u)) continue;
+          const int64_t blk = page_of(p, trow, k);
+          if (blk < 0) continue;
+          const uint32_t* v = reinterpret_cast<const uint32_t*>(
+              reinterpret_cast<const T*>(p.cache) +
+              ((p.num_slots + blk * p.block_size + k % p.block_size) * p.num_kv_heads + d.h) * 128 + c0);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t w = __ldg(v + e), b = nonfinite2<T>(w);
+            if (b & 0x8000u) o[2 * e] += to_float(reinterpret_cast<const T*>(&w)[0]);
+            if (b & 0x80000000u) o[2 * e + 1] += to_float(reinterpret_cast<const T*>(&w)[1]);
+          }
+        }
+      };
+      // Columns [c0, c0 + 32) of the row: its output, or its partial.
+      auto put = [&](float (&f)[32], int c0, float inv) {
+        if (d.slot < 0) {
+          uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + orow * 128 + c0);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            dst[e] = make_uint4(pack2<T>(f[8 * e] * inv, f[8 * e + 1] * inv),
+                                pack2<T>(f[8 * e + 2] * inv, f[8 * e + 3] * inv),
+                                pack2<T>(f[8 * e + 4] * inv, f[8 * e + 5] * inv),
+                                pack2<T>(f[8 * e + 6] * inv, f[8 * e + 7] * inv));
+        } else {
+          float4* dst = p.part_o + (part * 32 + c0 / 4) * kPartRows + part_row;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            dst[e * kPartRows] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+        }
+      };
+      if (d.two) {
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(kPvDone + x), (tcx + nx - 1) & 1))) {
+          fail();
+          break;
+        }
+        tc_fence_after();
+        const bool bad = bad_v_sh[i % kFlagSlots] != 0;
+        if (warp_valid) {
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          if (d.slot >= 0 && row_valid) p.part_ml[part * kPartRows + part_row] = make_float2(m_ref, l);
+#pragma unroll 1
+          for (int c0 = 0; c0 < 128; c0 += 32) {
+            uint32_t o[32];
+            tmem_ld32_raw(o_cols + c0, o);
+            tmem_wait_ld();
+            reg_fence(o);
+            float f[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(o[e]);
+            if (row_valid) {
+              if (bad) add_nonfinite(f, c0);
+              put(f, c0, inv);
+            }
+            __syncwarp();
+          }
+        }
+        tc_fence_before();
+      } else {
+        // Both streams hold the same rows: each warpgroup joins 64 columns.
+        const int y = x ^ 1;
+        const int ny = stream_tiles(d, y);
+        ml_sh[x][row] = make_float2(m_ref, l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kMl + x));
+        bool arrived = mbar_wait(bar(kMl + y), mc & 1);
+        // The other stream's last S is complete (its (m, l) are here), so its
+        // P.V barrier is in that tile's phase or just behind it.
+        if (nx > 0) arrived = arrived && mbar_wait(bar(kPvDone + x), (tcx + nx - 1) & 1);
+        if (ny > 0) arrived = arrived && mbar_wait(bar(kPvDone + y), ((y == 0 ? tc0 : tc1) + ny - 1) & 1);
+        if (!__all_sync(0xffffffffu, arrived)) {
+          fail();
+          break;
+        }
+        tc_fence_after();
+        const bool bad = bad_v_sh[i % kFlagSlots] != 0;
+        if (warp_valid) {
+          const float2 other = ml_sh[y][row];
+          const float m_all = fmaxf(m_ref, other.x);
+          const float mu = m_all == -INFINITY ? 0.f : m_all;
+          const float f_x = ex2(m_ref - mu), f_y = ex2(other.x - mu);
+          const float l_all = l * f_x + other.y * f_y;
+          const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+          if (x == 0 && d.slot >= 0 && row_valid)
+            p.part_ml[part * kPartRows + part_row] = make_float2(m_all, l_all);
+          const uint32_t other_cols = tmem + lane_base + col_o(y);
+#pragma unroll 1
+          for (int c0 = 64 * x; c0 < 64 * x + 64; c0 += 32) {
+            uint32_t o[32];
+            float f[32];
+            if (nx > 0) {
+              tmem_ld32_raw(o_cols + c0, o);
+              tmem_wait_ld();
+              reg_fence(o);
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) f[e] = nx > 0 ? __uint_as_float(o[e]) * f_x : 0.f;
+            if (ny > 0) {
+              tmem_ld32_raw(other_cols + c0, o);
+              tmem_wait_ld();
+              reg_fence(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) f[e] = fmaf(__uint_as_float(o[e]), f_y, f[e]);
+            }
+            if (row_valid) {
+              if (bad) add_nonfinite(f, c0);
+              put(f, c0, inv);
+            }
+            __syncwarp();
+          }
+        }
+        // The next item's first P.V overwrites O: not before the other
+        // warpgroup has read this stream's columns.
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kORead + y));
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(kORead + x), mc & 1))) {
+          fail();
+          break;
+        }
+        tc_fence_after();
+      }
+      advance(d);
+    }
+  }
+
+  // Everything this CTA issued lands before TMEM and shared memory go away.
+  if (warp == kMmaWarp && lane == 0) {
+    umma_commit(bar(kFinal));
+    mbar_wait(bar(kFinal), 0);
+  }
+  __syncthreads();
+  if (abort_sh && tid == 0) {
+    if (p.status != nullptr) atomicOr(p.status, kStatusWaitTimeout);
+    if (last_issued[0] >= 0) {
+      const uint32_t c = (uint32_t)last_issued[0];
+      mbar_wait(bar(kKFull + kslot(c)), kphase(c));
+    }
+    if (last_issued[1] >= 0) {
+      const uint32_t c = (uint32_t)last_issued[1];
+      mbar_wait(bar(kVFull + vslot(c)), vphase(c));
+    }
+    for (int32_t c = max(q_issued - kQStages, 0); c < q_issued; ++c)
+      mbar_wait(bar(kQFull + c % kQStages), (c / kQStages) & 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Joins the partials of the item that CTA b starts and does not finish, and
+// writes 0 to the rows that no request owns.  Block (b, y): 32 rows x 64
+// columns; a lane owns a row, so the partials (column chunks of 4, rows
+// adjacent) are read coalesced.
+constexpr int kMergeThreads = 256;
+constexpr int kMergeY = 2 * kPartRows / 32;
+constexpr int kZeroBlocks = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeParams p, int32_t ctas) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_dependency_wait();
+  if ((int)blockIdx.x >= ctas) {
+    const int64_t w0 = ((int64_t)(blockIdx.x - ctas) * gridDim.y + blockIdx.y) * (kMergeThreads / 32) + warp;
+    const int64_t warps = (int64_t)kZeroBlocks * gridDim.y * (kMergeThreads / 32);
+    for (int64_t t0 = 32 * w0; t0 < p.num_tokens; t0 += 32 * warps) {
+      const int64_t t = t0 + lane;
+      bool zero = false;
+      if (t < p.num_tokens) {
+        const int64_t r = find_request(p.qsl, p.num_requests, t);
+        TreeExtent e;
+        zero = r < 0 || !tree_extent(p, r, e);
+      }
+      for (uint32_t todo = __ballot_sync(0xffffffffu, zero); todo != 0; todo &= todo - 1) {
+        uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) +
+                                              (t0 + __ffs(todo) - 1) * p.num_q_heads * 128);
+        for (int e = lane; e < p.num_q_heads * 16; e += 32) dst[e] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    return;
+  }
+  const CutRecord c = p.cuts[blockIdx.x];
+  if (!c.valid) return;
+  const int row = 32 * (blockIdx.y >> 1) + lane;  // of the item's two query tiles
+  const int chunk = 16 * (blockIdx.y & 1) + 2 * warp;
+  const int in_tile = row & (kRows - 1);
+  const int64_t tok = c.q0 + (int64_t)(row / kRows) * p.block_q + in_tile / p.group;
+  const bool valid = in_tile < p.group * p.block_q && tok < c.qe &&
+                     (row < kRows || c.tile_cost == kTileCost2);
+  if (!valid) return;
+  const int64_t b0 = blockIdx.x;
+  const int64_t b_last = (c.cost0 + kItemCost + (int64_t)(c.tiles - 1) * c.tile_cost) / c.share;
+  float m = -INFINITY, l = 0.f;
+  float o[8] = {};
+#pragma unroll 2
+  for (int64_t b = b0; b <= b_last; ++b) {
+    if (tile_at(b * c.share, c.cost0, c.tile_cost, c.tiles) >=
+        tile_at((b + 1) * c.share, c.cost0, c.tile_cost, c.tiles))
+      continue;  // no tile in that share
+    const int64_t part = 2 * b + (b == b0 ? 1 : 0);
+    const float2 ml = __ldcg(p.part_ml + part * kPartRows + row);
+    const float4 u = __ldcg(p.part_o + (part * 32 + chunk) * kPartRows + row);
+    const float4 v = __ldcg(p.part_o + (part * 32 + chunk + 1) * kPartRows + row);
+    const float m_new = fmaxf(m, ml.x), mu = m_new == -INFINITY ? 0.f : m_new;
+    const float f0 = ex2(m - mu), f1 = ex2(ml.x - mu);
+    m = m_new;
+    l = l * f0 + ml.y * f1;
+    const float add[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = o[e] * f0 + add[e] * f1;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t orow = tok * p.num_q_heads + (int64_t)c.h * p.group + in_tile % p.group;
+  *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + orow * 128 + 4 * chunk) =
+      make_uint4(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv),
+                 pack2<T>(o[4] * inv, o[5] * inv), pack2<T>(o[6] * inv, o[7] * inv));
+}
+
+struct TreeDeviceState {
+  bool checked = false, fits = false;
+};
+std::mutex g_tree_lock;
+TreeDeviceState g_tree_state[kMaxDevices];
+
+// The kernels were built with the register count that the split assumes, and
+// take their shared memory on the current device.
+bool tree_kernels_fit() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return false;
+  std::lock_guard<std::mutex> guard(g_tree_lock);
+  TreeDeviceState& st = g_tree_state[dev];
+  if (!st.checked) {
+    const void* fns[2] = {reinterpret_cast<const void*>(tree_attention_kernel<__half>),
+                          reinterpret_cast<const void*>(tree_attention_kernel<__nv_bfloat16>)};
+    st.fits = true;
+    for (const void* fn : fns) {
+      cudaFuncAttributes fa;
+      st.fits = st.fits && cudaFuncGetAttributes(&fa, fn) == cudaSuccess &&
+                fa.maxThreadsPerBlock >= kThreads && fa.numRegs == kLaunchRegs &&
+                cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) == cudaSuccess;
+    }
+    st.checked = true;
+  }
+  return st.fits;
+}
+
+struct TreeLayout {
+  size_t cuts, part_ml, part_o, end;
+};
+TreeLayout tree_layout(int64_t ctas) {
+  TreeLayout w;
+  auto align = [](size_t v) { return (v + 255) & ~(size_t)255; };
+  w.cuts = 0;
+  w.part_ml = align((size_t)ctas * sizeof(CutRecord));
+  w.part_o = align(w.part_ml + (size_t)ctas * 2 * kPartRows * sizeof(float2));
+  w.end = w.part_o + (size_t)ctas * 2 * 32 * kPartRows * sizeof(float4);
+  return w;
+}
+
+// Rows of a TMA box: the most that divide a page.
+int box_rows_of(int32_t block_size) {
+  int rows = kKeys;
+  while (rows > 16 && block_size % rows != 0) rows >>= 1;
+  return rows;
+}
+
+}  // namespace
+
+size_t tree_workspace_bytes() { return tree_layout(kMaxTreeCtas).end; }
+
+bool tree_tc_supported(const TreeProblem& a) {
+  const int group = a.num_q_heads / a.num_kv_heads;
+  const int64_t num_slots = a.num_blocks * a.block_size;
+  return (a.dtype == MVB_DTYPE_F16 || a.dtype == MVB_DTYPE_BF16) && a.head_dim == 128 &&
+         group <= 64 && (a.block_size % 16) == 0 && a.num_blocks > 0 &&
+         ((uintptr_t)a.query % 16) == 0 && ((uintptr_t)a.cache % 16) == 0 &&
+         ((uintptr_t)a.out % 16) == 0 &&
+         (a.num_tokens == 1 || ((a.q_st % 8) == 0 && a.q_st >= 128)) &&
+         (a.num_q_heads == 1 || ((a.q_sh % 8) == 0 && a.q_sh >= 128)) &&
+         2 * num_slots < ((int64_t)1 << 31) && a.num_tokens < ((int64_t)1 << 31) &&
+         a.num_requests < ((int64_t)1 << 31) && tensor_map_encoder() != nullptr && tree_kernels_fit();
+}
+
+int launch_tree_attention(const TreeProblem& a) {
+  if (a.workspace == nullptr || ((uintptr_t)a.workspace % 256) != 0) return MVB_ERR_INVALID_ARGUMENT;
+  const int ctas = num_sms() < kMaxTreeCtas ? num_sms() : kMaxTreeCtas;
+  const TreeLayout w = tree_layout(ctas);
+  if (a.workspace_bytes < w.end) return MVB_ERR_WORKSPACE_TOO_SMALL;
+  EncodeTiled encode = tensor_map_encoder();
+  const CUtensorMapDataType dt =
+      a.dtype == MVB_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const int group = a.num_q_heads / a.num_kv_heads;
+  const int64_t num_slots = a.num_blocks * a.block_size;
+  const int box_rows = box_rows_of(a.block_size);
+  CUtensorMap qmap, kvmap;
+  {
+    const cuuint64_t q_sh = a.num_q_heads == 1 ? 128 : (cuuint64_t)a.q_sh;
+    const cuuint64_t q_st = a.num_tokens == 1 ? q_sh * a.num_q_heads : (cuuint64_t)a.q_st;
+    const cuuint64_t dims[3] = {128, (cuuint64_t)a.num_q_heads, (cuuint64_t)a.num_tokens};
+    const cuuint64_t strides[2] = {q_sh * 2, q_st * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)(kRows / group)};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    if (encode(&qmap, dt, 3, const_cast<void*>(a.query), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return MVB_ERR_UNSUPPORTED_SHAPE;
+  }
+  {
+    const cuuint64_t dims[2] = {(cuuint64_t)a.num_kv_heads * 128, (cuuint64_t)(2 * num_slots)};
+    const cuuint64_t strides[1] = {(cuuint64_t)a.num_kv_heads * 128 * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    if (encode(&kvmap, dt, 2, const_cast<void*>(a.cache), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return MVB_ERR_UNSUPPORTED_SHAPE;
+  }
+  char* ws = static_cast<char*>(a.workspace);
+  TreeParams p;
+  p.out = static_cast<char*>(a.out);
+  p.num_q_heads = a.num_q_heads;
+  p.num_kv_heads = a.num_kv_heads;
+  p.group = group;
+  p.block_q = kRows / group;
+  p.block_size = a.block_size;
+  p.bs_shift = (a.block_size & (a.block_size - 1)) == 0 ? __builtin_ctz(a.block_size) : -1;
+  p.box_rows = box_rows;
+  p.boxes = kKeys / box_rows;
+  p.num_blocks = a.num_blocks;
+  p.num_slots = num_slots;
+  p.qstart = a.qstart;
+  p.qsl = a.qsl;
+  p.ctx_len = a.ctx_len;
+  p.table = a.table;
+  p.table_stride = a.table_stride;
+  p.table_width = a.table_width;
+  p.mask = a.mask;
+  p.mask_words = a.mask_words;
+  p.num_tokens = a.num_tokens;
+  p.num_requests = a.num_requests;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.part_o = reinterpret_cast<float4*>(ws + w.part_o);
+  p.part_ml = reinterpret_cast<float2*>(ws + w.part_ml);
+  p.cuts = reinterpret_cast<CutRecord*>(ws + w.cuts);
+  p.cache = static_cast<const char*>(a.cache);
+  p.status = a.status;
+  const bool bf16 = a.dtype == MVB_DTYPE_BF16;
+  if (bf16)
+    tree_attention_kernel<__nv_bfloat16><<<ctas, kThreads, kSmemBytes, a.stream>>>(qmap, kvmap, p);
+  else
+    tree_attention_kernel<__half><<<ctas, kThreads, kSmemBytes, a.stream>>>(qmap, kvmap, p);
+  const int rc = check_launch();
+  if (rc != MVB_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(ctas + kZeroBlocks), kMergeY);
+  cfg.blockDim = dim3(kMergeThreads);
+  cfg.stream = a.stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = bf16 ? cudaLaunchKernelEx(&cfg, tree_merge_kernel<__nv_bfloat16>, p, ctas)
+                             : cudaLaunchKernelEx(&cfg, tree_merge_kernel<__half>, p, ctas);
+  if (e != cudaSuccess) {
+    set_last_cuda_error(e);
+    return MVB_ERR_CUDA;
+  }
+  return check_launch();
+}
+
+}  // namespace mvb
