@@ -68,6 +68,10 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int lim
 }
 
 // ---------------------------------------------------------------- TMA
+// Brings a kernel argument's tensor map into the descriptor cache.
+__device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int32_t x,
                                             int32_t y, uint32_t bar) {
   asm volatile(

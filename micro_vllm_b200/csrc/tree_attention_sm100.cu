@@ -76,7 +76,7 @@ constexpr float kRescaleLog2 = 8.f;
 
 // Cost axis: a KV tile of an item with one or two query tiles, an item's
 // fixed part, and the least share of a CTA.
-constexpr int kTileCost1 = 4, kTileCost2 = 6, kItemCost = 4, kMinShare = 8;
+constexpr int kTileCost1 = 4, kTileCost2 = 6, kItemCost = 20, kMinShare = 8;
 
 constexpr int kPartRows = 2 * kRows;  // rows of one partial
 
@@ -141,6 +141,11 @@ __device__ __forceinline__ int64_t page_of(const TreeParams& p, const int64_t* t
   if (pos < 0 || lb >= p.table_width) return -1;
   const int64_t blk = __ldg(trow + lb);
   return (blk >= 0 && blk < p.num_blocks) ? blk : -1;
+}
+
+__device__ __forceinline__ void touch(const int64_t* at) {
+  int64_t v;
+  asm volatile("ld.global.nc.b64 %0, [%1];\n" : "=l"(v) : "l"(at));
 }
 
 template <typename T>
@@ -258,10 +263,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int32_t* abort_flag = &abort_sh;
 
   if (tid == 0) {
+    prefetch_tensormap(&qmap);
+    prefetch_tensormap(&kvmap);
     for (int i = 0; i < kNumBars; ++i) {
       const bool four = (i >= kPFull && i < kPFull + 2) || (i >= kMl && i < kORead + 2);
       const bool readers = i >= kItemEmpty && i < kItemEmpty + kItemSlots;
-      mbar_init(bar(i), readers ? kItemReaders : four ? 4 : 1);
+      const bool eight = i >= kQEmpty && i < kQEmpty + kQStages;
+      mbar_init(bar(i), readers ? kItemReaders : eight ? 8 : four ? 4 : 1);
     }
     mbar_init_fence();
     abort_sh = 0;
@@ -426,6 +434,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
         if (!ok) fail();
+        // Under load a global load takes microseconds: bring what the other
+        // warps read first of this item into the SM's cache.
+        for (int64_t t = d.q0 + lane; t < min(d.q0 + 2 * (int64_t)p.block_q, d.qe); t += 32)
+          touch(p.mask + t * p.mask_words);
+        {
+          const int64_t pos = (int64_t)d.kbase + max(d.n - 2, 0) * kKeys + 8 * lane;
+          const int64_t lb = p.bs_shift >= 0 ? (pos >> p.bs_shift) : pos / p.block_size;
+          if (lb < p.table_width) touch(p.table + (int64_t)d.r * p.table_stride + lb);
+        }
         advance(d);
       }
       if (lane == 0 && cut.valid) p.cuts[blockIdx.x] = cut;
@@ -450,15 +467,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto issue_pv = [&](int x, uint32_t stage, bool acc) {
           const uint64_t dv = dv0 + (uint64_t)((stage * kTileBytes) >> 4);
 #pragma unroll
-          for (int part = 0; part < (kBf16 ? 2 : 1); ++part) {  // P_hi (+ P_lo in bf16)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const uint32_t pcol = 32 * (k >> 1) + 8 * (k & 1) + 16 * part;
-              umma_f16_ts(tmem + col_o(x), tmem + col_s(x) + pcol, dv + (uint64_t)(k * (2048 >> 4)),
-                          idesc_pv, acc || k > 0 || part > 0);
-            }
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t pcol = 32 * (k >> 1) + 8 * (k & 1);
+            umma_f16_ts(tmem + col_o(x), tmem + col_s(x) + pcol, dv + (uint64_t)(k * (2048 >> 4)),
+                        idesc_pv, acc || k > 0);
           }
           umma_commit(bar(kPvDone + x));
+        };
+        // A probe costs ~200 cycles, so what usually is there goes in one batch:
+        // V of tile c (landed, fixed) and, if `more`, the K tile ck.
+        auto wait_vk = [&](uint32_t c, bool more, uint32_t ck) -> bool {
+          const uint32_t vf = bar(kVFull + vslot(c)), vr = bar(kVReady + vslot(c));
+          const uint32_t kf = more ? bar(kKFull + kslot(ck)) : vr;
+          const uint32_t kp = more ? kphase(ck) : vphase(c);
+          bool r0, r1, r2;
+          mbar_test3(vf, vphase(c), vr, vphase(c), kf, kp, r0, r1, r2);
+          return (r0 || mbar_wait(vf, vphase(c))) && (r1 || mbar_wait(vr, vphase(c))) &&
+                 (r2 || mbar_wait(kf, kp));
         };
         bool ok = true;
         for (uint32_t i = 0; ok; ++i) {
@@ -483,28 +508,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             issue_s(1, qs1, kslot(kvc));
             umma_commit(bar(kKEmpty + kslot(kvc)));
-            if (n == 1) {
-              umma_commit(bar(kQEmpty + qs0));
-              umma_commit(bar(kQEmpty + qs1));
-            }
             for (int j = 0; ok && j < n; ++j) {
               const uint32_t c = kvc + j;
               for (int x = 0; x < 2; ++x) {
                 ok = mbar_wait(bar(kPFull + x), ((x == 0 ? tc0 : tc1) + j) & 1) &&
-                     (x == 1 || mbar_wait(bar(kVReady + vslot(c)), vphase(c)));
+                     (x == 1 || wait_vk(c, j + 1 < n, c + 1));
                 if (!ok) break;
                 tc_fence_after();
                 issue_pv(x, vslot(c), j > 0);
                 if (x == 1) umma_commit(bar(kVEmpty + vslot(c)));
                 if (j + 1 < n) {
-                  if (x == 0) {
-                    ok = mbar_wait(bar(kKFull + kslot(c + 1)), kphase(c + 1));
-                    if (!ok) break;
-                    tc_fence_after();
-                  }
                   issue_s(x, x == 0 ? qs0 : qs1, kslot(c + 1));
                   if (x == 1) umma_commit(bar(kKEmpty + kslot(c + 1)));
-                  if (j + 2 == n) umma_commit(bar(kQEmpty + (x == 0 ? qs0 : qs1)));
                 }
               }
             }
@@ -517,23 +532,18 @@ __global__ void __launch_bounds__(kThreads, 1)
               issue_s(1, qs0, kslot(kvc + 1));
               umma_commit(bar(kKEmpty + kslot(kvc + 1)));
             }
-            if (n <= 2) umma_commit(bar(kQEmpty + qs0));
             for (int j = 0; ok && j < n; ++j) {
               const uint32_t c = kvc + j;
               const int x = j & 1;
               ok = mbar_wait(bar(kPFull + x), ((x == 0 ? tc0 : tc1) + (j >> 1)) & 1) &&
-                   mbar_wait(bar(kVReady + vslot(c)), vphase(c));
+                   wait_vk(c, j + 2 < n, c + 2);
               if (!ok) break;
               tc_fence_after();
               issue_pv(x, vslot(c), j > 1);
               umma_commit(bar(kVEmpty + vslot(c)));
               if (j + 2 < n) {
-                ok = mbar_wait(bar(kKFull + kslot(c + 2)), kphase(c + 2));
-                if (!ok) break;
-                tc_fence_after();
                 issue_s(x, qs0, kslot(c + 2));
                 umma_commit(bar(kKEmpty + kslot(c + 2)));
-                if (j + 3 == n) umma_commit(bar(kQEmpty + qs0));
               }
             }
           }
@@ -546,29 +556,94 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
       // ---------------------------------------------------- producers
       const bool is_k = warp == kKProdWarp;
-      for (uint32_t i = 0;; ++i) {
+      // A V tile with rows that some query row does not see is fixed up once
+      // it lands: rows behind the last key, before the first and on missing
+      // pages are zeroed, the non-finite elements of rows that only some
+      // query rows see too.  The fix waits in `todo` until the next load is
+      // on its way.
+      struct Todo {
+        uint32_t c, item, boxes_ok;
+        int32_t k0, kv_lo, kv_hi, lo_all, committed;
+        bool last;
+      } todo{};
+      bool pending = false;
+      uint32_t bad_v = 0;  // a non-finite element was replaced in the item
+      auto leave_flag = [&](uint32_t item) {  // with the item's last tile
+        const bool any = __any_sync(0xffffffffu, bad_v) != 0;
+        if (lane == 0) bad_v_sh[item % kFlagSlots] = any ? 1 : 0;
+        bad_v = 0;
+      };
+      auto fix_v = [&]() -> bool {
+        pending = false;
+        const uint32_t s = vslot(todo.c);
+        if (!__all_sync(0xffffffffu, mbar_wait(bar(kVFull + s), vphase(todo.c)))) return false;
+        // Lane l takes 16-byte chunk l % 8 of row 4i + l / 8, both halves.
+        uint8_t* vt = smem + kOffV + s * kTileBytes + (lane & 7) * 16;
+        auto zero_rows = [&](int r0, int r1) {
+          for (int row = r0 + (lane >> 3); row < r1; row += 4) {
+            uint4* cell = reinterpret_cast<uint4*>(vt + row * 128);
+            cell[0] = make_uint4(0, 0, 0, 0);
+            cell[kHalf / 16] = make_uint4(0, 0, 0, 0);
+          }
+        };
+        auto clean_rows = [&](int r0, int r1) {
+#pragma unroll 4
+          for (int row = r0 + (lane >> 3); row < r1; row += 4) {
+            uint4* cell = reinterpret_cast<uint4*>(vt + row * 128);
+            uint4 v[2] = {cell[0], cell[kHalf / 16]};
+            uint32_t* w = reinterpret_cast<uint32_t*>(v);
+            uint32_t any = 0;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) any |= nonfinite2<T>(w[q]);
+            if (any) {
+              bad_v = 1;
+#pragma unroll
+              for (int q = 0; q < 8; ++q) w[q] &= ~((nonfinite2<T>(w[q]) >> 15) * 0xffffu);
+              cell[0] = v[0];
+              cell[kHalf / 16] = v[1];
+            }
+          }
+        };
+        const int lo = max(todo.kv_lo - todo.k0, 0), hi = min(todo.kv_hi - todo.k0, kKeys);
+        zero_rows(0, lo);
+        zero_rows(hi, kKeys);
+        for (int b = 0; b < p.boxes; ++b)
+          if (!((todo.boxes_ok >> b) & 1u)) zero_rows(b * p.box_rows, (b + 1) * p.box_rows);
+        __syncwarp();
+        clean_rows(lo, min(todo.lo_all - todo.k0, hi));
+        clean_rows(max(todo.committed - todo.k0, lo), hi);
+        fence_proxy_async();  // visible to the P.V MMAs
+        if (todo.last) leave_flag(todo.item);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kVReady + s));
+        return true;
+      };
+      bool ok = true;
+      for (uint32_t i = 0; ok; ++i) {
         ItemDesc d;
         if (!take_item(i, d)) {
-          fail();
+          ok = false;
           break;
         }
         if (d.r < 0 || *abort_flag != 0) break;
         const int64_t* trow = p.table + (int64_t)d.r * p.table_stride;
-        bool ok = true;
-        uint32_t bad_v = 0;  // this lane replaced a non-finite element
-        for (int j = 0; ok && j < d.n; ++j) {
+        for (int j = 0; j < d.n; ++j) {
           const uint32_t c = kvc + j;
           const uint32_t s = is_k ? kslot(c) : vslot(c);
           const uint32_t full = bar((is_k ? kKFull : kVFull) + s);
-          const int32_t k0 = d.kbase + j * kKeys;
+          const uint32_t empty = bar((is_k ? kKEmpty : kVEmpty) + s);
+          const uint32_t empty_phase = (is_k ? kphase(c) : vphase(c)) ^ 1;
+          const int32_t k0 = d.kbase + (d.n - 1 - j) * kKeys;  // the drafted keys first
           const int64_t pos = (int64_t)k0 + p.box_rows * lane;
           int64_t blk = -1;
           if (lane < p.boxes) blk = page_of(p, trow, pos);
-          if (!__all_sync(0xffffffffu, mbar_wait(bar((is_k ? kKEmpty : kVEmpty) + s),
-                                                 (is_k ? kphase(c) : vphase(c)) ^ 1))) {
-            ok = false;
-            break;
-          }
+          if (pending && !__all_sync(0xffffffffu, mbar_try_wait(empty, empty_phase))) ok = fix_v();
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(empty, empty_phase));
+          if (!ok) break;
+          const uint32_t boxes_ok = __ballot_sync(0xffffffffu, lane < p.boxes && blk >= 0);
+          const bool last = j == d.n - 1;
+          const bool dirty = k0 < d.lo_all || k0 + kKeys > d.committed ||
+                             boxes_ok != (1u << p.boxes) - 1u;
           if (lane == 0) {
             last_issued[is_k ? 0 : 1] = (int32_t)c;
             mbar_expect_tx(full, kTileBytes);
@@ -586,67 +661,21 @@ __global__ void __launch_bounds__(kThreads, 1)
               atomicOr(p.status, MVB_STATUS_BLOCK_OUT_OF_RANGE);
           }
           if (is_k) continue;
-          // Rows that some query row does not see: behind the last key,
-          // before the first, on missing pages (all zeroed), and those that
-          // only some rows see (their non-finite elements).
-          const uint32_t boxes_ok = __ballot_sync(0xffffffffu, lane < p.boxes && blk >= 0);
-          const bool all_pages = boxes_ok == (1u << p.boxes) - 1u;
-          const bool last = j == d.n - 1;
-          if (k0 < d.lo_all || k0 + kKeys > d.committed || k0 < d.kv_lo || !all_pages) {
-            if (!__all_sync(0xffffffffu, mbar_wait(full, vphase(c)))) {
-              ok = false;
-              break;
-            }
-            uint8_t* vt = smem + kOffV + s * kTileBytes;
-#pragma unroll 4
-            for (int it = 0; it < 32; ++it) {
-              const int row = 4 * it + (lane >> 3);
-              const int32_t key = k0 + row;
-              uint4* cell = reinterpret_cast<uint4*>(vt + row * 128 + (lane & 7) * 16);
-              if (key < d.kv_lo || key >= d.kv_hi || !((boxes_ok >> (row / p.box_rows)) & 1u)) {
-                cell[0] = make_uint4(0, 0, 0, 0);
-                cell[kHalf / 16] = make_uint4(0, 0, 0, 0);
-              } else if (key < d.lo_all || key >= d.committed) {
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                  uint4 v = cell[hf * (kHalf / 16)];
-                  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-                  uint32_t any = 0;
-#pragma unroll
-                  for (int q = 0; q < 4; ++q) {
-                    const uint32_t b = nonfinite2<T>(w[q]);
-                    any |= b;
-                    w[q] &= ~((b >> 15) * 0xffffu);
-                  }
-                  if (any) {
-                    cell[hf * (kHalf / 16)] = v;
-                    bad_v = 1;
-                  }
-                }
-              }
-            }
-            fence_proxy_async();  // visible to the P.V MMAs
-            if (last) bad_v = __any_sync(0xffffffffu, bad_v) ? 1 : 0;
-            if (last && lane == 0) bad_v_sh[i % kFlagSlots] = (int32_t)bad_v;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(kVReady + s));
+          if (pending) ok = fix_v();
+          if (!ok) break;
+          if (dirty) {
+            todo = {c, i, boxes_ok, k0, d.kv_lo, d.kv_hi, d.lo_all, d.committed, last};
+            pending = true;
           } else {
-            if (last) bad_v = __any_sync(0xffffffffu, bad_v) ? 1 : 0;
-            if (lane == 0) {
-              if (last) bad_v_sh[i % kFlagSlots] = (int32_t)bad_v;
-              if (!mbar_wait(full, vphase(c))) ok = false;
-              mbar_arrive(bar(kVReady + s));
-            }
+            if (last) leave_flag(i);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(kVReady + s));  // nothing to fix
           }
-          ok = __all_sync(0xffffffffu, ok);
         }
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) {
-          fail();
-          break;
-        }
-        advance(d);
+        if (ok) advance(d);
       }
+      if (ok && pending) ok = fix_v();
+      if (!ok) fail();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kSoftmaxRegs));
@@ -656,6 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t s_cols = tmem + lane_base + col_s(x);
     const uint32_t o_cols = tmem + lane_base + col_o(x);
+    const int row_tok = row / p.group, row_head = row % p.group;
     for (uint32_t i = 0;; ++i) {
       ItemDesc d;
       if (!take_item(i, d)) {
@@ -666,13 +696,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t* trow = p.table + (int64_t)d.r * p.table_stride;
       bool ok = true;
       const int qt = d.two ? x : 0;  // query tile of this stream
-      const int64_t tok = d.q0 + (int64_t)qt * p.block_q + row / p.group;
+      const int64_t tok = d.q0 + (int64_t)qt * p.block_q + row_tok;
       const bool row_valid = row < p.group * p.block_q && tok < d.qe;
       const bool warp_valid = __any_sync(0xffffffffu, row_valid);
       const int32_t lo_q =
           row_valid ? (int32_t)min(max((int64_t)d.kv_lo, __ldg(p.qstart + tok)), (int64_t)d.committed) : 0;
       const uint64_t* mrow =
           reinterpret_cast<const uint64_t*>(p.mask) + (row_valid ? tok * p.mask_words : 0);
+      const uint64_t mask0 = row_valid ? __ldg(mrow) : 0;  // in flight with the loads around it
       const int nx = stream_tiles(d, x), step = d.two ? 1 : 2, first = d.two ? 0 : x;
       const uint32_t tcx = x == 0 ? tc0 : tc1;
       // The row's keys among 32 from position k0 (32-aligned in the tile).
@@ -685,10 +716,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (j > -32 && j < nodes) {
           uint32_t tree;
           if (j <= 0) {
-            tree = (uint32_t)(__ldg(mrow) << (-j));
+            tree = (uint32_t)(mask0 << (-j));
           } else {
             const int w = j >> 6, sh = j & 63;
-            uint64_t v = __ldg(mrow + w) >> sh;
+            uint64_t v = (w == 0 ? mask0 : __ldg(mrow + w)) >> sh;
             if (sh > 32 && w + 1 < p.mask_words) v |= __ldg(mrow + w + 1) << (64 - sh);
             tree = (uint32_t)v;
           }
@@ -700,36 +731,45 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m_ref = -INFINITY, l = 0.f;
       int64_t blk_next = -1;
       if (lane < p.boxes && nx > 0)
-        blk_next = page_of(p, trow, (int64_t)d.kbase + first * kKeys + p.box_rows * lane);
+        blk_next = page_of(p, trow, (int64_t)d.kbase + (d.n - 1 - first) * kKeys + p.box_rows * lane);
       for (int jj = 0; jj < nx; ++jj) {
-        const int32_t k0 = d.kbase + (first + jj * step) * kKeys;
+        const int32_t k0 = d.kbase + (d.n - 1 - first - jj * step) * kKeys;
         const uint32_t pok = __ballot_sync(0xffffffffu, blk_next >= 0);
         blk_next = -1;
         if (lane < p.boxes && jj + 1 < nx)
-          blk_next = page_of(p, trow, (int64_t)k0 + step * kKeys + p.box_rows * lane);
+          blk_next = page_of(p, trow, (int64_t)k0 - step * kKeys + p.box_rows * lane);
         const bool all_pages = pok == (1u << p.boxes) - 1u;
         // Does every row of this warp see every key of the tile?
         const bool whole = all_pages && k0 >= d.lo_all && k0 + kKeys <= d.committed;
-        uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
-        if (!whole && warp_valid) {
-#pragma unroll
-          for (int ch = 0; ch < 4; ++ch) {
-            vis[ch] = seen32(k0 + 32 * ch);
-            if (!all_pages) {
-              uint32_t pages = 0;
-#pragma unroll
-              for (int u = 0; u < 2; ++u)
-                if ((pok >> ((32 * ch + 16 * u) / p.box_rows)) & 1u) pages |= 0xffffu << (16 * u);
-              vis[ch] &= pages;
-            }
-          }
-        }
         if (!__all_sync(0xffffffffu, mbar_wait(bar(kSFull + x), (tcx + jj) & 1))) {
           ok = false;
           break;
         }
         tc_fence_after();
         if (warp_valid) {
+          if (!whole) {
+            // Scores of keys that the row does not see become -inf, in place
+            // and in a small loop: one or two tiles of an item come here.
+#pragma unroll 1
+            for (int ch = 0; ch < 4; ++ch) {
+              uint32_t seen = seen32(k0 + 32 * ch);
+              if (!all_pages) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                  if (!((pok >> ((32 * ch + 16 * u) / p.box_rows)) & 1u)) seen &= ~(0xffffu << (16 * u));
+              }
+              __syncwarp();
+              uint32_t v[32];
+              tmem_ld32_raw(s_cols + 32 * ch, v);
+              tmem_wait_ld();
+              reg_fence(v);
+              float f[32];
+#pragma unroll
+              for (int e = 0; e < 32; ++e) f[e] = (seen >> e) & 1u ? __uint_as_float(v[e]) : -INFINITY;
+              tmem_st32(s_cols + 32 * ch, f);
+            }
+            tmem_wait_st();
+          }
           uint32_t sc[4][32];
 #pragma unroll
           for (int ch = 0; ch < 4; ++ch) tmem_ld32_raw(s_cols + 32 * ch, sc[ch]);
@@ -737,24 +777,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int ch = 0; ch < 4; ++ch) reg_fence(sc[ch]);
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          if (whole) {
 #pragma unroll
-            for (int e = 0; e < kKeys; e += 2)
-              mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], __uint_as_float(sc[e >> 5][e & 31]),
-                                       __uint_as_float(sc[e >> 5][(e & 31) + 1]));
-          } else {
-#pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                const float va = (vis[ch] >> e) & 1u ? __uint_as_float(sc[ch][e]) : -INFINITY;
-                const float vb = (vis[ch] >> (e + 1)) & 1u ? __uint_as_float(sc[ch][e + 1]) : -INFINITY;
-                sc[ch][e] = __float_as_uint(va);
-                sc[ch][e + 1] = __float_as_uint(vb);
-                mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], va, vb);
-              }
-            }
-          }
+          for (int e = 0; e < kKeys; e += 2)
+            mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], __uint_as_float(sc[e >> 5][e & 31]),
+                                     __uint_as_float(sc[e >> 5][(e & 31) + 1]));
           const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
           // The reference moves only when a score exceeds it by 2^8: O / l is
           // exact whatever it is, and P <= 2^8 stays well inside fp16 / bf16.
@@ -778,9 +804,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_st16(o_cols + 16 * ch, o);
             }
           }
-          // P = 2^(s*scale - m), over S as packed 16-bit pairs: keys
-          // 32ch..+31 in columns 32ch..+15, the bf16 remainder (P - bf16(P),
-          // which keeps 16 bits of P in the second product) in 32ch+16..+31.
+          // P = 2^(s*scale - m), over S as packed 16-bit pairs (keys 32ch..+31
+          // in columns 32ch..+15), summed before it is rounded.  bf16 P is
+          // rounded once too: its half step of 2^-8 is that of the output,
+          // and keeping 16 bits of it (a second product) measured 378 -> 518
+          // us at 64 requests x 128 rows x 6K keys.
           const float mu = m_ref == -INFINITY ? 0.f : m_ref;
           const uint64_t scale2 = f32x2_pack(p.scale_log2, p.scale_log2);
           const uint64_t negmu2 = f32x2_pack(-mu, -mu);
@@ -789,7 +817,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int ch = 0; ch < 4; ++ch) {
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
-              uint32_t hi[8], lo[8];
+              uint32_t pk[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 const int k = 16 * hh + 2 * e;
@@ -800,15 +828,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                              xa, xb);
                 const float pa = ex2(xa), pb = ex2(xb);
                 ps2[e & 1] = f32x2_add(ps2[e & 1], f32x2_pack(pa, pb));
-                hi[e] = pack2<T>(pa, pb);
-                if constexpr (kBf16) {
-                  const float2 hf =
-                      __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&hi[e]));
-                  lo[e] = pack2<T>(pa - hf.x, pb - hf.y);
-                }
+                pk[e] = pack2<T>(pa, pb);
               }
-              tmem_st8(s_cols + 32 * ch + 8 * hh, hi);
-              if constexpr (kBf16) tmem_st8(s_cols + 32 * ch + 16 + 8 * hh, lo);
+              tmem_st8(s_cols + 32 * ch + 8 * hh, pk);
             }
           }
           tmem_wait_st();
@@ -830,132 +852,131 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---- epilogue ----
       // The non-finite values that this row sees among the replaced ones:
       // columns [c0, c0 + 64) of the rows that only some query rows see.
-      // 32 columns at a time, which keeps them and the sums in registers.
-      const int64_t orow = tok * p.num_q_heads + (int64_t)d.h * p.group + row % p.group;
-      const int64_t part = (int64_t)blockIdx.x * 2 + d.slot;
-      const int part_row = qt * kRows + row;
-      // The non-finite values that this row sees among the replaced ones.
-      auto add_nonfinite = [&](float (&o)[32], int c0) {
-        const int32_t seg_end = min(d.kbase + d.n * kKeys, d.kv_hi);
-        for (int32_t k = max(d.kbase, d.kv_lo); k < seg_end; ++k) {
-          if (k >= d.lo_all && k < d.committed) {
-            k = d.committed - 1;
-            continue;
-          }
-          if (!(seen32(k) & 1u)) continue;
-          const int64_t blk = page_of(p, trow, k);
-          if (blk < 0) continue;
-          const uint32_t* v = reinterpret_cast<const uint32_t*>(
-              reinterpret_cast<const T*>(p.cache) +
-              ((p.num_slots + blk * p.block_size + k % p.block_size) * p.num_kv_heads + d.h) * 128 + c0);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint32_t w = __ldg(v + e), b = nonfinite2<T>(w);
-            if (b & 0x8000u) o[2 * e] += to_float(reinterpret_cast<const T*>(&w)[0]);
-            if (b & 0x80000000u) o[2 * e + 1] += to_float(reinterpret_cast<const T*>(&w)[1]);
-          }
-        }
-      };
-      // Columns [c0, c0 + 32) of the row: its output, or its partial.
-      auto put = [&](float (&f)[32], int c0, float inv) {
-        if (d.slot < 0) {
-          uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + orow * 128 + c0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            dst[e] = make_uint4(pack2<T>(f[8 * e] * inv, f[8 * e + 1] * inv),
-                                pack2<T>(f[8 * e + 2] * inv, f[8 * e + 3] * inv),
-                                pack2<T>(f[8 * e + 4] * inv, f[8 * e + 5] * inv),
-                                pack2<T>(f[8 * e + 6] * inv, f[8 * e + 7] * inv));
-        } else {
-          float4* dst = p.part_o + (part * 32 + c0 / 4) * kPartRows + part_row;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            dst[e * kPartRows] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
-        }
-      };
-      if (d.two) {
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(kPvDone + x), (tcx + nx - 1) & 1))) {
-          fail();
-          break;
-        }
-        tc_fence_after();
-        const bool bad = bad_v_sh[i % kFlagSlots] != 0;
-        if (warp_valid) {
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          if (d.slot >= 0 && row_valid) p.part_ml[part * kPartRows + part_row] = make_float2(m_ref, l);
-#pragma unroll 1
-          for (int c0 = 0; c0 < 128; c0 += 32) {
-            uint32_t o[32];
-            tmem_ld32_raw(o_cols + c0, o);
-            tmem_wait_ld();
-            reg_fence(o);
-            float f[32];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(o[e]);
-            if (row_valid) {
-              if (bad) add_nonfinite(f, c0);
-              put(f, c0, inv);
-            }
-            __syncwarp();
-          }
-        }
-        tc_fence_before();
-      } else {
-        // Both streams hold the same rows: each warpgroup joins 64 columns.
-        const int y = x ^ 1;
-        const int ny = stream_tiles(d, y);
+      // This warpgroup's columns of the row: all of its own stream's O, or,
+      // when both streams hold the same rows, one half of the sum of both.
+      const uint32_t qslot = (qc + (uint32_t)qt) % kQStages;
+      const int y = x ^ 1;
+      const int ny = d.two ? 0 : stream_tiles(d, y);
+      float m_all = m_ref, l_all = l, f_x = 1.f, f_y = 0.f;
+      bool arrived = true;
+      if (!d.two) {
         ml_sh[x][row] = make_float2(m_ref, l);
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kMl + x));
-        bool arrived = mbar_wait(bar(kMl + y), mc & 1);
-        // The other stream's last S is complete (its (m, l) are here), so its
-        // P.V barrier is in that tile's phase or just behind it.
-        if (nx > 0) arrived = arrived && mbar_wait(bar(kPvDone + x), (tcx + nx - 1) & 1);
-        if (ny > 0) arrived = arrived && mbar_wait(bar(kPvDone + y), ((y == 0 ? tc0 : tc1) + ny - 1) & 1);
-        if (!__all_sync(0xffffffffu, arrived)) {
-          fail();
-          break;
-        }
-        tc_fence_after();
+        arrived = mbar_wait(bar(kMl + y), mc & 1);
+        const float2 other = ml_sh[y][row];
+        m_all = fmaxf(m_ref, other.x);
+        const float mu = m_all == -INFINITY ? 0.f : m_all;
+        f_x = ex2(m_ref - mu);
+        f_y = ex2(other.x - mu);
+        l_all = l * f_x + other.y * f_y;
+      }
+      // A stream's last S is complete once its (m, l) are here, so its P.V
+      // barrier is in the last tile's phase or just behind it.
+      if (nx > 0) arrived = arrived && mbar_wait(bar(kPvDone + x), (tcx + nx - 1) & 1);
+      if (ny > 0) arrived = arrived && mbar_wait(bar(kPvDone + y), ((y == 0 ? tc0 : tc1) + ny - 1) & 1);
+      if (!__all_sync(0xffffffffu, arrived)) {
+        fail();
+        break;
+      }
+      tc_fence_after();
+      if (warp_valid) {
         const bool bad = bad_v_sh[i % kFlagSlots] != 0;
-        if (warp_valid) {
-          const float2 other = ml_sh[y][row];
-          const float m_all = fmaxf(m_ref, other.x);
-          const float mu = m_all == -INFINITY ? 0.f : m_all;
-          const float f_x = ex2(m_ref - mu), f_y = ex2(other.x - mu);
-          const float l_all = l * f_x + other.y * f_y;
-          const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
-          if (x == 0 && d.slot >= 0 && row_valid)
-            p.part_ml[part * kPartRows + part_row] = make_float2(m_all, l_all);
-          const uint32_t other_cols = tmem + lane_base + col_o(y);
+        const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+        const int64_t orow = tok * p.num_q_heads + (int64_t)d.h * p.group + row_head;
+        const int64_t part = (int64_t)blockIdx.x * 2 + d.slot;
+        const int part_row = qt * kRows + row;
+        if (d.slot >= 0 && row_valid && (d.two || x == 0))
+          p.part_ml[part * kPartRows + part_row] = make_float2(m_all, l_all);
+        const uint32_t other_cols = tmem + lane_base + col_o(y);
+        const int c_lo = d.two ? 0 : 64 * x, c_hi = d.two ? 128 : 64 * x + 64;
+        // Every S of the item is done with its Q tile, which stages the output.
+        uint8_t* qbuf = smem + kOffQ + qslot * kTileBytes;
+        // A small loop body: this code runs once per item, so most of its
+        // time is fetching it.
 #pragma unroll 1
-          for (int c0 = 64 * x; c0 < 64 * x + 64; c0 += 32) {
-            uint32_t o[32];
-            float f[32];
-            if (nx > 0) {
-              tmem_ld32_raw(o_cols + c0, o);
-              tmem_wait_ld();
-              reg_fence(o);
-            }
+        for (int c0 = c_lo; c0 < c_hi; c0 += 16) {
+          uint32_t o[16], u[16];
+          if (nx > 0) tmem_ld16_raw(o_cols + c0, o);
+          if (ny > 0) tmem_ld16_raw(other_cols + c0, u);
+          tmem_wait_ld();
+          reg_fence(o);
+          reg_fence(u);
+          float f[16];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) f[e] = nx > 0 ? __uint_as_float(o[e]) * f_x : 0.f;
-            if (ny > 0) {
-              tmem_ld32_raw(other_cols + c0, o);
-              tmem_wait_ld();
-              reg_fence(o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) f[e] = fmaf(__uint_as_float(o[e]), f_y, f[e]);
-            }
-            if (row_valid) {
-              if (bad) add_nonfinite(f, c0);
-              put(f, c0, inv);
-            }
-            __syncwarp();
+          for (int e = 0; e < 16; ++e) {
+            f[e] = nx > 0 ? __uint_as_float(o[e]) * f_x : 0.f;
+            if (ny > 0) f[e] = fmaf(__uint_as_float(u[e]), f_y, f[e]);
           }
+          if (bad && row_valid) {
+            // The non-finite values that this row sees among the replaced ones.
+            const int32_t seg_end = min(d.kbase + d.n * kKeys, d.kv_hi);
+#pragma unroll 1
+            for (int32_t k = max(d.kbase, d.kv_lo); k < seg_end; ++k) {
+              if (k >= d.lo_all && k < d.committed) {
+                k = d.committed - 1;
+                continue;
+              }
+              if (!(seen32(k) & 1u)) continue;
+              const int64_t blk = page_of(p, trow, k);
+              if (blk < 0) continue;
+              const uint32_t* v = reinterpret_cast<const uint32_t*>(
+                  reinterpret_cast<const T*>(p.cache) +
+                  ((p.num_slots + blk * p.block_size + k % p.block_size) * p.num_kv_heads + d.h) * 128 + c0);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const uint32_t w = __ldg(v + e), b = nonfinite2<T>(w);
+                if (b & 0x8000u) f[2 * e] += to_float(reinterpret_cast<const T*>(&w)[0]);
+                if (b & 0x80000000u) f[2 * e + 1] += to_float(reinterpret_cast<const T*>(&w)[1]);
+              }
+            }
+          }
+          if (d.slot >= 0) {
+            if (row_valid) {
+              float4* dst = p.part_o + (part * 32 + c0 / 4) * kPartRows + part_row;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                dst[e * kPartRows] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+            }
+          } else {
+            uint8_t* cell = qbuf + (c0 >> 6) * kHalf + row * 128;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              *reinterpret_cast<uint4*>(cell + (((((c0 & 63) >> 3) + e) ^ (row & 7)) << 4)) =
+                  make_uint4(pack2<T>(f[8 * e] * inv, f[8 * e + 1] * inv),
+                             pack2<T>(f[8 * e + 2] * inv, f[8 * e + 3] * inv),
+                             pack2<T>(f[8 * e + 4] * inv, f[8 * e + 5] * inv),
+                             pack2<T>(f[8 * e + 6] * inv, f[8 * e + 7] * inv));
+          }
+          __syncwarp();
         }
+        if (d.slot < 0) {
+          // Lane l stores 16-byte chunk l % 8 of row 4i + l / 8: whole lines.
+#pragma unroll 1
+          for (int hf = c_lo >> 6; hf < c_hi >> 6; ++hf)
+#pragma unroll 4
+            for (int it = 0; it < 8; ++it) {
+              const int r8 = 4 * it + (lane >> 3);  // row of this warp
+              const int64_t at = __shfl_sync(0xffffffffu, row_valid ? orow : -1, r8);
+              const uint4 v = *reinterpret_cast<const uint4*>(
+                  qbuf + hf * kHalf + (row - lane + r8) * 128 + (((lane & 7) ^ (r8 & 7)) << 4));
+              if (at >= 0)
+                *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + at * 128 + 64 * hf + 8 * (lane & 7)) = v;
+            }
+        }
+      }
+      // The staging buffer was the item's Q tile: a tile of its own is given
+      // back by one warpgroup's 4 warps, a shared one by all 8.
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar(kQEmpty + qslot));
+        if (d.two) mbar_arrive(bar(kQEmpty + qslot));
+      }
+      tc_fence_before();
+      if (!d.two) {
         // The next item's first P.V overwrites O: not before the other
         // warpgroup has read this stream's columns.
-        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kORead + y));
         if (!__all_sync(0xffffffffu, mbar_wait(bar(kORead + x), mc & 1))) {
@@ -993,72 +1014,96 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
 }
 
-// Joins the partials of the item that CTA b starts and does not finish, and
-// writes 0 to the rows that no request owns.  Block (b, y): 32 rows x 64
-// columns; a lane owns a row, so the partials (column chunks of 4, rows
-// adjacent) are read coalesced.
-constexpr int kMergeThreads = 256;
-constexpr int kMergeY = 2 * kPartRows / 32;
-constexpr int kZeroBlocks = 4;
+// Joins the partials of the items that were cut, and writes 0 to the rows that
+// no request owns.  Every block finds the cut items itself; a job is 32 rows x
+// 8 columns of one of them, a lane one row (the partials are column chunks of
+// 4 with the rows adjacent: coalesced), and the jobs go round all warps of the
+// grid, so that few items with many segments use the whole GPU too.  One block
+// per SM: launching more costs more than the work.
+constexpr int kMergeThreads = 1024;
 
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeParams p, int32_t ctas) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ int32_t job_end[kMaxTreeCtas];  // jobs of cut items 0 .. i
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t warp0 = (int64_t)warp * gridDim.x + blockIdx.x;  // neighbours on different SMs
+  const int64_t warps = (int64_t)gridDim.x * (kMergeThreads / 32);
   grid_dependency_wait();
-  if ((int)blockIdx.x >= ctas) {
-    const int64_t w0 = ((int64_t)(blockIdx.x - ctas) * gridDim.y + blockIdx.y) * (kMergeThreads / 32) + warp;
-    const int64_t warps = (int64_t)kZeroBlocks * gridDim.y * (kMergeThreads / 32);
-    for (int64_t t0 = 32 * w0; t0 < p.num_tokens; t0 += 32 * warps) {
-      const int64_t t = t0 + lane;
-      bool zero = false;
-      if (t < p.num_tokens) {
-        const int64_t r = find_request(p.qsl, p.num_requests, t);
-        TreeExtent e;
-        zero = r < 0 || !tree_extent(p, r, e);
-      }
-      for (uint32_t todo = __ballot_sync(0xffffffffu, zero); todo != 0; todo &= todo - 1) {
-        uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) +
-                                              (t0 + __ffs(todo) - 1) * p.num_q_heads * 128);
-        for (int e = lane; e < p.num_q_heads * 16; e += 32) dst[e] = make_uint4(0, 0, 0, 0);
-      }
-    }
-    return;
-  }
-  const CutRecord c = p.cuts[blockIdx.x];
-  if (!c.valid) return;
-  const int row = 32 * (blockIdx.y >> 1) + lane;  // of the item's two query tiles
-  const int chunk = 16 * (blockIdx.y & 1) + 2 * warp;
-  const int in_tile = row & (kRows - 1);
-  const int64_t tok = c.q0 + (int64_t)(row / kRows) * p.block_q + in_tile / p.group;
-  const bool valid = in_tile < p.group * p.block_q && tok < c.qe &&
-                     (row < kRows || c.tile_cost == kTileCost2);
-  if (!valid) return;
-  const int64_t b0 = blockIdx.x;
-  const int64_t b_last = (c.cost0 + kItemCost + (int64_t)(c.tiles - 1) * c.tile_cost) / c.share;
-  float m = -INFINITY, l = 0.f;
-  float o[8] = {};
-#pragma unroll 2
-  for (int64_t b = b0; b <= b_last; ++b) {
-    if (tile_at(b * c.share, c.cost0, c.tile_cost, c.tiles) >=
-        tile_at((b + 1) * c.share, c.cost0, c.tile_cost, c.tiles))
-      continue;  // no tile in that share
-    const int64_t part = 2 * b + (b == b0 ? 1 : 0);
-    const float2 ml = __ldcg(p.part_ml + part * kPartRows + row);
-    const float4 u = __ldcg(p.part_o + (part * 32 + chunk) * kPartRows + row);
-    const float4 v = __ldcg(p.part_o + (part * 32 + chunk + 1) * kPartRows + row);
-    const float m_new = fmaxf(m, ml.x), mu = m_new == -INFINITY ? 0.f : m_new;
-    const float f0 = ex2(m - mu), f1 = ex2(ml.x - mu);
-    m = m_new;
-    l = l * f0 + ml.y * f1;
-    const float add[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+  if (warp == 0) {
+    int32_t sum = 0;
+    for (int b0 = 0; b0 < ctas; b0 += 32) {
+      const int b = b0 + lane;
+      int32_t n = 0;
+      if (b < ctas && p.cuts[b].valid) n = (p.cuts[b].tile_cost == kTileCost2 ? 2 : 1) * (kRows / 32) * 16;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = o[e] * f0 + add[e] * f1;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int32_t u = __shfl_up_sync(0xffffffffu, n, o);
+        if (lane >= o) n += u;
+      }
+      if (b < ctas) job_end[b] = sum + n;
+      sum += __shfl_sync(0xffffffffu, n, 31);
+    }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int64_t orow = tok * p.num_q_heads + (int64_t)c.h * p.group + in_tile % p.group;
-  *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + orow * 128 + 4 * chunk) =
-      make_uint4(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv),
-                 pack2<T>(o[4] * inv, o[5] * inv), pack2<T>(o[6] * inv, o[7] * inv));
+  // Rows without an owner, 32 tokens to a warp.
+  for (int64_t t0 = 32 * warp0; t0 < p.num_tokens; t0 += 32 * warps) {
+    const int64_t t = t0 + lane;
+    bool zero = false;
+    if (t < p.num_tokens) {
+      const int64_t r = find_request(p.qsl, p.num_requests, t);
+      TreeExtent e;
+      zero = r < 0 || !tree_extent(p, r, e);
+    }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, zero); todo != 0; todo &= todo - 1) {
+      uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) +
+                                            (t0 + __ffs(todo) - 1) * p.num_q_heads * 128);
+      for (int e = lane; e < p.num_q_heads * 16; e += 32) dst[e] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  __syncthreads();
+  const int32_t jobs = job_end[ctas - 1];
+  for (int64_t job = warp0; job < jobs; job += warps) {
+    int lo = 0, hi = ctas - 1;  // the first cut item that ends behind this job
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (job_end[mid] > job)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    const int sub = (int)job - (lo > 0 ? job_end[lo - 1] : 0);
+    const CutRecord c = p.cuts[lo];
+    const int row = 32 * (sub >> 4) + lane;  // of the item's query tiles
+    const int chunk = 2 * (sub & 15);
+    const int in_tile = row & (kRows - 1);
+    const int64_t tok = c.q0 + (int64_t)(row / kRows) * p.block_q + in_tile / p.group;
+    if (in_tile >= p.group * p.block_q || tok >= c.qe) continue;
+    const int64_t b0 = lo;
+    const int64_t b_last = (c.cost0 + kItemCost + (int64_t)(c.tiles - 1) * c.tile_cost) / c.share;
+    float m = -INFINITY, l = 0.f;
+    float o[8] = {};
+#pragma unroll 4
+    for (int64_t b = b0; b <= b_last; ++b) {
+      if (tile_at(b * c.share, c.cost0, c.tile_cost, c.tiles) >=
+          tile_at((b + 1) * c.share, c.cost0, c.tile_cost, c.tiles))
+        continue;  // no tile in that share
+      const int64_t part = 2 * b + (b == b0 ? 1 : 0);
+      const float2 ml = __ldcg(p.part_ml + part * kPartRows + row);
+      const float4 u = __ldcg(p.part_o + (part * 32 + chunk) * kPartRows + row);
+      const float4 v = __ldcg(p.part_o + (part * 32 + chunk + 1) * kPartRows + row);
+      const float m_new = fmaxf(m, ml.x), mu = m_new == -INFINITY ? 0.f : m_new;
+      const float f0 = ex2(m - mu), f1 = ex2(ml.x - mu);
+      m = m_new;
+      l = l * f0 + ml.y * f1;
+      const float add[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = o[e] * f0 + add[e] * f1;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t orow = tok * p.num_q_heads + (int64_t)c.h * p.group + in_tile % p.group;
+    *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + orow * 128 + 4 * chunk) =
+        make_uint4(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv),
+                   pack2<T>(o[4] * inv, o[5] * inv), pack2<T>(o[6] * inv, o[7] * inv));
+  }
 }
 
 struct TreeDeviceState {
@@ -1197,7 +1242,7 @@ int launch_tree_attention(const TreeProblem& a) {
   const int rc = check_launch();
   if (rc != MVB_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(ctas + kZeroBlocks), kMergeY);
+  cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(kMergeThreads);
   cfg.stream = a.stream;
   cudaLaunchAttribute attr[1];

@@ -62,16 +62,15 @@ def attention_tolerance(size, reach, exact, dtype, keys: int, dim: int, largest:
     """Largest |out - exact| that the roundings allow, per output.
 
     u = finfo.eps / 2.  The output is rounded once: u(dtype) |exact|.  P is
-    rounded to the value's type before P.V: u(fp16) = 2^-11 of the weighted
-    |v| (``size``); bf16 P is kept as a sum of two bf16 (2^-16); fp32 keeps
-    it.  A score is a sum of dim products in fp32, off by at most
+    rounded to the value's type before P.V: u(dtype) of the weighted |v|
+    (``size``); fp32 keeps it.  A score is a sum of dim products in fp32, off by at most
     (dim + 2) 2^-23 times ``reach`` (the largest sum |q||k| scale, tensor
     cores truncating: one whole step per addition), which moves numerator
     and denominator by that factor each; the sums over the keys add keys
     2^-23 each, the exponential and the final division 2^-20."""
 
     rounded = torch.finfo(dtype).eps / 2
-    weight = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -16, torch.float32: 0.0}[dtype]
+    weight = 0.0 if dtype == torch.float32 else rounded
     score = 2 * (dim + 2) * 2.0 ** -23 * reach[..., None]
     relative = weight + score + 2 * keys * 2.0 ** -23 + 2.0 ** -20
     # Below 2^-14 an fp16 number (a P, or the output) is off by up to 2^-25;
