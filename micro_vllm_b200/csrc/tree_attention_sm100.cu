@@ -77,6 +77,8 @@ constexpr float kRescaleLog2 = 8.f;
 // Cost axis: a KV tile of an item with one or two query tiles, an item's
 // fixed part, and the least share of a CTA.
 constexpr int kTileCost1 = 4, kTileCost2 = 6, kItemCost = 20, kMinShare = 8;
+static_assert(kMinShare >= kTileCost1 && kMinShare >= kTileCost2,
+              "a share between an item's first and last holds a tile of it");
 
 constexpr int kPartRows = 2 * kRows;  // rows of one partial
 
@@ -116,7 +118,7 @@ struct ItemDesc {
 struct CutRecord {
   int64_t q0, qe, cost0;  // first token, end of tokens, place on the cost axis
   int64_t share;
-  int32_t h, tiles, tile_cost, valid;
+  int32_t h, tiles, two, valid;
 };
 
 struct TreeParams {
@@ -186,11 +188,16 @@ __device__ __forceinline__ RequestCost cost_of(const TreeParams& p, const TreeEx
   return c;
 }
 // First tile of an item at or behind cost position x (item at cost0).
-__host__ __device__ __forceinline__ int32_t tile_at(int64_t x, int64_t cost0, int32_t tile_cost,
-                                                    int32_t tiles) {
+__device__ __forceinline__ int32_t tile_at(int64_t x, int64_t cost0, bool two, int32_t tiles) {
   const int64_t d = x - cost0 - kItemCost;
-  const int64_t j = d <= 0 ? 0 : (d + tile_cost - 1) / tile_cost;
+  if (d <= 0) return 0;
+  const int64_t j = two ? (d + kTileCost2 - 1) / kTileCost2 : (d + kTileCost1 - 1) / kTileCost1;
   return (int32_t)(j < tiles ? j : tiles);
+}
+// a / b for a >= 0, b > 0; a 64-bit division is ~800 cycles on the way to
+// the first load of a CTA.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
 template <typename T>
@@ -238,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (w < warp) before += v;
     total += v;
   }
-  const int64_t share = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kMinShare);
+  const int64_t share = max(divide(total + gridDim.x - 1, gridDim.x), (int64_t)kMinShare);
   const int64_t my_lo = blockIdx.x * share, my_hi = min(my_lo + share, total);
   if (my_lo >= total) return;
   if (before <= my_lo && my_lo < before + mine) {
@@ -353,8 +360,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             h = pair = 0;
             if (cost0 < my_lo) {  // the share begins inside this request
               const int64_t in = my_lo - cost0;
-              h = (int32_t)(in / rc.head);
-              pair = (int32_t)min((in - h * rc.head) / rc.full, (int64_t)(rc.pairs - 1));
+              h = (int32_t)divide(in, rc.head);
+              pair = (int32_t)min(divide(in - h * rc.head, rc.full), (int64_t)(rc.pairs - 1));
               cost0 += h * rc.head + pair * rc.full;
             }
             fresh = false;
@@ -364,9 +371,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int64_t cost = last_pair ? rc.last : rc.full;
           d.q0 = e.qs + (int64_t)pair * 2 * p.block_q;
           d.two = d.q0 + p.block_q < e.qe ? 1 : 0;
-          const int32_t tile_cost = d.two ? kTileCost2 : kTileCost1;
-          const int32_t j0 = tile_at(my_lo, cost0, tile_cost, rc.tiles);
-          const int32_t j1 = tile_at(my_hi, cost0, tile_cost, rc.tiles);
+          const int32_t j0 = tile_at(my_lo, cost0, d.two, rc.tiles);
+          const int32_t j1 = tile_at(my_hi, cost0, d.two, rc.tiles);
           const bool some = j1 > j0;
           if (some) {
             d.r = (int32_t)r;
@@ -380,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             d.first = j0 == 0;
             d.last = j1 == rc.tiles;
             d.slot = d.first && d.last ? -1 : d.first ? 1 : 0;
-            if (d.first && !d.last) cut = {d.q0, e.qe, cost0, share, h, rc.tiles, tile_cost, 1};
+            if (d.first && !d.last) cut = {d.q0, e.qe, cost0, share, h, rc.tiles, d.two, 1};
           }
           cost0 += cost;
           if (!last_pair) {
@@ -1025,26 +1031,12 @@ constexpr int kMergeThreads = 1024;
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeParams p, int32_t ctas) {
   __shared__ int32_t job_end[kMaxTreeCtas];  // jobs of cut items 0 .. i
+  __shared__ int32_t warp_jobs[kMaxTreeCtas / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t warp0 = (int64_t)warp * gridDim.x + blockIdx.x;  // neighbours on different SMs
   const int64_t warps = (int64_t)gridDim.x * (kMergeThreads / 32);
-  grid_dependency_wait();
-  if (warp == 0) {
-    int32_t sum = 0;
-    for (int b0 = 0; b0 < ctas; b0 += 32) {
-      const int b = b0 + lane;
-      int32_t n = 0;
-      if (b < ctas && p.cuts[b].valid) n = (p.cuts[b].tile_cost == kTileCost2 ? 2 : 1) * (kRows / 32) * 16;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int32_t u = __shfl_up_sync(0xffffffffu, n, o);
-        if (lane >= o) n += u;
-      }
-      if (b < ctas) job_end[b] = sum + n;
-      sum += __shfl_sync(0xffffffffu, n, 31);
-    }
-  }
-  // Rows without an owner, 32 tokens to a warp.
+  // Rows without an owner, 32 tokens to a warp; the attention before does not
+  // write them, and its inputs were there before it began.
   for (int64_t t0 = 32 * warp0; t0 < p.num_tokens; t0 += 32 * warps) {
     const int64_t t = t0 + lane;
     bool zero = false;
@@ -1058,6 +1050,24 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
                                             (t0 + __ffs(todo) - 1) * p.num_q_heads * 128);
       for (int e = lane; e < p.num_q_heads * 16; e += 32) dst[e] = make_uint4(0, 0, 0, 0);
     }
+  }
+  grid_dependency_wait();
+  if (tid < kMaxTreeCtas) {
+    int32_t n = 0;
+    if (tid < ctas && p.cuts[tid].valid) n = (p.cuts[tid].two ? 2 : 1) * (kRows / 32) * 16;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int32_t u = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) n += u;
+    }
+    job_end[tid] = n;
+    if (lane == 31) warp_jobs[warp] = n;
+  }
+  __syncthreads();
+  if (tid < kMaxTreeCtas) {
+    int32_t before = 0;
+    for (int w = 0; w < warp; ++w) before += warp_jobs[w];
+    job_end[tid] += before;
   }
   __syncthreads();
   const int32_t jobs = job_end[ctas - 1];
@@ -1077,15 +1087,14 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
     const int in_tile = row & (kRows - 1);
     const int64_t tok = c.q0 + (int64_t)(row / kRows) * p.block_q + in_tile / p.group;
     if (in_tile >= p.group * p.block_q || tok >= c.qe) continue;
-    const int64_t b0 = lo;
-    const int64_t b_last = (c.cost0 + kItemCost + (int64_t)(c.tiles - 1) * c.tile_cost) / c.share;
+    // Every share from the item's first tile to its last holds some.
+    const int b0 = lo;
+    const int b_last = (int)divide(
+        c.cost0 + kItemCost + (int64_t)(c.tiles - 1) * (c.two ? kTileCost2 : kTileCost1), c.share);
     float m = -INFINITY, l = 0.f;
     float o[8] = {};
 #pragma unroll 4
-    for (int64_t b = b0; b <= b_last; ++b) {
-      if (tile_at(b * c.share, c.cost0, c.tile_cost, c.tiles) >=
-          tile_at((b + 1) * c.share, c.cost0, c.tile_cost, c.tiles))
-        continue;  // no tile in that share
+    for (int b = b0; b <= b_last; ++b) {
       const int64_t part = 2 * b + (b == b0 ? 1 : 0);
       const float2 ml = __ldcg(p.part_ml + part * kPartRows + row);
       const float4 u = __ldcg(p.part_o + (part * 32 + chunk) * kPartRows + row);
