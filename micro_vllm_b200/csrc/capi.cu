@@ -406,7 +406,9 @@ size_t mvb_tree_attention_workspace_size(int64_t max_num_tokens, int64_t max_num
   if (max_num_tokens < 0 || max_num_requests < 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
       head_dim <= 0)
     return 0;
-  return head_dim == 128 ? tree_workspace_bytes() : 256;
+  const size_t tc = head_dim == 128 ? tree_workspace_bytes() : 0;
+  const size_t exact = tree_generic_workspace_bytes(max_num_tokens, num_q_heads, head_dim);
+  return tc > exact ? tc : exact;
 }
 
 int mvb_tree_attention(const void* query, int64_t query_token_stride, int64_t query_head_stride,

@@ -242,6 +242,7 @@ struct TreeProblem : AttentionProblem {
   int32_t mask_words;
 };
 int launch_tree_attention_generic(const TreeProblem& p);
+size_t tree_generic_workspace_bytes(int64_t num_tokens, int32_t num_q_heads, int32_t head_dim);
 // The tensor-core kernel: CTAs at most (one per SM; they size its workspace),
 // what it takes, and its launch.
 constexpr int kMaxTreeCtas = 160;
