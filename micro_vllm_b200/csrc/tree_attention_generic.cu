@@ -41,7 +41,7 @@ struct GenericParams {
 __device__ __forceinline__ int64_t row_tiles(const TreeProblem& p, int64_t r, int32_t group) {
   TreeExtent e;
   if (!tree_extent(p, r, e)) return 0;
-  return ((e.qe - e.qs) * group + kRowTile - 1) / kRowTile;
+  return ((int32_t)(e.qe - e.qs) * group + kRowTile - 1) / kRowTile;
 }
 
 template <typename T>
@@ -127,24 +127,24 @@ __global__ void __launch_bounds__(kThreads) tree_attention_generic_kernel(const 
   if (r < 0) return;
   TreeExtent e;
   tree_extent(p, r, e);
-  const int64_t n_rows = (e.qe - e.qs) * group, row0 = found_tile * kRowTile;
+  // Rows and positions fit 32 bits (a context is at most 2^30 long); 64-bit
+  // divisions would cost microseconds before the first load.
+  const int32_t n_rows = (int32_t)(e.qe - e.qs) * group, row0 = (int32_t)found_tile * kRowTile;
 
   float* q_sh = sm;                                     // [kRowTile][dim4]
   float* k_sh = q_sh + kRowTile * dim4;                 // [kKeyTile][dim4 + 4]
   float* v_sh = k_sh + kKeyTile * (dim4 + 4);           // [kKeyTile][dim4]
   float* p_sh = v_sh + kKeyTile * dim4 + warp * kKeyTile * kWarpRows;  // this warp's [key][4 rows]
-  for (int i = tid; i < kRowTile * dim4; i += kThreads) {
-    const int64_t row = row0 + i / dim4;
-    const int32_t d = i % dim4;
-    float v = 0.f;
-    if (row < n_rows && d < dim)
-      v = to_float(static_cast<const T*>(
-          p.query)[(e.qs + row / group) * p.q_st + (int64_t)(h * group + row % group) * p.q_sh + d]);
-    q_sh[i] = v;
+  const int32_t wrow = row0 + warp * kWarpRows;  // this warp's rows
+  for (int i = 0; i < kWarpRows; ++i) {
+    const int32_t row = wrow + i;
+    const T* src = row < n_rows ? static_cast<const T*>(p.query) + (e.qs + row / group) * p.q_st +
+                                      (int64_t)(h * group + row % group) * p.q_sh
+                                : nullptr;
+    for (int d = lane; d < dim4; d += 32)
+      q_sh[(warp * kWarpRows + i) * dim4 + d] = src != nullptr && d < dim ? to_float(src[d]) : 0.f;
   }
 
-  // This warp's rows.
-  const int64_t wrow = row0 + warp * kWarpRows;
   const bool active = wrow < n_rows;
   int64_t tok[kWarpRows], lo_row[kWarpRows];
   int64_t lo_all = e.lo;
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kThreads) tree_attention_generic_kernel(const 
     const int64_t k0 = e.lo + j * kKeyTile;
     __syncthreads();  // the tile before is read
     if (tid < kKeyTile) {
-      const int64_t pos = k0 + tid, lb = pos / p.block_size;
+      const int32_t pos = (int32_t)k0 + tid, lb = pos / p.block_size;
       int64_t slot = -1;
       if (pos < e.hi) {
         const int64_t blk = lb < p.table_width ? __ldg(trow + lb) : -1;

@@ -1035,20 +1035,28 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t warp0 = (int64_t)warp * gridDim.x + blockIdx.x;  // neighbours on different SMs
   const int64_t warps = (int64_t)gridDim.x * (kMergeThreads / 32);
-  // Rows without an owner, 32 tokens to a warp; the attention before does not
-  // write them, and its inputs were there before it began.
-  for (int64_t t0 = 32 * warp0; t0 < p.num_tokens; t0 += 32 * warps) {
-    const int64_t t = t0 + lane;
-    bool zero = false;
-    if (t < p.num_tokens) {
-      const int64_t r = find_request(p.qsl, p.num_requests, t);
+  // Rows without an owner: before the first request, behind the last, and
+  // those of requests that do not fit.  The attention before does not write
+  // them, and its inputs were there before it began.
+  for (int64_t r0 = 32 * warp0; r0 < p.num_requests + 2; r0 += 32 * warps) {
+    const int64_t r = r0 + lane;
+    int64_t z0 = 0, z1 = 0;
+    if (r < p.num_requests) {
       TreeExtent e;
-      zero = r < 0 || !tree_extent(p, r, e);
+      if (!tree_extent(p, r, e)) z0 = e.qs, z1 = e.qe;
+    } else if (r == p.num_requests) {
+      z1 = p.num_requests > 0 ? __ldg(p.qsl) : p.num_tokens;
+    } else if (r == p.num_requests + 1 && p.num_requests > 0) {
+      z0 = __ldg(p.qsl + p.num_requests), z1 = p.num_tokens;
     }
-    for (uint32_t todo = __ballot_sync(0xffffffffu, zero); todo != 0; todo &= todo - 1) {
-      uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) +
-                                            (t0 + __ffs(todo) - 1) * p.num_q_heads * 128);
-      for (int e = lane; e < p.num_q_heads * 16; e += 32) dst[e] = make_uint4(0, 0, 0, 0);
+    z0 = max(z0, (int64_t)0);
+    z1 = min(z1, p.num_tokens);
+    for (uint32_t todo = __ballot_sync(0xffffffffu, z0 < z1); todo != 0; todo &= todo - 1) {
+      const int src = __ffs(todo) - 1;
+      const int64_t first = __shfl_sync(0xffffffffu, z0, src) * p.num_q_heads * 16;
+      const int64_t last = __shfl_sync(0xffffffffu, z1, src) * p.num_q_heads * 16;
+      for (int64_t e = first + lane; e < last; e += 32)
+        reinterpret_cast<uint4*>(p.out)[e] = make_uint4(0, 0, 0, 0);
     }
   }
   grid_dependency_wait();
