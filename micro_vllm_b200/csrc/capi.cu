@@ -512,6 +512,9 @@ int mvb_compact_draft_kv(void* const* layer_caches, int32_t num_layers, int64_t 
     return MVB_ERR_INVALID_ARGUMENT;
   for (int32_t i = 0; i < num_layers; ++i)
     if (!layer_caches[i] || ((uintptr_t)layer_caches[i] % eb) != 0) return MVB_ERR_INVALID_ARGUMENT;
+  for (int32_t i = 0; i < num_layers; ++i)  // a cache given twice would move twice
+    for (int32_t j = 0; j < i; ++j)
+      if (layer_caches[i] == layer_caches[j]) return MVB_ERR_INVALID_ARGUMENT;
   for (int32_t first = 0; first < num_layers; first += kMaxCompactLayers) {
     CompactArgs a;
     a.num_layers = num_layers - first < kMaxCompactLayers ? num_layers - first : kMaxCompactLayers;

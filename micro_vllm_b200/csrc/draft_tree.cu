@@ -156,27 +156,29 @@ __global__ void __launch_bounds__(kTreeThreads) accept_draft_tree_kernel(const A
 // Kept node k (path[k], strictly increasing) moves from logical position
 // C + path[k] to C + k in every layer and plane.  path[k] >= k, so a thread
 // that owns one column of the row and goes through k in order reads every
-// source before a store reaches it: no barrier between reads and writes.
+// source before a store reaches it: no barrier between reads and writes, and
+// kMoveBatch rows are loaded before the first of them is stored.  The bound is
+// HBM (a row is read once and written once); a block takes a few layers so
+// that the slot lookups (three dependent loads) are paid once for them.
+constexpr int kMoveBatch = 4, kMoveLayers = 4;
+
 template <typename Vec>
 __global__ void __launch_bounds__(256) compact_draft_kv_kernel(const CompactArgs a) {
   extern __shared__ int64_t slot_sh[];  // [max_accepted] sources, then targets
+  __shared__ int32_t moves_sh;
   const int64_t r = blockIdx.x;
-  const int tid = threadIdx.x;
-  const int64_t kept = a.num_accepted[r], c = a.committed[r];
+  const int tid = threadIdx.x, lane = tid & 31;
   int64_t* src = slot_sh;
   int64_t* dst = slot_sh + a.max_accepted;
-  int bits = 0;
-  if (kept < 0 || kept > a.max_accepted || c < 0 || c > kMaxContext) bits = MVB_STATUS_INCONSISTENT_COUNTS;
-  const int k_all = bits ? 0 : (int)kept;
-  for (int k = tid; k < k_all; k += blockDim.x) {
-    const int64_t node = a.nodes[r * a.max_accepted + k];
-    const int64_t before = k > 0 ? a.nodes[r * a.max_accepted + k - 1] : -1;
-    if (node <= before || node >= kMaxTreeNodes) {
-      bits |= MVB_STATUS_INCONSISTENT_COUNTS;
-      continue;
-    }
-    auto slot_of = [&](int64_t logical) -> int64_t {
-      const int64_t page = logical / a.block_size;
+  // One warp lists the rows that move, in order; -1 rows for a request with a
+  // bad entry, which is left as it was in every layer.
+  if (tid < 32) {
+    const int64_t kept = a.num_accepted[r], c = a.committed[r];
+    int bits = 0;
+    if (kept < 0 || kept > a.max_accepted || c < 0 || c > kMaxContext) bits = MVB_STATUS_INCONSISTENT_COUNTS;
+    const int k_all = bits ? 0 : (int)kept;
+    auto slot_of = [&](int32_t logical) -> int64_t {
+      const int32_t page = logical / (int32_t)a.block_size;
       if (page >= a.table_width) {
         bits |= MVB_STATUS_POSITION_PAST_TABLE;
         return -1;
@@ -186,23 +188,62 @@ __global__ void __launch_bounds__(256) compact_draft_kv_kernel(const CompactArgs
         bits |= MVB_STATUS_BLOCK_OUT_OF_RANGE;
         return -1;
       }
-      return blk * a.block_size + logical % a.block_size;
+      return blk * a.block_size + (logical - page * (int32_t)a.block_size);
     };
-    src[k] = node == k ? -1 : slot_of(c + node);
-    dst[k] = node == k ? -1 : slot_of(c + k);
+    int moves = 0;
+    int64_t last = -1;  // node of the 32 before
+    for (int k0 = 0; k0 < k_all; k0 += 32) {
+      const int k = k0 + lane;
+      const int64_t node = k < k_all ? a.nodes[r * a.max_accepted + k] : 0;
+      int64_t before = __shfl_up_sync(0xffffffffu, node, 1);
+      if (lane == 0) before = last;
+      last = __shfl_sync(0xffffffffu, node, 31);
+      bool move = false;
+      int64_t from = -1, to = -1;
+      if (k < k_all) {
+        if (node <= before || node >= kMaxTreeNodes) {
+          bits |= MVB_STATUS_INCONSISTENT_COUNTS;
+        } else if (node != k) {
+          move = true;
+          from = slot_of((int32_t)(c + node));
+          to = slot_of((int32_t)c + k);
+        }
+      }
+      const uint32_t m = __ballot_sync(0xffffffffu, move);
+      if (move) {
+        const int at = moves + __popc(m & ((1u << lane) - 1u));
+        src[at] = from * a.row_vecs;
+        dst[at] = to * a.row_vecs;
+      }
+      moves += __popc(m);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) bits |= __shfl_xor_sync(0xffffffffu, bits, o);
+    if (lane == 0) {
+      if (bits && a.status) atomicOr(a.status, bits);
+      moves_sh = bits ? 0 : moves;
+    }
   }
-  if (bits && a.status) atomicOr(a.status, bits);
-  // A request with a bad entry is left as it was, in every layer.
-  if (__syncthreads_or(bits)) return;
+  __syncthreads();
+  const int moves = moves_sh;
   const int64_t row_vecs = a.row_vecs;
   const int64_t plane = a.num_blocks * a.block_size * row_vecs;
-  const int64_t columns = 2 * row_vecs;
-  for (int layer = blockIdx.y; layer < a.num_layers; layer += gridDim.y) {
-    Vec* cache = static_cast<Vec*>(a.layers[layer]);
-    for (int64_t col = tid; col < columns; col += blockDim.x) {
-      Vec* base = cache + (col >= row_vecs ? plane + (col - row_vecs) : col);
-      for (int k = 0; k < k_all; ++k)
-        if (src[k] >= 0) base[dst[k] * row_vecs] = base[src[k] * row_vecs];
+  const int layer0 = blockIdx.y * a.layers_per_block;
+  const int layer1 = min(layer0 + a.layers_per_block, a.num_layers);
+  for (int64_t col = tid; col < 2 * row_vecs; col += blockDim.x) {
+    const int64_t at = col >= row_vecs ? plane + (col - row_vecs) : col;
+    for (int k0 = 0; k0 < moves; k0 += kMoveBatch) {
+#pragma unroll 2
+      for (int layer = layer0; layer < layer1; ++layer) {
+        Vec* base = static_cast<Vec*>(a.layers[layer]) + at;
+        Vec v[kMoveBatch];
+#pragma unroll
+        for (int u = 0; u < kMoveBatch; ++u)
+          if (k0 + u < moves) v[u] = base[src[k0 + u]];
+#pragma unroll
+        for (int u = 0; u < kMoveBatch; ++u)
+          if (k0 + u < moves) base[dst[k0 + u]] = v[u];
+      }
     }
   }
 }
@@ -221,7 +262,11 @@ int launch_accept_draft_tree(const AcceptArgs& a) {
 
 int launch_compact_draft_kv(CompactArgs a, int64_t row_bytes, bool aligned16) {
   const size_t smem = (size_t)2 * a.max_accepted * sizeof(int64_t);
-  const dim3 grid((unsigned)a.num_requests, (unsigned)a.num_layers);
+  // One layer to a block while that leaves SMs idle.
+  const int64_t blocks = a.num_requests * a.num_layers / (4 * (int64_t)num_sms());
+  a.layers_per_block = blocks < 1 ? 1 : blocks > kMoveLayers ? kMoveLayers : (int32_t)blocks;
+  const dim3 grid((unsigned)a.num_requests,
+                  (unsigned)((a.num_layers + a.layers_per_block - 1) / a.layers_per_block));
   if (aligned16 && row_bytes % 16 == 0) {
     a.row_vecs = row_bytes / 16;
     compact_draft_kv_kernel<uint4><<<grid, 256, smem, a.stream>>>(a);

@@ -226,7 +226,7 @@ int launch_accept_draft_tree(const AcceptArgs& a);
 
 struct CompactArgs {
   void* layers[kMaxCompactLayers];
-  int32_t num_layers, max_accepted;
+  int32_t num_layers, max_accepted, layers_per_block;
   int64_t num_blocks, block_size, row_vecs;
   const int64_t *block_table, *committed, *nodes, *num_accepted;
   int64_t table_stride, table_width, num_requests;

@@ -22,7 +22,6 @@ rotated at committed + depth(i).
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
 from dataclasses import dataclass
 
 import torch
@@ -65,10 +64,17 @@ class AcceptedDraft:
     last_rows: torch.Tensor
 
 
-def on_device(device: torch.device):
-    """Makes ``device`` current for a launch on one of its streams."""
+def launch(entry, device: torch.device, what: str, *args) -> None:
+    """Calls a C entry whose last argument is the stream, with ``device``
+    current and on its current stream, and raises for its status."""
 
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    if torch.cuda.current_device() == device.index:
+        rc = entry(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc != _lib.MVB_OK:
+        _lib.check(rc, what)
 
 
 def _vector(name: str, t: torch.Tensor, device: torch.device, size: int | None = None) -> torch.Tensor:
@@ -127,14 +133,13 @@ def build_draft_tree(
     table = _table(block_table, device, requests)
     buffer = torch.empty(rows * (3 + words) + requests, dtype=torch.int64, device=device)
     positions, context_starts, slots, mask, lengths = buffer.split((rows, rows, rows, rows * words, requests))
-    with on_device(device):
-        rc = _lib.load().mvb_build_draft_tree(
-            parents.data_ptr(), starts.data_ptr(), committed.data_ptr(), table.data_ptr(),
-            table.stride(0), table.shape[1], rows, requests, block_size, kind, param, words,
-            positions.data_ptr(), context_starts.data_ptr(), lengths.data_ptr(), slots.data_ptr(),
-            mask.data_ptr(), _status(status, device), torch.cuda.current_stream(device).cuda_stream,
-        )
-    _lib.check(rc, "b200_paged draft tree")
+    launch(
+        _lib.load().mvb_build_draft_tree, device, "b200_paged draft tree",
+        parents.data_ptr(), starts.data_ptr(), committed.data_ptr(), table.data_ptr(),
+        table.stride(0), table.shape[1], rows, requests, block_size, kind, param, words,
+        positions.data_ptr(), context_starts.data_ptr(), lengths.data_ptr(), slots.data_ptr(),
+        mask.data_ptr(), _status(status, device),
+    )
     return DraftTree(
         AttentionMetadata(
             query_positions=positions, query_context_start_positions=context_starts,
@@ -177,14 +182,12 @@ def accept_draft_tree(
     buffer = torch.empty(requests * (2 * max_accepted + 3), dtype=torch.int64, device=device)
     cells = requests * max_accepted
     nodes, tokens, count, lengths, last = buffer.split((cells, cells, requests, requests, requests))
-    with on_device(device):
-        rc = _lib.load().mvb_accept_draft_tree(
-            draft.data_ptr(), target.data_ptr(), parents.data_ptr(), starts.data_ptr(), committed.data_ptr(),
-            rows, requests, max_accepted, nodes.data_ptr(), count.data_ptr(), tokens.data_ptr(),
-            lengths.data_ptr(), last.data_ptr(), _status(status, device),
-            torch.cuda.current_stream(device).cuda_stream,
-        )
-    _lib.check(rc, "b200_paged draft acceptance")
+    launch(
+        _lib.load().mvb_accept_draft_tree, device, "b200_paged draft acceptance",
+        draft.data_ptr(), target.data_ptr(), parents.data_ptr(), starts.data_ptr(), committed.data_ptr(),
+        rows, requests, max_accepted, nodes.data_ptr(), count.data_ptr(), tokens.data_ptr(),
+        lengths.data_ptr(), last.data_ptr(), _status(status, device),
+    )
     return AcceptedDraft(nodes.view(requests, max_accepted), count, tokens.view(requests, max_accepted), lengths, last)
 
 
@@ -212,6 +215,8 @@ class DraftKVCompactor:
                 raise ValueError("layer caches must share one shape, dtype and device")
         if first.numel() == 0:
             raise ValueError("layer caches must not be empty")
+        if len({t.data_ptr() for t in caches}) != len(caches):
+            raise ValueError("layer caches must be distinct: a row would move twice")
         self.layer_kv_caches = caches
         self._device = first.device
         self._dtype = _CACHE_DTYPES[first.dtype]
@@ -244,11 +249,9 @@ class DraftKVCompactor:
             nodes = nodes.contiguous()
         blocks, block_size, kv_heads, head_dim = self._sizes
         pointers = (ctypes.c_void_p * len(self.layer_kv_caches))(*(t.data_ptr() for t in self.layer_kv_caches))
-        with on_device(device):
-            rc = _lib.load().mvb_compact_draft_kv(
-                pointers, len(pointers), blocks, block_size, kv_heads, head_dim, self._dtype,
-                table.data_ptr(), table.stride(0), table.shape[1], committed.data_ptr(), nodes.data_ptr(),
-                count.data_ptr(), requests, nodes.shape[1], _status(status, device),
-                torch.cuda.current_stream(device).cuda_stream,
-            )
-        _lib.check(rc, "b200_paged KV move")
+        launch(
+            _lib.load().mvb_compact_draft_kv, device, "b200_paged KV move",
+            pointers, len(pointers), blocks, block_size, kv_heads, head_dim, self._dtype,
+            table.data_ptr(), table.stride(0), table.shape[1], committed.data_ptr(), nodes.data_ptr(),
+            count.data_ptr(), requests, nodes.shape[1], _status(status, device),
+        )

@@ -16,7 +16,7 @@ from abc import ABC, abstractmethod
 import torch
 
 from micro_vllm_b200 import _lib
-from micro_vllm_b200.draft_tree import on_device
+from micro_vllm_b200.draft_tree import launch
 
 OPERATOR_NAME = "b200_paged"
 
@@ -242,7 +242,7 @@ class B200PagedAttentionOperator(AttentionOperator):
         if key.device != query.device or value.device != query.device:
             raise ValueError("query, key, value and layer_kv_cache must be on one device")
         self._check_tree(query, layer_kv_cache, tree)
-        with on_device(query.device):
+        with torch.cuda.device(query.device):
             write_kv_cache(key, value, layer_kv_cache, tree.attention)
         return self.attend_tree(query, layer_kv_cache, tree)
 
@@ -299,18 +299,16 @@ class B200PagedAttentionOperator(AttentionOperator):
             table = table.contiguous()
         output = torch.empty((num_tokens, num_q_heads, head_dim), dtype=query.dtype, device=device)
         nbytes = self._lib.mvb_tree_attention_workspace_size(num_tokens, num_requests, num_q_heads, num_kv_heads, head_dim)
-        with on_device(device):
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-            rc = self._lib.mvb_tree_attention(
-                query.data_ptr(), query.stride(0), query.stride(1), output.data_ptr(),
-                layer_kv_cache.data_ptr(), num_blocks, block_size, num_kv_heads, head_dim,
-                md_start.data_ptr(), md_qsl.data_ptr(), md_ctx.data_ptr(),
-                table.data_ptr(), table.stride(0), table.shape[1], mask.data_ptr(), mask.shape[1],
-                num_tokens, num_requests, num_q_heads, 1.0 / math.sqrt(head_dim), dtype,
-                workspace.data_ptr(), nbytes, self._state(device).status.data_ptr(),
-                torch.cuda.current_stream(device).cuda_stream,
-            )
-        _lib.check(rc, "b200_paged tree attention")
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        launch(
+            self._lib.mvb_tree_attention, device, "b200_paged tree attention",
+            query.data_ptr(), query.stride(0), query.stride(1), output.data_ptr(),
+            layer_kv_cache.data_ptr(), num_blocks, block_size, num_kv_heads, head_dim,
+            md_start.data_ptr(), md_qsl.data_ptr(), md_ctx.data_ptr(),
+            table.data_ptr(), table.stride(0), table.shape[1], mask.data_ptr(), mask.shape[1],
+            num_tokens, num_requests, num_q_heads, 1.0 / math.sqrt(head_dim), dtype,
+            workspace.data_ptr(), nbytes, self._state(device).status.data_ptr(),
+        )
         return output
 
 

@@ -123,6 +123,7 @@ def test_c_entries_refuse_before_touching_the_device(lib) -> None:
     assert move(dt=9) == dtype and move(n=0) == move(requests=0) == ok
     assert move(n=-1) == move(bs=0) == move(hkv=0) == move(d=0) == move(most=0) == move(most=1025) == bad
     assert move(caches=None) == move(nodes=None) == bad
+    assert move(caches=(ctypes.c_void_p * 2)(256, 256)) == bad
     assert move(caches=(ctypes.c_void_p * 2)(256, None)) == move(caches=(ctypes.c_void_p * 2)(256, 257)) == bad
 
 

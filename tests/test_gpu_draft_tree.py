@@ -426,6 +426,8 @@ def test_kv_move_leaves_requests_that_do_not_fit() -> None:
         DraftKVCompactor([gpu.cache, gpu.cache.float()])
     with pytest.raises(ValueError, match="contiguous"):
         DraftKVCompactor([gpu.cache[:, ::2]])
+    with pytest.raises(ValueError, match="distinct"):
+        DraftKVCompactor([gpu.cache, gpu.cache])
 
 
 # --------------------------------------------------------- steps in a row
