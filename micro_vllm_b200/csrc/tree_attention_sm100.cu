@@ -480,16 +480,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           umma_commit(bar(kPvDone + x));
         };
-        // A probe costs ~200 cycles, so what usually is there goes in one batch:
-        // V of tile c (landed, fixed) and, if `more`, the K tile ck.
-        auto wait_vk = [&](uint32_t c, bool more, uint32_t ck) -> bool {
+        // A probe costs ~200 cycles: V of tile c (landed and fixed) and, if
+        // `more`, K tile ck go in one batch, while the MMAs issued before run.
+        // V is waited for; k_ready says whether K is there.
+        bool k_ready = true;
+        auto wait_v = [&](uint32_t c, bool more, uint32_t ck) -> bool {
           const uint32_t vf = bar(kVFull + vslot(c)), vr = bar(kVReady + vslot(c));
           const uint32_t kf = more ? bar(kKFull + kslot(ck)) : vr;
           const uint32_t kp = more ? kphase(ck) : vphase(c);
-          bool r0, r1, r2;
-          mbar_test3(vf, vphase(c), vr, vphase(c), kf, kp, r0, r1, r2);
-          return (r0 || mbar_wait(vf, vphase(c))) && (r1 || mbar_wait(vr, vphase(c))) &&
-                 (r2 || mbar_wait(kf, kp));
+          bool r0, r1;
+          mbar_test3(vf, vphase(c), vr, vphase(c), kf, kp, r0, r1, k_ready);
+          return (r0 || mbar_wait(vf, vphase(c))) && (r1 || mbar_wait(vr, vphase(c)));
+        };
+        auto wait_k = [&](uint32_t ck) -> bool {
+          if (k_ready) return true;
+          const bool there = mbar_wait(bar(kKFull + kslot(ck)), kphase(ck));
+          tc_fence_after();
+          return there;
         };
         bool ok = true;
         for (uint32_t i = 0; ok; ++i) {
@@ -514,18 +521,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             issue_s(1, qs1, kslot(kvc));
             umma_commit(bar(kKEmpty + kslot(kvc)));
+            ok = wait_v(kvc, n > 1, kvc + 1);
             for (int j = 0; ok && j < n; ++j) {
               const uint32_t c = kvc + j;
               for (int x = 0; x < 2; ++x) {
-                ok = mbar_wait(bar(kPFull + x), ((x == 0 ? tc0 : tc1) + j) & 1) &&
-                     (x == 1 || wait_vk(c, j + 1 < n, c + 1));
+                ok = mbar_wait(bar(kPFull + x), ((x == 0 ? tc0 : tc1) + j) & 1);
                 if (!ok) break;
                 tc_fence_after();
                 issue_pv(x, vslot(c), j > 0);
                 if (x == 1) umma_commit(bar(kVEmpty + vslot(c)));
                 if (j + 1 < n) {
+                  ok = x == 1 || wait_k(c + 1);
+                  if (!ok) break;
                   issue_s(x, x == 0 ? qs0 : qs1, kslot(c + 1));
-                  if (x == 1) umma_commit(bar(kKEmpty + kslot(c + 1)));
+                  if (x == 1) {
+                    umma_commit(bar(kKEmpty + kslot(c + 1)));
+                    ok = wait_v(c + 1, j + 2 < n, c + 2);
+                  }
                 }
               }
             }
@@ -538,19 +550,22 @@ __global__ void __launch_bounds__(kThreads, 1)
               issue_s(1, qs0, kslot(kvc + 1));
               umma_commit(bar(kKEmpty + kslot(kvc + 1)));
             }
+            ok = wait_v(kvc, n > 2, kvc + 2);
             for (int j = 0; ok && j < n; ++j) {
               const uint32_t c = kvc + j;
               const int x = j & 1;
-              ok = mbar_wait(bar(kPFull + x), ((x == 0 ? tc0 : tc1) + (j >> 1)) & 1) &&
-                   wait_vk(c, j + 2 < n, c + 2);
+              ok = mbar_wait(bar(kPFull + x), ((x == 0 ? tc0 : tc1) + (j >> 1)) & 1);
               if (!ok) break;
               tc_fence_after();
               issue_pv(x, vslot(c), j > 1);
               umma_commit(bar(kVEmpty + vslot(c)));
               if (j + 2 < n) {
+                ok = wait_k(c + 2);
+                if (!ok) break;
                 issue_s(x, qs0, kslot(c + 2));
                 umma_commit(bar(kKEmpty + kslot(c + 2)));
               }
+              if (j + 1 < n) ok = wait_v(c + 1, j + 3 < n, c + 3);
             }
           }
           if (!ok) break;
