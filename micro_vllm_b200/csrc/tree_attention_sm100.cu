@@ -20,17 +20,19 @@
 // cut by share borders leaves fp32 partials (at most a head and a tail per
 // CTA), which the merge launch behind joins in a fixed order.
 //
-// Inside a CTA (12 warps, roles without a block-wide barrier between items):
+// Inside a CTA (16 warps, roles without a block-wide barrier between items):
 //   warp 11   scheduler: describes the next item in a 2-slot ring, loads its Q
 //   warps 8, 10  TMA producers of K (2 stages) and V (3 stages)
 //   warp 9    MMA issuer
 //   warps 0-3, 4-7  softmax of stream 0 and 1, one thread per row
+//   warps 12-15  epilogue: joins, normalises and writes an item while the
+//             softmax warps are in the next one
 // The two streams each own S/P and O columns in TMEM.  With two query tiles
 // (more than 128 rows) a stream is a query tile and both read every K/V tile.
 // With one, both streams hold the same query tile and take the even and the
 // odd key tiles: one stream's softmax runs under the other's MMAs, which a
 // single tile could not overlap, and the streams' (m, l, O) merge in the
-// epilogue, each warpgroup normalising half of the columns.
+// epilogue.
 //
 // Rows of V that a query row does not see but another row does (other
 // branches, window edges) may hold infinities or NaN, and 0 x NaN would reach
@@ -60,14 +62,16 @@ constexpr int kOffQ = 0;
 constexpr int kOffK = kQStages * kTileBytes;
 constexpr int kOffV = kOffK + kKStages * kTileBytes;
 constexpr int kSmemBytes = kOffV + kVStages * kTileBytes;  // 224 KiB of the SM's 227
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
 constexpr int kKProdWarp = 8, kMmaWarp = 9, kSchedWarp = 11;  // warp 10: V producer
-constexpr int kItemSlots = 2;
-constexpr int kItemReaders = 11;
-constexpr int kFlagSlots = 8;  // items whose V flag may still be read: V runs at most 3 tiles ahead
-// Register split (setmaxnreg): 2 x 128 x 200 + 128 x 96 <= 384 x 168.
-constexpr int kLaunchRegs = 168, kSoftmaxRegs = 200, kOtherRegs = 96;
-static_assert(2 * 128 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs,
+constexpr int kEpiWarp = 12;                                  // warps 12-15: epilogue
+constexpr int kItemSlots = 4;
+constexpr int kItemReaders = 15;
+constexpr int kFlagSlots = 8;  // items whose V flag may still be read (more than kItemSlots)
+// Register split (setmaxnreg) of the launch's 512 x 128 between the two
+// softmax warpgroups, the epilogue's and the one of the other roles.
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kEpiRegs = 96, kOtherRegs = 80;
+static_assert(2 * 128 * kSoftmaxRegs + 128 * kEpiRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs,
               "register split must fit the launch's registers");
 constexpr uint32_t kTmemCols = 512;
 __device__ __forceinline__ uint32_t col_s(int x) { return 128u * (uint32_t)x; }
@@ -94,8 +98,8 @@ enum Bar : int {
   kPFull = kSFull + 2,           // +stream
   kPvDone = kPFull + 2,          // +stream
   kMl = kPvDone + 2,             // +stream: its (m, l) are in shared memory
-  kORead = kMl + 2,              // +stream: the other warpgroup has read its O
-  kItemFull = kORead + 2,
+  kORead = kMl + 2,              // the epilogue has read (m, l) and O of both streams
+  kItemFull = kORead + 1,
   kItemEmpty = kItemFull + kItemSlots,
   kFinal = kItemEmpty + kItemSlots,
   kNumBars = kFinal + 1,
@@ -273,10 +277,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tensormap(&qmap);
     prefetch_tensormap(&kvmap);
     for (int i = 0; i < kNumBars; ++i) {
-      const bool four = (i >= kPFull && i < kPFull + 2) || (i >= kMl && i < kORead + 2);
+      const bool four = (i >= kPFull && i < kPFull + 2) || (i >= kMl && i <= kORead) ||
+                        (i >= kQEmpty && i < kQEmpty + kQStages);
       const bool readers = i >= kItemEmpty && i < kItemEmpty + kItemSlots;
-      const bool eight = i >= kQEmpty && i < kQEmpty + kQStages;
-      mbar_init(bar(i), readers ? kItemReaders : eight ? 8 : four ? 4 : 1);
+      mbar_init(bar(i), readers ? kItemReaders : four ? 4 : 1);
     }
     mbar_init_fence();
     abort_sh = 0;
@@ -302,14 +306,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   // of its own, else every other one.
   auto stream_tiles = [](const ItemDesc& d, int x) { return d.two ? d.n : (d.n + 1 - x) >> 1; };
   // Running counts (identical in every role): KV tiles of this CTA, tiles per
-  // stream, Q tiles, items with one query tile.
-  uint32_t kvc = 0, tc0 = 0, tc1 = 0, qc = 0, mc = 0;
+  // stream, Q tiles.
+  uint32_t kvc = 0, tc0 = 0, tc1 = 0, qc = 0;
   auto advance = [&](const ItemDesc& d) {
     kvc += (uint32_t)d.n;
     tc0 += (uint32_t)stream_tiles(d, 0);
     tc1 += (uint32_t)stream_tiles(d, 1);
     qc += d.two ? 2 : 1;
-    mc += d.two ? 0 : 1;
   };
   auto fail = [&]() {
     if (lane == 0) atomicOr(&abort_sh, 1);
@@ -319,7 +322,175 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto vslot = [](uint32_t c) { return c % kVStages; };
   auto vphase = [](uint32_t c) { return (c / kVStages) & 1; };
 
-  if (warp >= kKProdWarp) {
+  // The row's keys among 32 from position k (row of token tok, window lo_q).
+  auto seen32 = [&](const ItemDesc& d, int32_t lo_q, const uint64_t* mrow, uint64_t mask0,
+                    int32_t k) -> uint32_t {
+    const int32_t a = min(max(lo_q - k, 0), 32), b = min(max(d.committed - k, 0), 32);
+    const uint32_t below_a = a >= 32 ? ~0u : (1u << a) - 1u, below_b = b >= 32 ? ~0u : (1u << b) - 1u;
+    uint32_t bits = below_b & ~below_a;
+    const int32_t j = k - d.committed, nodes = d.kv_hi - d.committed;  // first node of the 32
+    if (j > -32 && j < nodes) {
+      uint32_t tree;
+      if (j <= 0) {
+        tree = (uint32_t)(mask0 << (-j));
+      } else {
+        const int w = j >> 6, sh = j & 63;
+        uint64_t v = (w == 0 ? mask0 : __ldg(mrow + w)) >> sh;
+        if (sh > 32 && w + 1 < p.mask_words) v |= __ldg(mrow + w + 1) << (64 - sh);
+        tree = (uint32_t)v;
+      }
+      if (nodes - j < 32) tree &= (1u << (nodes - j)) - 1u;
+      bits |= tree;
+    }
+    return bits;
+  };
+
+  if (warp >= kEpiWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kEpiRegs));
+    // ------------------------------------------------ epilogue
+    // Joins the streams, normalises, and writes the item's rows or its
+    // partial, while the softmax warpgroups are in the next item.  The loop
+    // bodies are small: they run once per item, so fetching them counts.
+    const int row = 32 * (warp & 3) + lane;  // TMEM lane of this thread
+    const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
+    const int row_tok = row / p.group, row_head = row % p.group;
+    for (uint32_t i = 0;; ++i) {
+      ItemDesc d;
+      if (!take_item(i, d)) {
+        fail();
+        break;
+      }
+      if (d.r < 0 || *abort_flag != 0) break;
+      const int n0 = stream_tiles(d, 0), n1 = stream_tiles(d, 1);
+      // A stream's last S is complete once its (m, l) are here, so its P.V
+      // barrier is in the last tile's phase or just behind it.
+      bool arrived = mbar_wait(bar(kMl), i & 1) && mbar_wait(bar(kMl + 1), i & 1) &&
+                     mbar_wait(bar(kPvDone), (tc0 + n0 - 1) & 1);
+      if (n1 > 0) arrived = arrived && mbar_wait(bar(kPvDone + 1), (tc1 + n1 - 1) & 1);
+      if (!__all_sync(0xffffffffu, arrived)) {
+        fail();
+        break;
+      }
+      tc_fence_after();
+      const bool bad = bad_v_sh[i % kFlagSlots] != 0;
+      const float2 ml[2] = {ml_sh[0][row], ml_sh[1][row]};
+      const int64_t part = (int64_t)blockIdx.x * 2 + d.slot;
+      const int passes = d.two ? 2 : 1;
+#pragma unroll 1
+      for (int t = 0; t < passes; ++t) {  // query tiles
+        const int64_t tok = d.q0 + (int64_t)t * p.block_q + row_tok;
+        const bool row_valid = row < p.group * p.block_q && tok < d.qe;
+        if (__any_sync(0xffffffffu, row_valid)) {
+          float m_all = t == 0 ? ml[0].x : ml[1].x, l_all = t == 0 ? ml[0].y : ml[1].y;
+          float f_a = 1.f, f_b = 0.f;
+          const bool both = !d.two && n1 > 0;  // the row's other keys are in stream 1
+          if (both) {
+            m_all = fmaxf(ml[0].x, ml[1].x);
+            const float mu = m_all == -INFINITY ? 0.f : m_all;
+            f_a = ex2(ml[0].x - mu);
+            f_b = ex2(ml[1].x - mu);
+            l_all = ml[0].y * f_a + ml[1].y * f_b;
+          }
+          const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+          const int64_t orow = tok * p.num_q_heads + (int64_t)d.h * p.group + row_head;
+          const int part_row = t * kRows + row;
+          if (d.slot >= 0 && row_valid) p.part_ml[part * kPartRows + part_row] = make_float2(m_all, l_all);
+          // Every S of the item is done with its Q tile, which stages the output.
+          uint8_t* qbuf = smem + kOffQ + (int)((qc + (uint32_t)t) % kQStages) * kTileBytes;
+#pragma unroll 1
+          for (int c0 = 0; c0 < 128; c0 += 16) {
+            uint32_t o[16], u[16];
+            tmem_ld16_raw(tmem + lane_base + col_o(t) + c0, o);
+            if (both) tmem_ld16_raw(tmem + lane_base + col_o(1) + c0, u);
+            tmem_wait_ld();
+            reg_fence(o);
+            reg_fence(u);
+            float f[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              f[e] = __uint_as_float(o[e]) * f_a;
+              if (both) f[e] = fmaf(__uint_as_float(u[e]), f_b, f[e]);
+            }
+            if (bad && row_valid) {
+              // The non-finite values that this row sees among the replaced ones.
+              const int64_t* trow = p.table + (int64_t)d.r * p.table_stride;
+              const uint64_t* mrow = reinterpret_cast<const uint64_t*>(p.mask) + tok * p.mask_words;
+              const int32_t lo_q =
+                  (int32_t)min(max((int64_t)d.kv_lo, __ldg(p.qstart + tok)), (int64_t)d.committed);
+              const int32_t seg_end = min(d.kbase + d.n * kKeys, d.kv_hi);
+#pragma unroll 1
+              for (int32_t k = max(d.kbase, d.kv_lo); k < seg_end; ++k) {
+                if (k >= d.lo_all && k < d.committed) {
+                  k = d.committed - 1;
+                  continue;
+                }
+                if (!(seen32(d, lo_q, mrow, __ldg(mrow), k) & 1u)) continue;
+                const int64_t blk = page_of(p, trow, k);
+                if (blk < 0) continue;
+                const uint32_t* v = reinterpret_cast<const uint32_t*>(
+                    reinterpret_cast<const T*>(p.cache) +
+                    ((p.num_slots + blk * p.block_size + k % p.block_size) * p.num_kv_heads + d.h) * 128 + c0);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const uint32_t w = __ldg(v + e), b = nonfinite2<T>(w);
+                  if (b & 0x8000u) f[2 * e] += to_float(reinterpret_cast<const T*>(&w)[0]);
+                  if (b & 0x80000000u) f[2 * e + 1] += to_float(reinterpret_cast<const T*>(&w)[1]);
+                }
+              }
+            }
+            if (d.slot >= 0) {
+              if (row_valid) {
+                float4* dst = p.part_o + (part * 32 + c0 / 4) * kPartRows + part_row;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  dst[e * kPartRows] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+              }
+            } else {
+              uint8_t* cell = qbuf + (c0 >> 6) * kHalf + row * 128;
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                *reinterpret_cast<uint4*>(cell + (((((c0 & 63) >> 3) + e) ^ (row & 7)) << 4)) =
+                    make_uint4(pack2<T>(f[8 * e] * inv, f[8 * e + 1] * inv),
+                               pack2<T>(f[8 * e + 2] * inv, f[8 * e + 3] * inv),
+                               pack2<T>(f[8 * e + 4] * inv, f[8 * e + 5] * inv),
+                               pack2<T>(f[8 * e + 6] * inv, f[8 * e + 7] * inv));
+            }
+            __syncwarp();
+          }
+        }
+        if (t == passes - 1) {  // O and (m, l) are read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(kORead));
+        }
+      }
+      if (d.slot < 0) {
+        // Lane l stores 16-byte chunk l % 8 of row 4i + l / 8: whole lines.
+#pragma unroll 1
+        for (int t = 0; t < passes; ++t) {
+          const int64_t tok = d.q0 + (int64_t)t * p.block_q + row_tok;
+          const bool row_valid = row < p.group * p.block_q && tok < d.qe;
+          const int64_t orow = tok * p.num_q_heads + (int64_t)d.h * p.group + row_head;
+          const uint8_t* qbuf = smem + kOffQ + (int)((qc + (uint32_t)t) % kQStages) * kTileBytes;
+          if (!__any_sync(0xffffffffu, row_valid)) continue;
+#pragma unroll 2
+          for (int it = 0; it < 16; ++it) {
+            const int hf = it >> 3, r8 = 4 * (it & 7) + (lane >> 3);  // row of this warp
+            const int64_t at = __shfl_sync(0xffffffffu, row_valid ? orow : -1, r8);
+            const uint4 v = *reinterpret_cast<const uint4*>(
+                qbuf + hf * kHalf + (row - lane + r8) * 128 + (((lane & 7) ^ (r8 & 7)) << 4));
+            if (at >= 0)
+              *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + at * 128 + 64 * hf + 8 * (lane & 7)) = v;
+          }
+        }
+      }
+      fence_proxy_async();  // the Q tiles may be loaded again
+      __syncwarp();
+      if (lane == 0)
+        for (int t = 0; t < passes; ++t) mbar_arrive(bar(kQEmpty + (qc + (uint32_t)t) % kQStages));
+      advance(d);
+    }
+  } else if (warp >= kKProdWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kOtherRegs));
     if (warp == kSchedWarp) {
       // ---------------------------------------------------- scheduler
@@ -521,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             issue_s(1, qs1, kslot(kvc));
             umma_commit(bar(kKEmpty + kslot(kvc)));
-            ok = wait_v(kvc, n > 1, kvc + 1);
+            ok = wait_v(kvc, n > 1, kvc + 1) && mbar_wait(bar(kORead), (i & 1) ^ 1);
             for (int j = 0; ok && j < n; ++j) {
               const uint32_t c = kvc + j;
               for (int x = 0; x < 2; ++x) {
@@ -550,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               issue_s(1, qs0, kslot(kvc + 1));
               umma_commit(bar(kKEmpty + kslot(kvc + 1)));
             }
-            ok = wait_v(kvc, n > 2, kvc + 2);
+            ok = wait_v(kvc, n > 2, kvc + 2) && mbar_wait(bar(kORead), (i & 1) ^ 1);
             for (int j = 0; ok && j < n; ++j) {
               const uint32_t c = kvc + j;
               const int x = j & 1;
@@ -706,7 +877,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t s_cols = tmem + lane_base + col_s(x);
     const uint32_t o_cols = tmem + lane_base + col_o(x);
-    const int row_tok = row / p.group, row_head = row % p.group;
+    const int row_tok = row / p.group;
     for (uint32_t i = 0;; ++i) {
       ItemDesc d;
       if (!take_item(i, d)) {
@@ -727,28 +898,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t mask0 = row_valid ? __ldg(mrow) : 0;  // in flight with the loads around it
       const int nx = stream_tiles(d, x), step = d.two ? 1 : 2, first = d.two ? 0 : x;
       const uint32_t tcx = x == 0 ? tc0 : tc1;
-      // The row's keys among 32 from position k0 (32-aligned in the tile).
-      auto seen32 = [&](int32_t k) -> uint32_t {
-        if (!row_valid) return 0u;
-        const int32_t a = min(max(lo_q - k, 0), 32), b = min(max(d.committed - k, 0), 32);
-        const uint32_t below_a = a >= 32 ? ~0u : (1u << a) - 1u, below_b = b >= 32 ? ~0u : (1u << b) - 1u;
-        uint32_t bits = below_b & ~below_a;
-        const int32_t j = k - d.committed, nodes = d.kv_hi - d.committed;  // first node of the 32
-        if (j > -32 && j < nodes) {
-          uint32_t tree;
-          if (j <= 0) {
-            tree = (uint32_t)(mask0 << (-j));
-          } else {
-            const int w = j >> 6, sh = j & 63;
-            uint64_t v = (w == 0 ? mask0 : __ldg(mrow + w)) >> sh;
-            if (sh > 32 && w + 1 < p.mask_words) v |= __ldg(mrow + w + 1) << (64 - sh);
-            tree = (uint32_t)v;
-          }
-          if (nodes - j < 32) tree &= (1u << (nodes - j)) - 1u;
-          bits |= tree;
-        }
-        return bits;
-      };
       float m_ref = -INFINITY, l = 0.f;
       int64_t blk_next = -1;
       if (lane < p.boxes && nx > 0)
@@ -773,7 +922,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // and in a small loop: one or two tiles of an item come here.
 #pragma unroll 1
             for (int ch = 0; ch < 4; ++ch) {
-              uint32_t seen = seen32(k0 + 32 * ch);
+              uint32_t seen = row_valid ? seen32(d, lo_q, mrow, mask0, k0 + 32 * ch) : 0u;
               if (!all_pages) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
@@ -870,142 +1019,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
 
-      // ---- epilogue ----
-      // The non-finite values that this row sees among the replaced ones:
-      // columns [c0, c0 + 64) of the rows that only some query rows see.
-      // This warpgroup's columns of the row: all of its own stream's O, or,
-      // when both streams hold the same rows, one half of the sum of both.
-      const uint32_t qslot = (qc + (uint32_t)qt) % kQStages;
-      const int y = x ^ 1;
-      const int ny = d.two ? 0 : stream_tiles(d, y);
-      float m_all = m_ref, l_all = l, f_x = 1.f, f_y = 0.f;
-      bool arrived = true;
-      if (!d.two) {
-        ml_sh[x][row] = make_float2(m_ref, l);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kMl + x));
-        arrived = mbar_wait(bar(kMl + y), mc & 1);
-        const float2 other = ml_sh[y][row];
-        m_all = fmaxf(m_ref, other.x);
-        const float mu = m_all == -INFINITY ? 0.f : m_all;
-        f_x = ex2(m_ref - mu);
-        f_y = ex2(other.x - mu);
-        l_all = l * f_x + other.y * f_y;
-      }
-      // A stream's last S is complete once its (m, l) are here, so its P.V
-      // barrier is in the last tile's phase or just behind it.
-      if (nx > 0) arrived = arrived && mbar_wait(bar(kPvDone + x), (tcx + nx - 1) & 1);
-      if (ny > 0) arrived = arrived && mbar_wait(bar(kPvDone + y), ((y == 0 ? tc0 : tc1) + ny - 1) & 1);
-      if (!__all_sync(0xffffffffu, arrived)) {
+      // (m, l) go to the epilogue's warpgroup, which has read the item before.
+      if (!__all_sync(0xffffffffu, mbar_wait(bar(kORead), (i & 1) ^ 1))) {
         fail();
         break;
       }
-      tc_fence_after();
-      if (warp_valid) {
-        const bool bad = bad_v_sh[i % kFlagSlots] != 0;
-        const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
-        const int64_t orow = tok * p.num_q_heads + (int64_t)d.h * p.group + row_head;
-        const int64_t part = (int64_t)blockIdx.x * 2 + d.slot;
-        const int part_row = qt * kRows + row;
-        if (d.slot >= 0 && row_valid && (d.two || x == 0))
-          p.part_ml[part * kPartRows + part_row] = make_float2(m_all, l_all);
-        const uint32_t other_cols = tmem + lane_base + col_o(y);
-        const int c_lo = d.two ? 0 : 64 * x, c_hi = d.two ? 128 : 64 * x + 64;
-        // Every S of the item is done with its Q tile, which stages the output.
-        uint8_t* qbuf = smem + kOffQ + qslot * kTileBytes;
-        // A small loop body: this code runs once per item, so most of its
-        // time is fetching it.
-#pragma unroll 1
-        for (int c0 = c_lo; c0 < c_hi; c0 += 16) {
-          uint32_t o[16], u[16];
-          if (nx > 0) tmem_ld16_raw(o_cols + c0, o);
-          if (ny > 0) tmem_ld16_raw(other_cols + c0, u);
-          tmem_wait_ld();
-          reg_fence(o);
-          reg_fence(u);
-          float f[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            f[e] = nx > 0 ? __uint_as_float(o[e]) * f_x : 0.f;
-            if (ny > 0) f[e] = fmaf(__uint_as_float(u[e]), f_y, f[e]);
-          }
-          if (bad && row_valid) {
-            // The non-finite values that this row sees among the replaced ones.
-            const int32_t seg_end = min(d.kbase + d.n * kKeys, d.kv_hi);
-#pragma unroll 1
-            for (int32_t k = max(d.kbase, d.kv_lo); k < seg_end; ++k) {
-              if (k >= d.lo_all && k < d.committed) {
-                k = d.committed - 1;
-                continue;
-              }
-              if (!(seen32(k) & 1u)) continue;
-              const int64_t blk = page_of(p, trow, k);
-              if (blk < 0) continue;
-              const uint32_t* v = reinterpret_cast<const uint32_t*>(
-                  reinterpret_cast<const T*>(p.cache) +
-                  ((p.num_slots + blk * p.block_size + k % p.block_size) * p.num_kv_heads + d.h) * 128 + c0);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const uint32_t w = __ldg(v + e), b = nonfinite2<T>(w);
-                if (b & 0x8000u) f[2 * e] += to_float(reinterpret_cast<const T*>(&w)[0]);
-                if (b & 0x80000000u) f[2 * e + 1] += to_float(reinterpret_cast<const T*>(&w)[1]);
-              }
-            }
-          }
-          if (d.slot >= 0) {
-            if (row_valid) {
-              float4* dst = p.part_o + (part * 32 + c0 / 4) * kPartRows + part_row;
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                dst[e * kPartRows] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
-            }
-          } else {
-            uint8_t* cell = qbuf + (c0 >> 6) * kHalf + row * 128;
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              *reinterpret_cast<uint4*>(cell + (((((c0 & 63) >> 3) + e) ^ (row & 7)) << 4)) =
-                  make_uint4(pack2<T>(f[8 * e] * inv, f[8 * e + 1] * inv),
-                             pack2<T>(f[8 * e + 2] * inv, f[8 * e + 3] * inv),
-                             pack2<T>(f[8 * e + 4] * inv, f[8 * e + 5] * inv),
-                             pack2<T>(f[8 * e + 6] * inv, f[8 * e + 7] * inv));
-          }
-          __syncwarp();
-        }
-        if (d.slot < 0) {
-          // Lane l stores 16-byte chunk l % 8 of row 4i + l / 8: whole lines.
-#pragma unroll 1
-          for (int hf = c_lo >> 6; hf < c_hi >> 6; ++hf)
-#pragma unroll 4
-            for (int it = 0; it < 8; ++it) {
-              const int r8 = 4 * it + (lane >> 3);  // row of this warp
-              const int64_t at = __shfl_sync(0xffffffffu, row_valid ? orow : -1, r8);
-              const uint4 v = *reinterpret_cast<const uint4*>(
-                  qbuf + hf * kHalf + (row - lane + r8) * 128 + (((lane & 7) ^ (r8 & 7)) << 4));
-              if (at >= 0)
-                *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + at * 128 + 64 * hf + 8 * (lane & 7)) = v;
-            }
-        }
-      }
-      // The staging buffer was the item's Q tile: a tile of its own is given
-      // back by one warpgroup's 4 warps, a shared one by all 8.
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(bar(kQEmpty + qslot));
-        if (d.two) mbar_arrive(bar(kQEmpty + qslot));
-      }
+      ml_sh[x][row] = make_float2(m_ref, l);
       tc_fence_before();
-      if (!d.two) {
-        // The next item's first P.V overwrites O: not before the other
-        // warpgroup has read this stream's columns.
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(kORead + y));
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(kORead + x), mc & 1))) {
-          fail();
-          break;
-        }
-        tc_fence_after();
-      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kMl + x));
       advance(d);
     }
   }
