@@ -57,6 +57,9 @@ constexpr int kRows = 128;                 // MMA M: rows of one query tile
 constexpr int kKeys = 128;                 // keys per KV tile
 constexpr int kHalf = kRows * 128;         // [128 rows][64 elements] swizzled: 16 KiB
 constexpr int kTileBytes = 2 * kHalf;      // [128][128] 16-bit
+// A K/V tile: 8-row groups, each the swizzle atom of its columns 0-63 and then
+// that of 64-127, so a page is one TMA box.
+constexpr int kAtom = 1024, kGroupBytes = 2 * kAtom;
 constexpr int kKStages = 2, kVStages = 3, kQStages = 2;
 constexpr int kOffQ = 0;
 constexpr int kOffK = kQStages * kTileBytes;
@@ -629,15 +632,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t idesc_qk = f16_idesc(kBf16, false, kRows, kKeys);
         const uint32_t idesc_pv = f16_idesc(kBf16, true, kRows, 128);
         const uint64_t dq0 = sw128_desc(sb + kOffQ, 16, 1024);
-        const uint64_t dk0 = sw128_desc(sb + kOffK, 16, 1024);
-        const uint64_t dv0 = sw128_desc(sb + kOffV, kHalf, 1024);
+        const uint64_t dk0 = sw128_desc(sb + kOffK, 16, kGroupBytes);
+        const uint64_t dv0 = sw128_desc(sb + kOffV, kAtom, kGroupBytes);
         auto issue_s = [&](int x, uint32_t qs, uint32_t stage) {
           const uint64_t dq = dq0 + (uint64_t)((qs * kTileBytes) >> 4);
           const uint64_t dk = dk0 + (uint64_t)((stage * kTileBytes) >> 4);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const uint32_t step = (uint32_t)((k >> 2) * (kHalf >> 4) + 2 * (k & 3));
-            umma_f16(tmem + col_s(x), dq + step, dk + step, idesc_qk, k > 0);
+            const uint32_t q_step = (uint32_t)((k >> 2) * (kHalf >> 4) + 2 * (k & 3));
+            const uint32_t k_step = (uint32_t)((k >> 2) * (kAtom >> 4) + 2 * (k & 3));
+            umma_f16(tmem + col_s(x), dq + q_step, dk + k_step, idesc_qk, k > 0);
           }
           umma_commit(bar(kSFull + x));
         };
@@ -646,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint32_t pcol = 32 * (k >> 1) + 8 * (k & 1);
-            umma_f16_ts(tmem + col_o(x), tmem + col_s(x) + pcol, dv + (uint64_t)(k * (2048 >> 4)),
+            umma_f16_ts(tmem + col_o(x), tmem + col_s(x) + pcol, dv + (uint64_t)(k * (2 * kGroupBytes >> 4)),
                         idesc_pv, acc || k > 0);
           }
           umma_commit(bar(kPvDone + x));
@@ -771,18 +775,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!__all_sync(0xffffffffu, mbar_wait(bar(kVFull + s), vphase(todo.c)))) return false;
         // Lane l takes 16-byte chunk l % 8 of row 4i + l / 8, both halves.
         uint8_t* vt = smem + kOffV + s * kTileBytes + (lane & 7) * 16;
+        auto cell_of = [&](int row) {
+          return reinterpret_cast<uint4*>(vt + (row >> 3) * kGroupBytes + (row & 7) * 128);
+        };
         auto zero_rows = [&](int r0, int r1) {
           for (int row = r0 + (lane >> 3); row < r1; row += 4) {
-            uint4* cell = reinterpret_cast<uint4*>(vt + row * 128);
+            uint4* cell = cell_of(row);
             cell[0] = make_uint4(0, 0, 0, 0);
-            cell[kHalf / 16] = make_uint4(0, 0, 0, 0);
+            cell[kAtom / 16] = make_uint4(0, 0, 0, 0);
           }
         };
         auto clean_rows = [&](int r0, int r1) {
 #pragma unroll 4
           for (int row = r0 + (lane >> 3); row < r1; row += 4) {
-            uint4* cell = reinterpret_cast<uint4*>(vt + row * 128);
-            uint4 v[2] = {cell[0], cell[kHalf / 16]};
+            uint4* cell = cell_of(row);
+            uint4 v[2] = {cell[0], cell[kAtom / 16]};
             uint32_t* w = reinterpret_cast<uint32_t*>(v);
             uint32_t any = 0;
 #pragma unroll
@@ -792,7 +799,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int q = 0; q < 8; ++q) w[q] &= ~((nonfinite2<T>(w[q]) >> 15) * 0xffffu);
               cell[0] = v[0];
-              cell[kHalf / 16] = v[1];
+              cell[kAtom / 16] = v[1];
             }
           }
         };
@@ -818,7 +825,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         if (d.r < 0 || *abort_flag != 0) break;
+        // Block ids of 32 boxes at a time, a group ahead: under load a lookup
+        // takes longer than a tile.  Boxes count from the segment's first key;
+        // group g holds the 32 that end 32 g before its last.
         const int64_t* trow = p.table + (int64_t)d.r * p.table_stride;
+        const int boxes_all = d.n * p.boxes;
+        auto lookup = [&](int g) -> int32_t {
+          const int b = boxes_all - 32 * (g + 1) + lane;
+          return b >= 0 ? (int32_t)page_of(p, trow, (int64_t)d.kbase + (int64_t)b * p.box_rows) : -1;
+        };
+        int32_t ids = -1, ids_next = lookup(0);
         for (int j = 0; j < d.n; ++j) {
           const uint32_t c = kvc + j;
           const uint32_t s = is_k ? kslot(c) : vslot(c);
@@ -827,9 +843,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t empty_phase = (is_k ? kphase(c) : vphase(c)) ^ 1;
           const int32_t k0 = d.kbase + (d.n - 1 - j) * kKeys;  // the drafted keys first
           const int64_t pos = (int64_t)k0 + p.box_rows * lane;
-          int64_t blk = -1;
-          if (lane < p.boxes) blk = page_of(p, trow, pos);
-          if (pending && !__all_sync(0xffffffffu, mbar_try_wait(empty, empty_phase))) ok = fix_v();
+          const int in_group = (j * p.boxes) & 31;
+          if (in_group == 0) {
+            ids = ids_next;
+            ids_next = lookup(j * p.boxes / 32 + 1);
+          }
+          const int64_t blk = __shfl_sync(0xffffffffu, ids, (32 - in_group - p.boxes + lane) & 31);
+          if (pending && !__all_sync(0xffffffffu, mbar_test(empty, empty_phase))) ok = fix_v();
           ok = ok && __all_sync(0xffffffffu, mbar_wait(empty, empty_phase));
           if (!ok) break;
           const uint32_t boxes_ok = __ballot_sync(0xffffffffu, lane < p.boxes && blk >= 0);
@@ -846,9 +866,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int64_t page = blk >= 0 ? blk : 0;
             const int64_t off = p.bs_shift >= 0 ? (pos & (p.block_size - 1)) : pos % p.block_size;
             const int32_t y = (int32_t)(page * p.block_size + off) + (is_k ? 0 : (int32_t)p.num_slots);
-            const uint32_t dst = sb + (is_k ? kOffK : kOffV) + s * kTileBytes + lane * p.box_rows * 128;
-            tma_load_2d(dst, &kvmap, d.h * 128, y, full);
-            tma_load_2d(dst + kHalf, &kvmap, d.h * 128 + 64, y, full);
+            const uint32_t dst = sb + (is_k ? kOffK : kOffV) + s * kTileBytes + lane * p.box_rows * 256;
+            tma_load_4d(dst, &kvmap, 0, 0, 2 * d.h, y >> 3, full);
             if (is_k && blk < 0 && pos < d.kv_hi && pos + p.box_rows > d.kv_lo && p.status != nullptr)
               atomicOr(p.status, MVB_STATUS_BLOCK_OUT_OF_RANGE);
           }
@@ -1250,11 +1269,14 @@ int launch_tree_attention(const TreeProblem& a) {
       return MVB_ERR_UNSUPPORTED_SHAPE;
   }
   {
-    const cuuint64_t dims[2] = {(cuuint64_t)a.num_kv_heads * 128, (cuuint64_t)(2 * num_slots)};
-    const cuuint64_t strides[1] = {(cuuint64_t)a.num_kv_heads * 128 * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    if (encode(&kvmap, dt, 2, const_cast<void*>(a.cache), dims, strides, box, estr,
+    // [slot / 8][64-column segment][slot % 8][64 elements]: a box of a page is
+    // 8-row groups of two segments, as the tiles lie in shared memory.
+    const cuuint64_t row = (cuuint64_t)a.num_kv_heads * 256;
+    const cuuint64_t dims[4] = {64, 8, (cuuint64_t)a.num_kv_heads * 2, (cuuint64_t)(2 * num_slots / 8)};
+    const cuuint64_t strides[3] = {row, 128, 8 * row};
+    const cuuint32_t box[4] = {64, 8, 2, (cuuint32_t)box_rows / 8};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    if (encode(&kvmap, dt, 4, const_cast<void*>(a.cache), dims, strides, box, estr,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
       return MVB_ERR_UNSUPPORTED_SHAPE;
