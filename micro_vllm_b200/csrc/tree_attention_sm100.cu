@@ -73,7 +73,7 @@ constexpr int kItemReaders = 15;
 constexpr int kFlagSlots = 8;  // items whose V flag may still be read (more than kItemSlots)
 // Register split (setmaxnreg) of the launch's 512 x 128 between the two
 // softmax warpgroups, the epilogue's and the one of the other roles.
-constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kEpiRegs = 96, kOtherRegs = 80;
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kEpiRegs = 80, kOtherRegs = 96;
 static_assert(2 * 128 * kSoftmaxRegs + 128 * kEpiRegs + 128 * kOtherRegs <= kThreads * kLaunchRegs,
               "register split must fit the launch's registers");
 constexpr uint32_t kTmemCols = 512;
@@ -645,13 +645,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           umma_commit(bar(kSFull + x));
         };
-        auto issue_pv = [&](int x, uint32_t stage, bool acc) {
+        // O_x += P_x . V of tile j.  16-key steps with no key of [kv_lo, kv_hi)
+        // are left out: their V rows may hold anything.
+        auto issue_pv = [&](const ItemDesc& d, int j, int x, uint32_t stage, bool acc) {
           const uint64_t dv = dv0 + (uint64_t)((stage * kTileBytes) >> 4);
+          const uint32_t d_tmem = tmem + col_o(x), p_tmem = tmem + col_s(x);
+          const int32_t k0 = d.kbase + (d.n - 1 - j) * kKeys;
+          if (k0 >= d.kv_lo && k0 + kKeys <= d.kv_hi) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t pcol = 32 * (k >> 1) + 8 * (k & 1);
-            umma_f16_ts(tmem + col_o(x), tmem + col_s(x) + pcol, dv + (uint64_t)(k * (2 * kGroupBytes >> 4)),
-                        idesc_pv, acc || k > 0);
+            for (int k = 0; k < 8; ++k)
+              umma_f16_ts(d_tmem, p_tmem + 32 * (k >> 1) + 8 * (k & 1),
+                          dv + (uint64_t)(k * (2 * kGroupBytes >> 4)), idesc_pv, acc || k > 0);
+          } else {
+            const int lo = max(d.kv_lo - k0, 0) >> 4, hi = (min(d.kv_hi - k0, kKeys) + 15) >> 4;
+#pragma unroll 1
+            for (int k = lo; k < hi; ++k)
+              umma_f16_ts(d_tmem, p_tmem + 32 * (k >> 1) + 8 * (k & 1),
+                          dv + (uint64_t)(k * (2 * kGroupBytes >> 4)), idesc_pv, acc || k > lo);
           }
           umma_commit(bar(kPvDone + x));
         };
@@ -703,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = mbar_wait(bar(kPFull + x), ((x == 0 ? tc0 : tc1) + j) & 1);
                 if (!ok) break;
                 tc_fence_after();
-                issue_pv(x, vslot(c), j > 0);
+                issue_pv(d, j, x, vslot(c), j > 0);
                 if (x == 1) umma_commit(bar(kVEmpty + vslot(c)));
                 if (j + 1 < n) {
                   ok = x == 1 || wait_k(c + 1);
@@ -732,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               ok = mbar_wait(bar(kPFull + x), ((x == 0 ? tc0 : tc1) + (j >> 1)) & 1);
               if (!ok) break;
               tc_fence_after();
-              issue_pv(x, vslot(c), j > 1);
+              issue_pv(d, j, x, vslot(c), j > 1);
               umma_commit(bar(kVEmpty + vslot(c)));
               if (j + 2 < n) {
                 ok = wait_k(c + 2);
@@ -753,10 +763,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---------------------------------------------------- producers
       const bool is_k = warp == kKProdWarp;
       // A V tile with rows that some query row does not see is fixed up once
-      // it lands: rows behind the last key, before the first and on missing
-      // pages are zeroed, the non-finite elements of rows that only some
-      // query rows see too.  The fix waits in `todo` until the next load is
-      // on its way.
+      // it lands: rows behind the last key, before the first (within their
+      // 16-key steps) and on missing pages are zeroed, the non-finite elements
+      // of rows that only some query rows see too.  The fix waits in `todo`
+      // while further loads can be sent.
       struct Todo {
         uint32_t c, item, boxes_ok;
         int32_t k0, kv_lo, kv_hi, lo_all, committed;
@@ -779,6 +789,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           return reinterpret_cast<uint4*>(vt + (row >> 3) * kGroupBytes + (row & 7) * 128);
         };
         auto zero_rows = [&](int r0, int r1) {
+#pragma unroll 1
           for (int row = r0 + (lane >> 3); row < r1; row += 4) {
             uint4* cell = cell_of(row);
             cell[0] = make_uint4(0, 0, 0, 0);
@@ -786,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         };
         auto clean_rows = [&](int r0, int r1) {
-#pragma unroll 4
+#pragma unroll 1
           for (int row = r0 + (lane >> 3); row < r1; row += 4) {
             uint4* cell = cell_of(row);
             uint4 v[2] = {cell[0], cell[kAtom / 16]};
@@ -804,10 +815,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         };
         const int lo = max(todo.kv_lo - todo.k0, 0), hi = min(todo.kv_hi - todo.k0, kKeys);
-        zero_rows(0, lo);
-        zero_rows(hi, kKeys);
-        for (int b = 0; b < p.boxes; ++b)
-          if (!((todo.boxes_ok >> b) & 1u)) zero_rows(b * p.box_rows, (b + 1) * p.box_rows);
+        zero_rows(lo & ~15, lo);  // 16-key steps beyond are not multiplied
+        zero_rows(hi, (hi + 15) & ~15);
+        if (todo.boxes_ok != (1u << p.boxes) - 1u)
+          for (int b = 0; b < p.boxes; ++b)
+            if (!((todo.boxes_ok >> b) & 1u)) zero_rows(b * p.box_rows, (b + 1) * p.box_rows);
         __syncwarp();
         clean_rows(lo, min(todo.lo_all - todo.k0, hi));
         clean_rows(max(todo.committed - todo.k0, lo), hi);
@@ -872,13 +884,20 @@ __global__ void __launch_bounds__(kThreads, 1)
               atomicOr(p.status, MVB_STATUS_BLOCK_OUT_OF_RANGE);
           }
           if (is_k) continue;
-          if (pending) ok = fix_v();
+          // A pending fix waits as long as loads can go out, unless its tile is here.
+          if (pending &&
+              (dirty || __all_sync(0xffffffffu, mbar_test(bar(kVFull + vslot(todo.c)), vphase(todo.c)))))
+            ok = fix_v();
           if (!ok) break;
           if (dirty) {
             todo = {c, i, boxes_ok, k0, d.kv_lo, d.kv_hi, d.lo_all, d.committed, last};
             pending = true;
           } else {
-            if (last) leave_flag(i);
+            if (last) {
+              if (pending) ok = fix_v();
+              leave_flag(i);
+              if (!ok) break;
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(kVReady + s));  // nothing to fix
           }
