@@ -53,6 +53,16 @@ namespace {
 
 using namespace sm100;
 
+// sm100::mbar_wait with its loop kept a loop: unrolled at every call it made
+// this kernel 160 KB of code, and each role's first steps of an item wait for
+// instructions.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < (1 << 22); ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return false;
+}
+
 constexpr int kRows = 128;                 // MMA M: rows of one query tile
 constexpr int kKeys = 128;                 // keys per KV tile
 constexpr int kHalf = kRows * 128;         // [128 rows][64 elements] swizzled: 16 KiB
@@ -145,11 +155,19 @@ struct TreeParams {
   int32_t* status;
 };
 
-__device__ __forceinline__ int64_t page_of(const TreeParams& p, const int64_t* trow, int64_t pos) {
-  const int64_t lb = p.bs_shift >= 0 ? (pos >> p.bs_shift) : pos / p.block_size;
-  if (pos < 0 || lb >= p.table_width) return -1;
+// Positions fit 32 bits (a context is at most 2^30 long).
+__device__ __forceinline__ int32_t block_of(const TreeParams& p, int32_t pos) {
+  return p.bs_shift >= 0 ? pos >> p.bs_shift : pos / p.block_size;
+}
+__device__ __forceinline__ int32_t page_of(const TreeParams& p, const int64_t* trow, int32_t pos) {
+  const int32_t lb = block_of(p, pos);
+  if (lb >= p.table_width) return -1;
   const int64_t blk = __ldg(trow + lb);
-  return (blk >= 0 && blk < p.num_blocks) ? blk : -1;
+  return (blk >= 0 && blk < p.num_blocks) ? (int32_t)blk : -1;
+}
+// Slot of position pos on page blk (slots of both planes fit 32 bits).
+__device__ __forceinline__ int32_t slot_of(const TreeParams& p, int32_t blk, int32_t pos) {
+  return blk * p.block_size + pos - block_of(p, pos) * p.block_size;
 }
 
 __device__ __forceinline__ void touch(const int64_t* at) {
@@ -232,6 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int64_t per = (p.num_requests + kThreads - 1) / kThreads;
   const int64_t r_lo = min(tid * per, p.num_requests), r_hi = min(r_lo + per, p.num_requests);
   int64_t mine = 0;
+#pragma unroll 1
   for (int64_t r = r_lo; r < r_hi; ++r) {
     TreeExtent e;
     if (tree_extent(p, r, e)) mine += cost_of(p, e).head * p.num_kv_heads;
@@ -257,6 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (my_lo >= total) return;
   if (before <= my_lo && my_lo < before + mine) {
     int64_t r = r_lo, at = before;
+#pragma unroll 1
     for (;; ++r) {
       TreeExtent e;
       const int64_t c = tree_extent(p, r, e) ? cost_of(p, e).head * p.num_kv_heads : 0;
@@ -279,6 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     prefetch_tensormap(&qmap);
     prefetch_tensormap(&kvmap);
+#pragma unroll 1
     for (int i = 0; i < kNumBars; ++i) {
       const bool four = (i >= kPFull && i < kPFull + 2) || (i >= kMl && i <= kORead) ||
                         (i >= kQEmpty && i < kQEmpty + kQStages);
@@ -298,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   auto take_item = [&](uint32_t i, ItemDesc& d) -> bool {
     const uint32_t slot = i % kItemSlots;
-    if (!__all_sync(0xffffffffu, mbar_wait(bar(kItemFull + slot), (i / kItemSlots) & 1)))
+    if (!__all_sync(0xffffffffu, bar_wait(bar(kItemFull + slot), (i / kItemSlots) & 1)))
       return false;
     d = items[slot];
     __syncwarp();
@@ -367,9 +388,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int n0 = stream_tiles(d, 0), n1 = stream_tiles(d, 1);
       // A stream's last S is complete once its (m, l) are here, so its P.V
       // barrier is in the last tile's phase or just behind it.
-      bool arrived = mbar_wait(bar(kMl), i & 1) && mbar_wait(bar(kMl + 1), i & 1) &&
-                     mbar_wait(bar(kPvDone), (tc0 + n0 - 1) & 1);
-      if (n1 > 0) arrived = arrived && mbar_wait(bar(kPvDone + 1), (tc1 + n1 - 1) & 1);
+      bool arrived = bar_wait(bar(kMl), i & 1) && bar_wait(bar(kMl + 1), i & 1) &&
+                     bar_wait(bar(kPvDone), (tc0 + n0 - 1) & 1);
+      if (n1 > 0) arrived = arrived && bar_wait(bar(kPvDone + 1), (tc1 + n1 - 1) & 1);
       if (!__all_sync(0xffffffffu, arrived)) {
         fail();
         break;
@@ -428,11 +449,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                   continue;
                 }
                 if (!(seen32(d, lo_q, mrow, __ldg(mrow), k) & 1u)) continue;
-                const int64_t blk = page_of(p, trow, k);
+                const int32_t blk = page_of(p, trow, k);
                 if (blk < 0) continue;
                 const uint32_t* v = reinterpret_cast<const uint32_t*>(
                     reinterpret_cast<const T*>(p.cache) +
-                    ((p.num_slots + blk * p.block_size + k % p.block_size) * p.num_kv_heads + d.h) * 128 + c0);
+                    ((p.num_slots + slot_of(p, blk, k)) * p.num_kv_heads + d.h) * 128 + c0);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                   const uint32_t w = __ldg(v + e), b = nonfinite2<T>(w);
@@ -513,6 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // The next item with tiles in this share.
         ItemDesc d;
         d.r = -1;
+#pragma unroll 1
         while (*abort_flag == 0) {
           if (fresh) {
             if (cost0 >= my_hi || r >= p.num_requests) break;
@@ -578,6 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // Committed keys that every row of the item sees start here.
           int32_t hi_start = d.kv_lo;
           const int64_t tend = min(d.q0 + 2 * (int64_t)p.block_q, d.qe);
+#pragma unroll 1
           for (int64_t t = d.q0 + lane; t < tend; t += 32)
             hi_start = max(hi_start, (int32_t)min(max(__ldg(p.qstart + t), (int64_t)0), (int64_t)d.committed));
 #pragma unroll
@@ -587,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const uint32_t slot = i % kItemSlots;
         if (!__all_sync(0xffffffffu,
-                        mbar_wait(bar(kItemEmpty + slot), ((i / kItemSlots) & 1) ^ 1))) {
+                        bar_wait(bar(kItemEmpty + slot), ((i / kItemSlots) & 1) ^ 1))) {
           fail();
           break;
         }
@@ -599,9 +622,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (d.r < 0) break;
         if (lane == 0) {
           const int qn = d.two ? 2 : 1;
+#pragma unroll 1
           for (int t = 0; ok && t < qn; ++t) {
             const uint32_t c = qc + (uint32_t)t, qs = c % kQStages;
-            if (!mbar_wait(bar(kQEmpty + qs), ((c / kQStages) & 1) ^ 1)) {
+            if (!bar_wait(bar(kQEmpty + qs), ((c / kQStages) & 1) ^ 1)) {
               ok = false;
               break;
             }
@@ -616,11 +640,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) fail();
         // Under load a global load takes microseconds: bring what the other
         // warps read first of this item into the SM's cache.
+#pragma unroll 1
         for (int64_t t = d.q0 + lane; t < min(d.q0 + 2 * (int64_t)p.block_q, d.qe); t += 32)
           touch(p.mask + t * p.mask_words);
         {
-          const int64_t pos = (int64_t)d.kbase + max(d.n - 2, 0) * kKeys + 8 * lane;
-          const int64_t lb = p.bs_shift >= 0 ? (pos >> p.bs_shift) : pos / p.block_size;
+          const int32_t lb = block_of(p, d.kbase + max(d.n - 2, 0) * kKeys + 8 * lane);
           if (lb < p.table_width) touch(p.table + (int64_t)d.r * p.table_stride + lb);
         }
         advance(d);
@@ -675,18 +699,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t kp = more ? kphase(ck) : vphase(c);
           bool r0, r1;
           mbar_test3(vf, vphase(c), vr, vphase(c), kf, kp, r0, r1, k_ready);
-          return (r0 || mbar_wait(vf, vphase(c))) && (r1 || mbar_wait(vr, vphase(c)));
+          return (r0 || bar_wait(vf, vphase(c))) && (r1 || bar_wait(vr, vphase(c)));
         };
         auto wait_k = [&](uint32_t ck) -> bool {
           if (k_ready) return true;
-          const bool there = mbar_wait(bar(kKFull + kslot(ck)), kphase(ck));
+          const bool there = bar_wait(bar(kKFull + kslot(ck)), kphase(ck));
           tc_fence_after();
           return there;
         };
         bool ok = true;
         for (uint32_t i = 0; ok; ++i) {
           const uint32_t slot = i % kItemSlots;
-          if (!mbar_wait(bar(kItemFull + slot), (i / kItemSlots) & 1)) {
+          if (!bar_wait(bar(kItemFull + slot), (i / kItemSlots) & 1)) {
             ok = false;
             break;
           }
@@ -695,22 +719,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (d.r < 0 || *abort_flag != 0) break;
           const int n = d.n;
           const uint32_t qs0 = qc % kQStages, qs1 = (qc + 1) % kQStages;
-          ok = mbar_wait(bar(kQFull + qs0), (qc / kQStages) & 1) &&
-               mbar_wait(bar(kKFull + kslot(kvc)), kphase(kvc));
+          ok = bar_wait(bar(kQFull + qs0), (qc / kQStages) & 1) &&
+               bar_wait(bar(kKFull + kslot(kvc)), kphase(kvc));
           if (!ok) break;
           tc_fence_after();
           issue_s(0, qs0, kslot(kvc));
-          if (d.two) {
-            ok = mbar_wait(bar(kQFull + qs1), ((qc + 1) / kQStages) & 1);
+          if (!d.two) umma_commit(bar(kKEmpty + kslot(kvc)));
+          if (d.two || n > 1) {  // stream 1: the other query tile, or the next KV tile
+            const uint32_t c1 = kvc + (d.two ? 0 : 1);
+            ok = d.two ? bar_wait(bar(kQFull + qs1), ((qc + 1) / kQStages) & 1)
+                       : bar_wait(bar(kKFull + kslot(c1)), kphase(c1));
             if (!ok) break;
             tc_fence_after();
-            issue_s(1, qs1, kslot(kvc));
-            umma_commit(bar(kKEmpty + kslot(kvc)));
-            ok = wait_v(kvc, n > 1, kvc + 1) && mbar_wait(bar(kORead), (i & 1) ^ 1);
+            issue_s(1, d.two ? qs1 : qs0, kslot(c1));
+            umma_commit(bar(kKEmpty + kslot(c1)));
+          }
+          if (d.two) {
+            ok = wait_v(kvc, n > 1, kvc + 1) && bar_wait(bar(kORead), (i & 1) ^ 1);
+#pragma unroll 1
             for (int j = 0; ok && j < n; ++j) {
               const uint32_t c = kvc + j;
+#pragma unroll 1
               for (int x = 0; x < 2; ++x) {
-                ok = mbar_wait(bar(kPFull + x), ((x == 0 ? tc0 : tc1) + j) & 1);
+                ok = bar_wait(bar(kPFull + x), ((x == 0 ? tc0 : tc1) + j) & 1);
                 if (!ok) break;
                 tc_fence_after();
                 issue_pv(d, j, x, vslot(c), j > 0);
@@ -727,19 +758,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           } else {
-            umma_commit(bar(kKEmpty + kslot(kvc)));
-            if (n > 1) {
-              ok = mbar_wait(bar(kKFull + kslot(kvc + 1)), kphase(kvc + 1));
-              if (!ok) break;
-              tc_fence_after();
-              issue_s(1, qs0, kslot(kvc + 1));
-              umma_commit(bar(kKEmpty + kslot(kvc + 1)));
-            }
-            ok = wait_v(kvc, n > 2, kvc + 2) && mbar_wait(bar(kORead), (i & 1) ^ 1);
+            ok = wait_v(kvc, n > 2, kvc + 2) && bar_wait(bar(kORead), (i & 1) ^ 1);
+#pragma unroll 1
             for (int j = 0; ok && j < n; ++j) {
               const uint32_t c = kvc + j;
               const int x = j & 1;
-              ok = mbar_wait(bar(kPFull + x), ((x == 0 ? tc0 : tc1) + (j >> 1)) & 1);
+              ok = bar_wait(bar(kPFull + x), ((x == 0 ? tc0 : tc1) + (j >> 1)) & 1);
               if (!ok) break;
               tc_fence_after();
               issue_pv(d, j, x, vslot(c), j > 1);
@@ -782,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto fix_v = [&]() -> bool {
         pending = false;
         const uint32_t s = vslot(todo.c);
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(kVFull + s), vphase(todo.c)))) return false;
+        if (!__all_sync(0xffffffffu, bar_wait(bar(kVFull + s), vphase(todo.c)))) return false;
         // Lane l takes 16-byte chunk l % 8 of row 4i + l / 8, both halves.
         uint8_t* vt = smem + kOffV + s * kTileBytes + (lane & 7) * 16;
         auto cell_of = [&](int row) {
@@ -818,6 +842,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         zero_rows(lo & ~15, lo);  // 16-key steps beyond are not multiplied
         zero_rows(hi, (hi + 15) & ~15);
         if (todo.boxes_ok != (1u << p.boxes) - 1u)
+#pragma unroll 1
           for (int b = 0; b < p.boxes; ++b)
             if (!((todo.boxes_ok >> b) & 1u)) zero_rows(b * p.box_rows, (b + 1) * p.box_rows);
         __syncwarp();
@@ -836,75 +861,83 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = false;
           break;
         }
-        if (d.r < 0 || *abort_flag != 0) break;
+        const bool end = d.r < 0 || *abort_flag != 0;
+        if (end && !pending) break;
         // Block ids of 32 boxes at a time, a group ahead: under load a lookup
         // takes longer than a tile.  Boxes count from the segment's first key;
         // group g holds the 32 that end 32 g before its last.
-        const int64_t* trow = p.table + (int64_t)d.r * p.table_stride;
-        const int boxes_all = d.n * p.boxes;
+        const int n = end ? 1 : d.n;  // at the end, a fix may be left
+        const int64_t* trow = p.table + (int64_t)max(d.r, 0) * p.table_stride;
         auto lookup = [&](int g) -> int32_t {
-          const int b = boxes_all - 32 * (g + 1) + lane;
-          return b >= 0 ? (int32_t)page_of(p, trow, (int64_t)d.kbase + (int64_t)b * p.box_rows) : -1;
+          const int b = n * p.boxes - 32 * (g + 1) + lane;
+          return !end && b >= 0 ? page_of(p, trow, d.kbase + b * p.box_rows) : -1;
         };
         int32_t ids = -1, ids_next = lookup(0);
-        for (int j = 0; j < d.n; ++j) {
+#pragma unroll 1
+        for (int j = 0; ok && j < n; ++j) {
           const uint32_t c = kvc + j;
           const uint32_t s = is_k ? kslot(c) : vslot(c);
           const uint32_t full = bar((is_k ? kKFull : kVFull) + s);
           const uint32_t empty = bar((is_k ? kKEmpty : kVEmpty) + s);
           const uint32_t empty_phase = (is_k ? kphase(c) : vphase(c)) ^ 1;
-          const int32_t k0 = d.kbase + (d.n - 1 - j) * kKeys;  // the drafted keys first
-          const int64_t pos = (int64_t)k0 + p.box_rows * lane;
+          const int32_t k0 = d.kbase + (n - 1 - j) * kKeys;  // the drafted keys first
+          const int32_t pos = k0 + p.box_rows * lane;
           const int in_group = (j * p.boxes) & 31;
           if (in_group == 0) {
             ids = ids_next;
             ids_next = lookup(j * p.boxes / 32 + 1);
           }
-          const int64_t blk = __shfl_sync(0xffffffffu, ids, (32 - in_group - p.boxes + lane) & 31);
-          if (pending && !__all_sync(0xffffffffu, mbar_test(empty, empty_phase))) ok = fix_v();
-          ok = ok && __all_sync(0xffffffffu, mbar_wait(empty, empty_phase));
-          if (!ok) break;
+          const int32_t blk = __shfl_sync(0xffffffffu, ids, (32 - in_group - p.boxes + lane) & 31);
           const uint32_t boxes_ok = __ballot_sync(0xffffffffu, lane < p.boxes && blk >= 0);
-          const bool last = j == d.n - 1;
+          const bool last = j == n - 1;
           const bool dirty = k0 < d.lo_all || k0 + kKeys > d.committed ||
                              boxes_ok != (1u << p.boxes) - 1u;
-          if (lane == 0) {
-            last_issued[is_k ? 0 : 1] = (int32_t)c;
-            mbar_expect_tx(full, kTileBytes);
+          // A pending fix is done before the load when that has to wait, else
+          // behind it: before the next fix, before the item's flag is left, or
+          // when its tile is here.
+#pragma unroll 1
+          for (int step = 0; ok && step < 2; ++step) {
+            bool fix = pending;
+            if (step == 0) {
+              fix = fix && (end || !__all_sync(0xffffffffu, mbar_test(empty, empty_phase)));
+            } else {
+              if (!__all_sync(0xffffffffu, bar_wait(empty, empty_phase))) {
+                ok = false;
+                break;
+              }
+              if (lane == 0) {
+                last_issued[is_k ? 0 : 1] = (int32_t)c;
+                mbar_expect_tx(full, kTileBytes);
+              }
+              __syncwarp();
+              if (lane < p.boxes) {
+                // Missing pages load page 0; the softmax masks their keys.
+                const int32_t y = slot_of(p, max(blk, 0), pos) + (is_k ? 0 : (int32_t)p.num_slots);
+                const uint32_t dst =
+                    sb + (is_k ? kOffK : kOffV) + s * kTileBytes + lane * p.box_rows * 256;
+                tma_load_4d(dst, &kvmap, 0, 0, 2 * d.h, y >> 3, full);
+                if (is_k && blk < 0 && pos < d.kv_hi && pos + p.box_rows > d.kv_lo && p.status != nullptr)
+                  atomicOr(p.status, MVB_STATUS_BLOCK_OUT_OF_RANGE);
+              }
+              fix = fix && (dirty || last ||
+                            __all_sync(0xffffffffu, mbar_test(bar(kVFull + vslot(todo.c)), vphase(todo.c))));
+            }
+            if (fix) ok = fix_v();
+            if (end) break;
           }
-          __syncwarp();
-          if (lane < p.boxes) {
-            // Missing pages load page 0; the softmax masks their keys.
-            const int64_t page = blk >= 0 ? blk : 0;
-            const int64_t off = p.bs_shift >= 0 ? (pos & (p.block_size - 1)) : pos % p.block_size;
-            const int32_t y = (int32_t)(page * p.block_size + off) + (is_k ? 0 : (int32_t)p.num_slots);
-            const uint32_t dst = sb + (is_k ? kOffK : kOffV) + s * kTileBytes + lane * p.box_rows * 256;
-            tma_load_4d(dst, &kvmap, 0, 0, 2 * d.h, y >> 3, full);
-            if (is_k && blk < 0 && pos < d.kv_hi && pos + p.box_rows > d.kv_lo && p.status != nullptr)
-              atomicOr(p.status, MVB_STATUS_BLOCK_OUT_OF_RANGE);
-          }
-          if (is_k) continue;
-          // A pending fix waits as long as loads can go out, unless its tile is here.
-          if (pending &&
-              (dirty || __all_sync(0xffffffffu, mbar_test(bar(kVFull + vslot(todo.c)), vphase(todo.c)))))
-            ok = fix_v();
-          if (!ok) break;
+          if (is_k || end || !ok) continue;
           if (dirty) {
             todo = {c, i, boxes_ok, k0, d.kv_lo, d.kv_hi, d.lo_all, d.committed, last};
             pending = true;
           } else {
-            if (last) {
-              if (pending) ok = fix_v();
-              leave_flag(i);
-              if (!ok) break;
-            }
+            if (last) leave_flag(i);
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(kVReady + s));  // nothing to fix
           }
         }
+        if (end) break;
         if (ok) advance(d);
       }
-      if (ok && pending) ok = fix_v();
       if (!ok) fail();
     }
   } else {
@@ -937,19 +970,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int nx = stream_tiles(d, x), step = d.two ? 1 : 2, first = d.two ? 0 : x;
       const uint32_t tcx = x == 0 ? tc0 : tc1;
       float m_ref = -INFINITY, l = 0.f;
-      int64_t blk_next = -1;
+      int32_t blk_next = -1;
       if (lane < p.boxes && nx > 0)
-        blk_next = page_of(p, trow, (int64_t)d.kbase + (d.n - 1 - first) * kKeys + p.box_rows * lane);
+        blk_next = page_of(p, trow, d.kbase + (d.n - 1 - first) * kKeys + p.box_rows * lane);
+#pragma unroll 1
       for (int jj = 0; jj < nx; ++jj) {
         const int32_t k0 = d.kbase + (d.n - 1 - first - jj * step) * kKeys;
         const uint32_t pok = __ballot_sync(0xffffffffu, blk_next >= 0);
         blk_next = -1;
         if (lane < p.boxes && jj + 1 < nx)
-          blk_next = page_of(p, trow, (int64_t)k0 - step * kKeys + p.box_rows * lane);
+          blk_next = page_of(p, trow, k0 - step * kKeys + p.box_rows * lane);
         const bool all_pages = pok == (1u << p.boxes) - 1u;
         // Does every row of this warp see every key of the tile?
         const bool whole = all_pages && k0 >= d.lo_all && k0 + kKeys <= d.committed;
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(kSFull + x), (tcx + jj) & 1))) {
+        if (!__all_sync(0xffffffffu, bar_wait(bar(kSFull + x), (tcx + jj) & 1))) {
           ok = false;
           break;
         }
@@ -1058,7 +1092,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
 
       // (m, l) go to the epilogue's warpgroup, which has read the item before.
-      if (!__all_sync(0xffffffffu, mbar_wait(bar(kORead), (i & 1) ^ 1))) {
+      if (!__all_sync(0xffffffffu, bar_wait(bar(kORead), (i & 1) ^ 1))) {
         fail();
         break;
       }
@@ -1073,21 +1107,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Everything this CTA issued lands before TMEM and shared memory go away.
   if (warp == kMmaWarp && lane == 0) {
     umma_commit(bar(kFinal));
-    mbar_wait(bar(kFinal), 0);
+    bar_wait(bar(kFinal), 0);
   }
   __syncthreads();
   if (abort_sh && tid == 0) {
     if (p.status != nullptr) atomicOr(p.status, kStatusWaitTimeout);
     if (last_issued[0] >= 0) {
       const uint32_t c = (uint32_t)last_issued[0];
-      mbar_wait(bar(kKFull + kslot(c)), kphase(c));
+      bar_wait(bar(kKFull + kslot(c)), kphase(c));
     }
     if (last_issued[1] >= 0) {
       const uint32_t c = (uint32_t)last_issued[1];
-      mbar_wait(bar(kVFull + vslot(c)), vphase(c));
+      bar_wait(bar(kVFull + vslot(c)), vphase(c));
     }
+#pragma unroll 1
     for (int32_t c = max(q_issued - kQStages, 0); c < q_issued; ++c)
-      mbar_wait(bar(kQFull + c % kQStages), (c / kQStages) & 1);
+      bar_wait(bar(kQFull + c % kQStages), (c / kQStages) & 1);
   }
   tc_fence_before();
   __syncthreads();
