@@ -157,7 +157,7 @@ struct TreeParams {
 
 // Positions fit 32 bits (a context is at most 2^30 long).
 __device__ __forceinline__ int32_t block_of(const TreeParams& p, int32_t pos) {
-  return p.bs_shift >= 0 ? pos >> p.bs_shift : pos / p.block_size;
+  return pos >> p.bs_shift;
 }
 __device__ __forceinline__ int32_t page_of(const TreeParams& p, const int64_t* trow, int32_t pos) {
   const int32_t lb = block_of(p, pos);
@@ -167,7 +167,7 @@ __device__ __forceinline__ int32_t page_of(const TreeParams& p, const int64_t* t
 }
 // Slot of position pos on page blk (slots of both planes fit 32 bits).
 __device__ __forceinline__ int32_t slot_of(const TreeParams& p, int32_t blk, int32_t pos) {
-  return blk * p.block_size + pos - block_of(p, pos) * p.block_size;
+  return (blk << p.bs_shift) + (pos & (p.block_size - 1));
 }
 
 __device__ __forceinline__ void touch(const int64_t* at) {
@@ -271,7 +271,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (w < warp) before += v;
     total += v;
   }
-  const int64_t share = max(divide(total + gridDim.x - 1, gridDim.x), (int64_t)kMinShare);
+  // (Past 2^32 cost units the share is the next power of two's.)
+  const int64_t share = max(total < ((int64_t)1 << 32)
+                                ? (int64_t)(((uint32_t)total + gridDim.x - 1) / gridDim.x)
+                                : (total >> (31 - __clz((int)gridDim.x))) + 1,
+                            (int64_t)kMinShare);
   const int64_t my_lo = blockIdx.x * share, my_hi = min(my_lo + share, total);
   if (my_lo >= total) return;
   if (before <= my_lo && my_lo < before + mine) {
@@ -435,33 +439,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               f[e] = __uint_as_float(o[e]) * f_a;
               if (both) f[e] = fmaf(__uint_as_float(u[e]), f_b, f[e]);
             }
-            if (bad && row_valid) {
-              // The non-finite values that this row sees among the replaced ones.
-              const int64_t* trow = p.table + (int64_t)d.r * p.table_stride;
-              const uint64_t* mrow = reinterpret_cast<const uint64_t*>(p.mask) + tok * p.mask_words;
-              const int32_t lo_q =
-                  (int32_t)min(max((int64_t)d.kv_lo, __ldg(p.qstart + tok)), (int64_t)d.committed);
-              const int32_t seg_end = min(d.kbase + d.n * kKeys, d.kv_hi);
-#pragma unroll 1
-              for (int32_t k = max(d.kbase, d.kv_lo); k < seg_end; ++k) {
-                if (k >= d.lo_all && k < d.committed) {
-                  k = d.committed - 1;
-                  continue;
-                }
-                if (!(seen32(d, lo_q, mrow, __ldg(mrow), k) & 1u)) continue;
-                const int32_t blk = page_of(p, trow, k);
-                if (blk < 0) continue;
-                const uint32_t* v = reinterpret_cast<const uint32_t*>(
-                    reinterpret_cast<const T*>(p.cache) +
-                    ((p.num_slots + slot_of(p, blk, k)) * p.num_kv_heads + d.h) * 128 + c0);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  const uint32_t w = __ldg(v + e), b = nonfinite2<T>(w);
-                  if (b & 0x8000u) f[2 * e] += to_float(reinterpret_cast<const T*>(&w)[0]);
-                  if (b & 0x80000000u) f[2 * e + 1] += to_float(reinterpret_cast<const T*>(&w)[1]);
-                }
-              }
-            }
             if (d.slot >= 0) {
               if (row_valid) {
                 float4* dst = p.part_o + (part * 32 + c0 / 4) * kPartRows + part_row;
@@ -482,6 +459,41 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
           }
         }
+        if (bad && row_valid) {
+          // The non-finite values that this row sees among the replaced ones,
+          // added to what was just written.
+          const int64_t* trow = p.table + (int64_t)d.r * p.table_stride;
+          const uint64_t* mrow = reinterpret_cast<const uint64_t*>(p.mask) + tok * p.mask_words;
+          const int32_t lo_q = (int32_t)min(max((int64_t)d.kv_lo, __ldg(p.qstart + tok)), (int64_t)d.committed);
+          const int32_t seg_end = min(d.kbase + d.n * kKeys, d.kv_hi);
+          uint8_t* qrow = smem + kOffQ + (int)((qc + (uint32_t)t) % kQStages) * kTileBytes + row * 128;
+          float* prow = reinterpret_cast<float*>(p.part_o + part * 32 * kPartRows + t * kRows + row);
+#pragma unroll 1
+          for (int32_t k = max(d.kbase, d.kv_lo); k < seg_end; ++k) {
+            if (k >= d.lo_all && k < d.committed) {
+              k = d.committed - 1;
+              continue;
+            }
+            if (!(seen32(d, lo_q, mrow, __ldg(mrow), k) & 1u)) continue;
+            const int32_t blk = page_of(p, trow, k);
+            if (blk < 0) continue;
+            const T* v = reinterpret_cast<const T*>(p.cache) +
+                         ((p.num_slots + slot_of(p, blk, k)) * p.num_kv_heads + d.h) * 128;
+#pragma unroll 1
+            for (int e = 0; e < 128; ++e) {
+              const float f = to_float(v[e]);
+              if (fabsf(f) < INFINITY) continue;
+              if (d.slot >= 0) {
+                prow[(e >> 2) * kPartRows * 4 + (e & 3)] += f;
+              } else {
+                T* cell = reinterpret_cast<T*>(qrow + (e >> 6) * kHalf +
+                                               (((e & 63) >> 3) ^ (row & 7)) * 16) + (e & 7);
+                *cell = from_float<T>(to_float(*cell) + f);
+              }
+            }
+          }
+        }
+        __syncwarp();
         if (t == passes - 1) {  // O and (m, l) are read
           tc_fence_before();
           __syncwarp();
@@ -555,10 +567,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             rc = cost_of(p, e);
             h = pair = 0;
             if (cost0 < my_lo) {  // the share begins inside this request
-              const int64_t in = my_lo - cost0;
-              h = (int32_t)divide(in, rc.head);
-              pair = (int32_t)min(divide(in - h * rc.head, rc.full), (int64_t)(rc.pairs - 1));
-              cost0 += h * rc.head + pair * rc.full;
+#pragma unroll 1
+              for (; my_lo - cost0 >= rc.head; cost0 += rc.head) ++h;
+#pragma unroll 1
+              for (; pair < rc.pairs - 1 && my_lo - cost0 >= rc.full; cost0 += rc.full) ++pair;
             }
             fresh = false;
           }
@@ -658,15 +670,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t dq0 = sw128_desc(sb + kOffQ, 16, 1024);
         const uint64_t dk0 = sw128_desc(sb + kOffK, 16, kGroupBytes);
         const uint64_t dv0 = sw128_desc(sb + kOffV, kAtom, kGroupBytes);
-        auto issue_s = [&](int x, uint32_t qs, uint32_t stage) {
+        auto s_step = [&](int x, uint32_t qs, uint32_t stage, int k) {
           const uint64_t dq = dq0 + (uint64_t)((qs * kTileBytes) >> 4);
           const uint64_t dk = dk0 + (uint64_t)((stage * kTileBytes) >> 4);
+          const uint32_t q_step = (uint32_t)((k >> 2) * (kHalf >> 4) + 2 * (k & 3));
+          const uint32_t k_step = (uint32_t)((k >> 2) * (kAtom >> 4) + 2 * (k & 3));
+          umma_f16(tmem + col_s(x), dq + q_step, dk + k_step, idesc_qk, k > 0);
+        };
+        auto issue_s = [&](int x, uint32_t qs, uint32_t stage) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t q_step = (uint32_t)((k >> 2) * (kHalf >> 4) + 2 * (k & 3));
-            const uint32_t k_step = (uint32_t)((k >> 2) * (kAtom >> 4) + 2 * (k & 3));
-            umma_f16(tmem + col_s(x), dq + q_step, dk + k_step, idesc_qk, k > 0);
-          }
+          for (int k = 0; k < 8; ++k) s_step(x, qs, stage, k);
+          umma_commit(bar(kSFull + x));
+        };
+        // An item's first S: rolled (measured: unrolled MMA issue in the tile
+        // loops is 15 % of them, code fetched once per item costs more than it saves).
+        auto issue_first_s = [&](int x, uint32_t qs, uint32_t stage) {
+#pragma unroll 1
+          for (int k = 0; k < 8; ++k) s_step(x, qs, stage, k);
           umma_commit(bar(kSFull + x));
         };
         // O_x += P_x . V of tile j.  16-key steps with no key of [kv_lo, kv_hi)
@@ -723,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                bar_wait(bar(kKFull + kslot(kvc)), kphase(kvc));
           if (!ok) break;
           tc_fence_after();
-          issue_s(0, qs0, kslot(kvc));
+          issue_first_s(0, qs0, kslot(kvc));
           if (!d.two) umma_commit(bar(kKEmpty + kslot(kvc)));
           if (d.two || n > 1) {  // stream 1: the other query tile, or the next KV tile
             const uint32_t c1 = kvc + (d.two ? 0 : 1);
@@ -731,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                        : bar_wait(bar(kKFull + kslot(c1)), kphase(c1));
             if (!ok) break;
             tc_fence_after();
-            issue_s(1, d.two ? qs1 : qs0, kslot(c1));
+            issue_first_s(1, d.two ? qs1 : qs0, kslot(c1));
             umma_commit(bar(kKEmpty + kslot(c1)));
           }
           if (d.two) {
@@ -1274,12 +1294,8 @@ TreeLayout tree_layout(int64_t ctas) {
   return w;
 }
 
-// Rows of a TMA box: the most that divide a page.
-int box_rows_of(int32_t block_size) {
-  int rows = kKeys;
-  while (rows > 16 && block_size % rows != 0) rows >>= 1;
-  return rows;
-}
+// Rows of a TMA box: a page, or a tile's part of it.
+int box_rows_of(int32_t block_size) { return block_size < kKeys ? block_size : kKeys; }
 
 }  // namespace
 
@@ -1289,7 +1305,8 @@ bool tree_tc_supported(const TreeProblem& a) {
   const int group = a.num_q_heads / a.num_kv_heads;
   const int64_t num_slots = a.num_blocks * a.block_size;
   return (a.dtype == MVB_DTYPE_F16 || a.dtype == MVB_DTYPE_BF16) && a.head_dim == 128 &&
-         group <= 64 && (a.block_size % 16) == 0 && a.num_blocks > 0 &&
+         group <= 64 && a.block_size >= 16 && (a.block_size & (a.block_size - 1)) == 0 &&
+         a.num_blocks > 0 &&
          ((uintptr_t)a.query % 16) == 0 && ((uintptr_t)a.cache % 16) == 0 &&
          ((uintptr_t)a.out % 16) == 0 &&
          (a.num_tokens == 1 || ((a.q_st % 8) == 0 && a.q_st >= 128)) &&
@@ -1343,7 +1360,7 @@ int launch_tree_attention(const TreeProblem& a) {
   p.group = group;
   p.block_q = kRows / group;
   p.block_size = a.block_size;
-  p.bs_shift = (a.block_size & (a.block_size - 1)) == 0 ? __builtin_ctz(a.block_size) : -1;
+  p.bs_shift = __builtin_ctz(a.block_size);
   p.box_rows = box_rows;
   p.boxes = kKeys / box_rows;
   p.num_blocks = a.num_blocks;
