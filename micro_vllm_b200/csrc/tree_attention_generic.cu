@@ -1,23 +1,25 @@
-// Exact CUDA-core attention of draft trees over the paged cache, for every
-// shape the tensor-core kernel does not take: fp32, any head_dim up to 256,
-// any block size, any GQA ratio.  All arithmetic is fp32.
+// Attention of draft trees over the paged cache for every shape that the
+// tcgen05 kernel does not take: fp32, any head_dim up to 256, any block size,
+// any GQA ratio.
 //
 // A CTA takes 32 query rows (node, head of one GQA group) of a request and KV
 // head, and walks the request's keys in tiles of 64: K and V rows come into
-// shared memory once for the 32 rows, converted to fp32.  A warp owns 4 rows:
-// for q.k a lane owns 2 keys (12 shared-memory wavefronts for 32 FMA
-// instructions), for P.V a lane owns 4 columns per 128 (5 wavefronts for 16),
-// so the bound is FMA issue and shared memory together, about half of the
-// fp32 peak; the softmax statistics stay in the warp's registers.
+// shared memory once for the 32 rows, as fp32.  q.k and P.V run on the tensor
+// cores (mma.sync, TF32 operands, fp32 sums) with fp32 accuracy: a value is
+// hi + lo, both TF32 (21 bits), and a product hi hi + hi lo + lo hi.  fp16 and
+// bf16 values have no lo.  On the CUDA cores the same tiles are bound by
+// shared memory (12-18 TFLOP/s; two operand loads for 32 FMA instructions).
+// The softmax is fp32, a warp owning 4 rows, their statistics in registers.
+// Tiles that hold infinities or NaN go through scalar loops: hi and lo of an
+// infinity are no sum, and what a row does not see must not reach it as 0 x NaN.
 //
 // When there are fewer CTAs than the GPU holds, the key axis is cut into
 // `splits` equal parts, whose (max, sum, weighted V) partials a second launch
-// joins in order.  What a row does not see does not reach it: its score is
-// -inf and its value is replaced by 0 (0 x NaN) in the tiles that hold keys
-// not every row sees.
+// joins in order.
 #include <math.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "mvb_common.cuh"
 #include "mvb_internal.h"
@@ -65,17 +67,37 @@ __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* at) 
   return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// DQ: 4-column chunks of a lane (head_dim <= 128 DQ).  kVec: cache rows are
+// x = hi + lo: hi is x rounded to TF32 (10 mantissa bits), lo the rest, of
+// which the MMA reads the upper 10 bits: 21 bits of x in all.  Integer
+// rounding, since conversions run at a quarter of the rate.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
+// NT: 8-column tiles of a warp (head_dim <= 32 NT).  kVec: cache rows are
 // whole, aligned 4-element vectors.
-template <typename T, int DQ, bool kVec>
+template <typename T, int NT, bool kVec>
 __global__ void __launch_bounds__(kThreads) tree_attention_generic_kernel(const TreeProblem p,
                                                                           const GenericParams g) {
+  constexpr int kDim = 32 * NT;                                // padded columns (zeros behind head_dim)
+  constexpr int kQStride = kDim + 4, kVStride = kDim + 8;      // conflict-free fragment loads
+  constexpr int kSStride = kKeyTile + 4;
+  constexpr bool kSplit = std::is_same<T, float>::value;       // q, k and v have a lo
   extern __shared__ __align__(16) float sm[];
   __shared__ int64_t warp_sum_sh[kThreads / 32];
   __shared__ int64_t found_r, found_tile;
   __shared__ int64_t slot_sh[kKeyTile];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int32_t dim = p.head_dim, dim4 = (dim + 3) & ~3, group = p.num_q_heads / p.num_kv_heads;
+  const int32_t dim = p.head_dim, group = p.num_q_heads / p.num_kv_heads;
   const int32_t h = blockIdx.y, split = blockIdx.z;
   T* out = static_cast<T*>(p.out);
 
@@ -131,21 +153,32 @@ __global__ void __launch_bounds__(kThreads) tree_attention_generic_kernel(const 
   // divisions would cost microseconds before the first load.
   const int32_t n_rows = (int32_t)(e.qe - e.qs) * group, row0 = (int32_t)found_tile * kRowTile;
 
-  float* q_sh = sm;                                     // [kRowTile][dim4]
-  float* k_sh = q_sh + kRowTile * dim4;                 // [kKeyTile][dim4 + 4]
-  float* v_sh = k_sh + kKeyTile * (dim4 + 4);           // [kKeyTile][dim4]
-  float* p_sh = v_sh + kKeyTile * dim4 + warp * kKeyTile * kWarpRows;  // this warp's [key][4 rows]
+  float* q_sh = sm;                           // [kRowTile][kQStride]
+  float* k_sh = q_sh + kRowTile * kQStride;   // [kKeyTile][kQStride]
+  float* v_sh = k_sh + kKeyTile * kQStride;   // [kKeyTile][kVStride]
+  float* s_sh = v_sh + kKeyTile * kVStride;   // [kRowTile][kSStride]: scores, then P
+  float* corr_sh = s_sh + kRowTile * kSStride;
   const int32_t wrow = row0 + warp * kWarpRows;  // this warp's rows
+  bool odd_q = false;  // an infinity or NaN
   for (int i = 0; i < kWarpRows; ++i) {
     const int32_t row = wrow + i;
     const T* src = row < n_rows ? static_cast<const T*>(p.query) + (e.qs + row / group) * p.q_st +
                                       (int64_t)(h * group + row % group) * p.q_sh
                                 : nullptr;
-    for (int d = lane; d < dim4; d += 32)
-      q_sh[(warp * kWarpRows + i) * dim4 + d] = src != nullptr && d < dim ? to_float(src[d]) : 0.f;
+    for (int d = lane; d < kDim; d += 32) {
+      const float v = src != nullptr && d < dim ? to_float(src[d]) : 0.f;
+      odd_q |= !finite(v);
+      q_sh[(warp * kWarpRows + i) * kQStride + d] = v;
+    }
   }
+  // Columns behind head_dim stay 0 in every tile.
+  for (int i = tid; i < kKeyTile * (kDim - dim); i += kThreads) {
+    const int key = i / (kDim - dim), d = dim + i % (kDim - dim);
+    k_sh[key * kQStride + d] = 0.f;
+    v_sh[key * kVStride + d] = 0.f;
+  }
+  odd_q = __syncthreads_or(odd_q) != 0;
 
-  const bool active = wrow < n_rows;
   int64_t tok[kWarpRows], lo_row[kWarpRows];
   int64_t lo_all = e.lo;
 #pragma unroll
@@ -155,19 +188,23 @@ __global__ void __launch_bounds__(kThreads) tree_attention_generic_kernel(const 
     lo_row[i] = ok ? min(max(e.lo, __ldg(p.qstart + tok[i])), e.committed) : e.lo;
     lo_all = max(lo_all, lo_row[i]);
   }
-  float m[kWarpRows], l[kWarpRows], acc[DQ][kWarpRows][4];
+  float m[kWarpRows], l[kWarpRows], acc[NT][4];
 #pragma unroll
   for (int i = 0; i < kWarpRows; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
-#pragma unroll
-    for (int c = 0; c < DQ; ++c)
-#pragma unroll
-      for (int d = 0; d < 4; ++d) acc[c][i][d] = 0.f;
   }
+#pragma unroll
+  for (int c = 0; c < NT; ++c)
+#pragma unroll
+    for (int d = 0; d < 4; ++d) acc[c][d] = 0.f;
+  // MMA fragments: 16 rows from r16, keys from 16 (warp / 2), columns from c0;
+  // fr = lane / 4 and fc = lane % 4 place a lane in a fragment.
+  const int r16 = 16 * (warp & 1), key16 = 16 * (warp >> 1), c0 = (warp >> 1) * 8 * NT;
+  const int fr = lane >> 2, fc = lane & 3;
 
-  const int64_t tiles = (e.hi - e.lo + kKeyTile - 1) / kKeyTile;
-  const int64_t share = (tiles + g.splits - 1) / g.splits;
+  const int64_t tiles = ((int32_t)(e.hi - e.lo) + kKeyTile - 1) / kKeyTile;
+  const int64_t share = ((int32_t)tiles + g.splits - 1) / g.splits;
   const int64_t j0 = min(split * share, tiles), j1 = min(j0 + share, tiles);
   const T* cache = static_cast<const T*>(p.cache);
   const int64_t plane = p.num_blocks * p.block_size * p.num_kv_heads * dim;
@@ -188,13 +225,14 @@ __global__ void __launch_bounds__(kThreads) tree_attention_generic_kernel(const 
       slot_sh[tid] = slot;
     }
     __syncthreads();
-    // A warp takes every eighth key, a lane 4 columns per 128.
+    // A warp takes every eighth key.
+    bool odd = odd_q;
     if constexpr (kVec) {
 #pragma unroll 4
       for (int key = warp; key < kKeyTile; key += kThreads / 32) {
         const int64_t slot = slot_sh[key];
 #pragma unroll
-        for (int c = 0; c < DQ; ++c) {
+        for (int c = 0; c < (kDim + 127) / 128; ++c) {
           const int d = 128 * c + 4 * lane;
           if (d >= dim) continue;
           float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
@@ -202,45 +240,79 @@ __global__ void __launch_bounds__(kThreads) tree_attention_generic_kernel(const 
             k = load4<T>(cache + slot + d);
             v = load4<T>(cache + plane + slot + d);
           }
-          *reinterpret_cast<float4*>(k_sh + key * (dim4 + 4) + d) = k;
-          *reinterpret_cast<float4*>(v_sh + key * dim4 + d) = v;
+          // A sum of differences is NaN where a term is not finite.
+          const float zero = (k.x - k.x) + (k.y - k.y) + (k.z - k.z) + (k.w - k.w) + (v.x - v.x) +
+                             (v.y - v.y) + (v.z - v.z) + (v.w - v.w);
+          odd |= zero != 0.f;
+          *reinterpret_cast<float4*>(k_sh + key * kQStride + d) = k;
+          *reinterpret_cast<float4*>(v_sh + key * kVStride + d) = v;
         }
       }
     } else {
       for (int key = warp; key < kKeyTile; key += kThreads / 32) {
         const int64_t slot = slot_sh[key];
-        for (int d = lane; d < dim4; d += 32) {
-          const bool ok = slot >= 0 && d < dim;
-          k_sh[key * (dim4 + 4) + d] = ok ? to_float(cache[slot + d]) : 0.f;
-          v_sh[key * dim4 + d] = ok ? to_float(cache[plane + slot + d]) : 0.f;
+        for (int d = lane; d < dim; d += 32) {
+          const float k = slot >= 0 ? to_float(cache[slot + d]) : 0.f;
+          const float v = slot >= 0 ? to_float(cache[plane + slot + d]) : 0.f;
+          odd |= !finite(k) || !finite(v);
+          k_sh[key * kQStride + d] = k;
+          v_sh[key * kVStride + d] = v;
         }
       }
     }
-    __syncthreads();
-    if (!active) continue;
+    odd = __syncthreads_or(odd) != 0;
 
-    // Scores of 4 rows x this lane's keys k0 + lane and k0 + 32 + lane.
-    float s[2][kWarpRows] = {};
-    const float* qr = q_sh + warp * kWarpRows * dim4;
-    const float* kr = k_sh + lane * (dim4 + 4);
-#pragma unroll 2
-    for (int d = 0; d < dim4; d += 4) {
-      const float4 ka = *reinterpret_cast<const float4*>(kr + d);
-      const float4 kb = *reinterpret_cast<const float4*>(kr + 32 * (dim4 + 4) + d);
+    // Scores: 16 rows x 16 keys of this warp.
+    float s[2][4] = {};
+    const float* qa = q_sh + (r16 + fr) * kQStride + fc;
+    const float* kb = k_sh + (key16 + fr) * kQStride + fc;
+    if (!odd) {
+#pragma unroll 4
+      for (int d = 0; d < kDim; d += 8) {
+        const float a[4] = {qa[d], qa[8 * kQStride + d], qa[d + 4], qa[8 * kQStride + d + 4]};
+        uint32_t ah[4], al[4];
 #pragma unroll
-      for (int i = 0; i < kWarpRows; ++i) {
-        const float4 q = *reinterpret_cast<const float4*>(qr + i * dim4 + d);
-        s[0][i] = fmaf(q.w, ka.w, fmaf(q.z, ka.z, fmaf(q.y, ka.y, fmaf(q.x, ka.x, s[0][i]))));
-        s[1][i] = fmaf(q.w, kb.w, fmaf(q.z, kb.z, fmaf(q.y, kb.y, fmaf(q.x, kb.x, s[1][i]))));
+        for (int i = 0; i < 4; ++i) split_tf32(a[i], ah[i], al[i]);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          uint32_t bh[2], bl[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) split_tf32(kb[8 * n * kQStride + d + 4 * i], bh[i], bl[i]);
+          if constexpr (kSplit) {
+            mma_tf32(s[n], al, bh[0], bh[1]);
+            mma_tf32(s[n], ah, bl[0], bl[1]);
+          }
+          mma_tf32(s[n], ah, bh[0], bh[1]);
+        }
       }
+    } else {
+      for (int n = 0; n < 2; ++n)
+        for (int i = 0; i < 4; ++i) {
+          const float* qr = q_sh + (r16 + fr + 8 * (i >> 1)) * kQStride;
+          const float* kr = k_sh + (key16 + 8 * n + 2 * fc + (i & 1)) * kQStride;
+          float dot = 0.f;
+          for (int d = 0; d < dim; ++d) dot = fmaf(qr[d], kr[d], dot);
+          s[n][i] = dot;
+        }
     }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<float2*>(s_sh + (r16 + fr + 8 * i) * kSStride + key16 + 8 * n + 2 * fc) =
+            make_float2(s[n][2 * i], s[n][2 * i + 1]);
+    __syncthreads();
+
+    // Softmax of this warp's 4 rows, a lane at keys lane and lane + 32.
     const bool whole = k0 >= lo_all && k0 + kKeyTile <= e.committed &&
                        __all_sync(0xffffffffu, slot_sh[lane] >= 0 && slot_sh[lane + 32] >= 0);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int64_t pos = k0 + 32 * u + lane;
+    for (int i = 0; i < kWarpRows; ++i) {
+      float* row = s_sh + (warp * kWarpRows + i) * kSStride;
+      float x[2];
 #pragma unroll
-      for (int i = 0; i < kWarpRows; ++i) {
+      for (int u = 0; u < 2; ++u) {
+        const int64_t pos = k0 + 32 * u + lane;
         bool seen = whole;
         if (!whole && tok[i] >= 0 && slot_sh[32 * u + lane] >= 0) {
           if (pos < e.committed) {
@@ -250,73 +322,96 @@ __global__ void __launch_bounds__(kThreads) tree_attention_generic_kernel(const 
             seen = ((uint64_t)__ldg(p.mask + tok[i] * p.mask_words + (node >> 6)) >> (node & 63)) & 1u;
           }
         }
-        s[u][i] = seen ? s[u][i] * g.scale_log2 : -INFINITY;
+        x[u] = seen ? row[32 * u + lane] * g.scale_log2 : -INFINITY;
       }
-    }
-#pragma unroll
-    for (int i = 0; i < kWarpRows; ++i) {
-      float top = fmaxf(s[0][i], s[1][i]);
+      float top = fmaxf(x[0], x[1]);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       const float m_new = fmaxf(m[i], top), mu = m_new == -INFINITY ? 0.f : m_new;
       const float corr = exp2f(m[i] - mu);
-      s[0][i] = exp2f(s[0][i] - mu);
-      s[1][i] = exp2f(s[1][i] - mu);
+      x[0] = exp2f(x[0] - mu);
+      x[1] = exp2f(x[1] - mu);
       m[i] = m_new;
-      l[i] = l[i] * corr + warp_sum(s[0][i] + s[1][i]);
-#pragma unroll
-      for (int c = 0; c < DQ; ++c)
-#pragma unroll
-        for (int d = 0; d < 4; ++d) acc[c][i][d] *= corr;
+      l[i] = l[i] * corr + warp_sum(x[0] + x[1]);
+      row[lane] = x[0];
+      row[32 + lane] = x[1];
+      if (lane == 0) corr_sh[warp * kWarpRows + i] = corr;
     }
-    __syncwarp();
+    __syncthreads();
+
+    // O = O corr + P V: 16 rows x 8 NT columns of this warp.
+    const float corr_a = corr_sh[r16 + fr], corr_b = corr_sh[r16 + fr + 8];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      *reinterpret_cast<float4*>(p_sh + (32 * u + lane) * kWarpRows) =
-          make_float4(s[u][0], s[u][1], s[u][2], s[u][3]);
-    __syncwarp();
-    auto weigh = [&](bool guard) {
-#pragma unroll 4
-      for (int key = 0; key < kKeyTile; ++key) {
-        const float4 w4 = *reinterpret_cast<const float4*>(p_sh + key * kWarpRows);
-        const float w[kWarpRows] = {w4.x, w4.y, w4.z, w4.w};
+    for (int c = 0; c < NT; ++c) {
+      acc[c][0] *= corr_a;
+      acc[c][1] *= corr_a;
+      acc[c][2] *= corr_b;
+      acc[c][3] *= corr_b;
+    }
+    const float* pa = s_sh + (r16 + fr) * kSStride + fc;
+    const float* vb = v_sh + fc * kVStride + c0 + fr;
+    if (!odd) {
+#pragma unroll 2
+      for (int k = 0; k < kKeyTile; k += 8) {
+        const float a[4] = {pa[k], pa[8 * kSStride + k], pa[k + 4], pa[8 * kSStride + k + 4]};
+        uint32_t ah[4], al[4];
 #pragma unroll
-        for (int c = 0; c < DQ; ++c) {
-          const int d0 = 128 * c + 4 * lane;
-          if (d0 >= dim4) continue;
-          const float4 v4 = *reinterpret_cast<const float4*>(v_sh + key * dim4 + d0);
-          const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+        for (int i = 0; i < 4; ++i) split_tf32(a[i], ah[i], al[i]);
 #pragma unroll
-          for (int i = 0; i < kWarpRows; ++i)
+        for (int c = 0; c < NT; ++c) {
+          uint32_t bh[2], bl[2];
 #pragma unroll
-            for (int d = 0; d < 4; ++d) acc[c][i][d] = fmaf(w[i], guard && w[i] == 0.f ? 0.f : v[d], acc[c][i][d]);
+          for (int i = 0; i < 2; ++i) split_tf32(vb[(k + 4 * i) * kVStride + 8 * c], bh[i], bl[i]);
+          mma_tf32(acc[c], al, bh[0], bh[1]);
+          if constexpr (kSplit) mma_tf32(acc[c], ah, bl[0], bl[1]);
+          mma_tf32(acc[c], ah, bh[0], bh[1]);
         }
       }
-    };
-    if (whole)
-      weigh(false);
-    else
-      weigh(true);
+    } else {
+#pragma unroll
+      for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float* pr = s_sh + (r16 + fr + 8 * (i >> 1)) * kSStride;
+          const float* vr = v_sh + c0 + 8 * c + 2 * fc + (i & 1);
+          float sum = acc[c][i];
+#pragma unroll 1
+          for (int k = 0; k < kKeyTile; ++k)
+            if (pr[k] != 0.f) sum = fmaf(pr[k], vr[k * kVStride], sum);  // 0: not seen
+          acc[c][i] = sum;
+        }
+    }
   }
-  if (!active) return;
 
+  // Each row's (max, sum) from the warp that owns it to the warps that hold its O.
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWarpRows; ++i)
+    if (lane == 0) {
+      s_sh[(warp * kWarpRows + i) * kSStride] = m[i];
+      s_sh[(warp * kWarpRows + i) * kSStride + 1] = l[i];
+    }
+  __syncthreads();
   const int64_t rows = p.num_tokens * p.num_q_heads;
 #pragma unroll
-  for (int i = 0; i < kWarpRows; ++i) {
-    if (tok[i] < 0) continue;
-    const int64_t row = tok[i] * p.num_q_heads + h * group + (wrow + i) % group;
-    const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-    if (g.splits > 1 && lane == 0) g.part_ml[split * rows + row] = make_float2(m[i], l[i]);
+  for (int i = 0; i < 2; ++i) {
+    const int in_tile = r16 + fr + 8 * i;
+    if (row0 + in_tile >= n_rows) continue;
+    const int64_t row =
+        (e.qs + (row0 + in_tile) / group) * p.num_q_heads + h * group + (row0 + in_tile) % group;
+    const float m_row = s_sh[in_tile * kSStride], l_row = s_sh[in_tile * kSStride + 1];
+    const float inv = l_row == 0.f ? 0.f : 1.f / l_row;
+    if (g.splits > 1 && c0 == 0 && fc == 0) g.part_ml[split * rows + row] = make_float2(m_row, l_row);
 #pragma unroll
-    for (int c = 0; c < DQ; ++c)
+    for (int c = 0; c < NT; ++c)
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const int at_d = 128 * c + 4 * lane + d;
-        if (at_d >= dim) continue;
+      for (int u = 0; u < 2; ++u) {
+        const int d = c0 + 8 * c + 2 * fc + u;
+        if (d >= dim) continue;
         if (g.splits > 1)
-          g.part_o[(split * rows + row) * dim + at_d] = acc[c][i][d];
+          g.part_o[(split * rows + row) * dim + d] = acc[c][2 * i + u];
         else
-          out[row * dim + at_d] = from_float<T>(acc[c][i][d] * inv);
+          out[row * dim + d] = from_float<T>(acc[c][2 * i + u] * inv);
       }
   }
 }
@@ -367,8 +462,11 @@ int32_t splits_for(int64_t num_tokens, int64_t num_requests, int32_t num_q_heads
   return (int32_t)(want < kMaxSplits ? want : kMaxSplits);
 }
 
-template <typename T, int DQ, bool kVec>
-int launch(const TreeProblem& p, const GenericParams& g, dim3 grid, size_t smem) {
+template <typename T, int NT, bool kVec>
+int launch(const TreeProblem& p, const GenericParams& g, dim3 grid) {
+  constexpr int kDim = 32 * NT;
+  constexpr size_t kSmem = sizeof(float) * (kRowTile * (kDim + 4) + kKeyTile * (kDim + 4) + kKeyTile * (kDim + 8) +
+                                            kRowTile * (kKeyTile + 4) + kRowTile);
   static std::mutex lock;
   static bool configured[kMaxDevices] = {};
   int dev = 0;
@@ -376,8 +474,8 @@ int launch(const TreeProblem& p, const GenericParams& g, dim3 grid, size_t smem)
   {
     std::lock_guard<std::mutex> guard(lock);
     if (dev < 0 || dev >= kMaxDevices || !configured[dev]) {
-      const cudaError_t err = cudaFuncSetAttribute(tree_attention_generic_kernel<T, DQ, kVec>,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+      const cudaError_t err = cudaFuncSetAttribute(tree_attention_generic_kernel<T, NT, kVec>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
       if (err != cudaSuccess) {
         set_last_cuda_error(err);
         return MVB_ERR_CUDA;
@@ -385,7 +483,7 @@ int launch(const TreeProblem& p, const GenericParams& g, dim3 grid, size_t smem)
       if (dev >= 0 && dev < kMaxDevices) configured[dev] = true;
     }
   }
-  tree_attention_generic_kernel<T, DQ, kVec><<<grid, kThreads, smem, p.stream>>>(p, g);
+  tree_attention_generic_kernel<T, NT, kVec><<<grid, kThreads, kSmem, p.stream>>>(p, g);
   int rc = check_launch();
   if (rc != MVB_OK || g.splits == 1) return rc;
   const int64_t rows = p.num_tokens * p.num_q_heads;
@@ -394,11 +492,11 @@ int launch(const TreeProblem& p, const GenericParams& g, dim3 grid, size_t smem)
 }
 
 template <typename T>
-int launch_typed(const TreeProblem& p, const GenericParams& g, dim3 grid, size_t smem) {
+int launch_typed(const TreeProblem& p, const GenericParams& g, dim3 grid) {
   const bool vec = p.head_dim % 4 == 0 && ((uintptr_t)p.cache % (4 * sizeof(T))) == 0;
-  if (p.head_dim <= 128)
-    return vec ? launch<T, 1, true>(p, g, grid, smem) : launch<T, 1, false>(p, g, grid, smem);
-  return vec ? launch<T, 2, true>(p, g, grid, smem) : launch<T, 2, false>(p, g, grid, smem);
+  if (p.head_dim <= 64) return vec ? launch<T, 2, true>(p, g, grid) : launch<T, 2, false>(p, g, grid);
+  if (p.head_dim <= 128) return vec ? launch<T, 4, true>(p, g, grid) : launch<T, 4, false>(p, g, grid);
+  return vec ? launch<T, 8, true>(p, g, grid) : launch<T, 8, false>(p, g, grid);
 }
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -433,17 +531,14 @@ int launch_tree_attention_generic(const TreeProblem& p) {
   }
   g.part_ml = static_cast<float2*>(p.workspace);
   g.part_o = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + ml);
-  const int32_t dim4 = (p.head_dim + 3) & ~3;
-  const size_t smem = sizeof(float) * ((size_t)kRowTile * dim4 + kKeyTile * (dim4 + 4) + kKeyTile * dim4 +
-                                       (kThreads / 32) * kKeyTile * kWarpRows);
   const dim3 grid((unsigned)(tiles > 0 ? tiles : 1), (unsigned)p.num_kv_heads, (unsigned)g.splits);
   switch (p.dtype) {
     case MVB_DTYPE_F16:
-      return launch_typed<__half>(p, g, grid, smem);
+      return launch_typed<__half>(p, g, grid);
     case MVB_DTYPE_BF16:
-      return launch_typed<__nv_bfloat16>(p, g, grid, smem);
+      return launch_typed<__nv_bfloat16>(p, g, grid);
     case MVB_DTYPE_F32:
-      return launch_typed<float>(p, g, grid, smem);
+      return launch_typed<float>(p, g, grid);
     default:
       return MVB_ERR_UNSUPPORTED_DTYPE;
   }
