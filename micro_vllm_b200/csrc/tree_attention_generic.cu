@@ -49,10 +49,6 @@ __device__ __forceinline__ int64_t row_tiles(const TreeProblem& p, int64_t r, in
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* at);
 template <>
-__device__ __forceinline__ float4 load4<float>(const float* at) {
-  return __ldg(reinterpret_cast<const float4*>(at));
-}
-template <>
 __device__ __forceinline__ float4 load4<__half>(const __half* at) {
   const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
   const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
@@ -83,42 +79,52 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
 }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
+// 16 bytes to shared memory, zeros where `there` is false (src is not read).
+__device__ __forceinline__ void copy16(float* dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(
+                   (uint32_t)__cvta_generic_to_shared(dst)),
+               "l"(src), "r"(there ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+__device__ __forceinline__ void copy_wait_but_last() {
+  asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+}
+
 // NT: 8-column tiles of a warp (head_dim <= 32 NT).  kVec: cache rows are
 // whole, aligned 4-element vectors.
 template <typename T, int NT, bool kVec>
-__global__ void __launch_bounds__(kThreads) tree_attention_generic_kernel(const TreeProblem p,
-                                                                          const GenericParams g) {
-  constexpr int kDim = 32 * NT;                                // padded columns (zeros behind head_dim)
-  constexpr int kQStride = kDim + 4, kVStride = kDim + 8;      // conflict-free fragment loads
+__global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
+    tree_attention_generic_kernel(const TreeProblem p, const GenericParams g) {
+  constexpr int kDim = 32 * NT;                            // padded columns (zeros behind head_dim)
+  constexpr int kQStride = kDim + 4, kVStride = kDim + 8;  // conflict-free fragment loads
   constexpr int kSStride = kKeyTile + 4;
-  constexpr bool kSplit = std::is_same<T, float>::value;       // q, k and v have a lo
+  constexpr bool kFp32 = std::is_same<T, float>::value;    // q, k and v have a lo
   extern __shared__ __align__(16) float sm[];
   __shared__ int64_t warp_sum_sh[kThreads / 32];
   __shared__ int64_t found_r, found_tile;
-  __shared__ int64_t slot_sh[kKeyTile];
+  __shared__ int64_t slots_sh[2][kKeyTile];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int32_t dim = p.head_dim, group = p.num_q_heads / p.num_kv_heads;
-  const int32_t h = blockIdx.y, split = blockIdx.z;
   T* out = static_cast<T*>(p.out);
 
   // Rows that no request owns, 32 tokens to a warp.
-  if (h == 0 && split == 0) {
-    for (int64_t t0 = 32 * ((int64_t)blockIdx.x * (kThreads / 32) + warp); t0 < p.num_tokens;
-         t0 += 32 * (int64_t)gridDim.x * (kThreads / 32)) {
-      const int64_t t = t0 + lane;
-      bool zero = false;
-      if (t < p.num_tokens) {
-        const int64_t r = find_request(p.qsl, p.num_requests, t);
-        TreeExtent e;
-        zero = r < 0 || !tree_extent(p, r, e);
-      }
-      for (uint32_t todo = __ballot_sync(0xffffffffu, zero); todo != 0; todo &= todo - 1)
-        for (int64_t d = lane; d < (int64_t)p.num_q_heads * dim; d += 32)
-          out[(t0 + __ffs(todo) - 1) * p.num_q_heads * dim + d] = from_float<T>(0.f);
+  for (int64_t t0 = 32 * ((int64_t)warp * gridDim.x + blockIdx.x); t0 < p.num_tokens;
+       t0 += 32 * (int64_t)gridDim.x * (kThreads / 32)) {
+    const int64_t t = t0 + lane;
+    bool zero = false;
+    if (t < p.num_tokens) {
+      const int64_t r = find_request(p.qsl, p.num_requests, t);
+      TreeExtent e;
+      zero = r < 0 || !tree_extent(p, r, e);
     }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, zero); todo != 0; todo &= todo - 1)
+      for (int64_t d = lane; d < (int64_t)p.num_q_heads * dim; d += 32)
+        out[(t0 + __ffs(todo) - 1) * p.num_q_heads * dim + d] = from_float<T>(0.f);
   }
 
-  // The request and row tile of block x.
+  // Row tiles of all requests, counted once; an item is (row tile, KV head,
+  // split), and a CTA takes every gridDim.x-th.
   const int64_t per = (p.num_requests + kThreads - 1) / kThreads;
   const int64_t r_lo = min(tid * per, p.num_requests), r_hi = min(r_lo + per, p.num_requests);
   int64_t mine = 0;
@@ -130,143 +136,147 @@ __global__ void __launch_bounds__(kThreads) tree_attention_generic_kernel(const 
     if (lane >= o) incl += u;
   }
   if (lane == 31) warp_sum_sh[warp] = incl;
-  if (tid == 0) found_r = -1;
   __syncthreads();
-  int64_t at = incl - mine;
-  for (int w = 0; w < warp; ++w) at += warp_sum_sh[w];
-  if (at <= blockIdx.x && blockIdx.x < at + mine) {
-    int64_t r = r_lo;
-    for (;; ++r) {
-      const int64_t n = row_tiles(p, r, group);
-      if (blockIdx.x < at + n) break;
-      at += n;
-    }
-    found_r = r;
-    found_tile = blockIdx.x - at;
+  int64_t first = incl - mine, all = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) first += warp_sum_sh[w];
+    all += warp_sum_sh[w];
   }
-  __syncthreads();
-  const int64_t r = found_r;
-  if (r < 0) return;
-  TreeExtent e;
-  tree_extent(p, r, e);
-  // Rows and positions fit 32 bits (a context is at most 2^30 long); 64-bit
-  // divisions would cost microseconds before the first load.
-  const int32_t n_rows = (int32_t)(e.qe - e.qs) * group, row0 = (int32_t)found_tile * kRowTile;
 
-  float* q_sh = sm;                           // [kRowTile][kQStride]
-  float* k_sh = q_sh + kRowTile * kQStride;   // [kKeyTile][kQStride]
-  float* v_sh = k_sh + kKeyTile * kQStride;   // [kKeyTile][kVStride]
-  float* s_sh = v_sh + kKeyTile * kVStride;   // [kRowTile][kSStride]: scores, then P
+  float* q_sh = sm;                          // [kRowTile][kQStride]
+  float* k_sh = q_sh + kRowTile * kQStride;  // [kKeyTile][kQStride]
+  float* v_sh = k_sh + kKeyTile * kQStride;  // [kKeyTile][kVStride]
+  float* s_sh = v_sh + kKeyTile * kVStride;  // [kRowTile][kSStride]: scores, then P
   float* corr_sh = s_sh + kRowTile * kSStride;
-  const int32_t wrow = row0 + warp * kWarpRows;  // this warp's rows
-  bool odd_q = false;  // an infinity or NaN
-  for (int i = 0; i < kWarpRows; ++i) {
-    const int32_t row = wrow + i;
-    const T* src = row < n_rows ? static_cast<const T*>(p.query) + (e.qs + row / group) * p.q_st +
-                                      (int64_t)(h * group + row % group) * p.q_sh
-                                : nullptr;
-    for (int d = lane; d < kDim; d += 32) {
-      const float v = src != nullptr && d < dim ? to_float(src[d]) : 0.f;
-      odd_q |= !finite(v);
-      q_sh[(warp * kWarpRows + i) * kQStride + d] = v;
-    }
-  }
   // Columns behind head_dim stay 0 in every tile.
   for (int i = tid; i < kKeyTile * (kDim - dim); i += kThreads) {
     const int key = i / (kDim - dim), d = dim + i % (kDim - dim);
     k_sh[key * kQStride + d] = 0.f;
     v_sh[key * kVStride + d] = 0.f;
   }
-  odd_q = __syncthreads_or(odd_q) != 0;
-
-  int64_t tok[kWarpRows], lo_row[kWarpRows];
-  int64_t lo_all = e.lo;
-#pragma unroll
-  for (int i = 0; i < kWarpRows; ++i) {
-    const bool ok = wrow + i < n_rows;
-    tok[i] = ok ? e.qs + (wrow + i) / group : -1;
-    lo_row[i] = ok ? min(max(e.lo, __ldg(p.qstart + tok[i])), e.committed) : e.lo;
-    lo_all = max(lo_all, lo_row[i]);
-  }
-  float m[kWarpRows], l[kWarpRows], acc[NT][4];
-#pragma unroll
-  for (int i = 0; i < kWarpRows; ++i) {
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-  }
-#pragma unroll
-  for (int c = 0; c < NT; ++c)
-#pragma unroll
-    for (int d = 0; d < 4; ++d) acc[c][d] = 0.f;
-  // MMA fragments: 16 rows from r16, keys from 16 (warp / 2), columns from c0;
-  // fr = lane / 4 and fc = lane % 4 place a lane in a fragment.
+  const T* keys = static_cast<const T*>(p.cache);
+  const T* values = keys + p.num_blocks * p.block_size * p.num_kv_heads * dim;
+  const int64_t rows = p.num_tokens * p.num_q_heads;
+  // MMA fragments: 16 rows from r16, keys from key16, columns from c0; fr =
+  // lane / 4 and fc = lane % 4 place a lane in a fragment.
   const int r16 = 16 * (warp & 1), key16 = 16 * (warp >> 1), c0 = (warp >> 1) * 8 * NT;
   const int fr = lane >> 2, fc = lane & 3;
 
-  const int64_t tiles = ((int32_t)(e.hi - e.lo) + kKeyTile - 1) / kKeyTile;
-  const int64_t share = ((int32_t)tiles + g.splits - 1) / g.splits;
-  const int64_t j0 = min(split * share, tiles), j1 = min(j0 + share, tiles);
-  const T* cache = static_cast<const T*>(p.cache);
-  const int64_t plane = p.num_blocks * p.block_size * p.num_kv_heads * dim;
-  const int64_t* trow = p.table + r * p.table_stride;
-  for (int64_t j = j0; j < j1; ++j) {
-    const int64_t k0 = e.lo + j * kKeyTile;
-    __syncthreads();  // the tile before is read
-    if (tid < kKeyTile) {
-      const int32_t pos = (int32_t)k0 + tid, lb = pos / p.block_size;
+  const uint32_t items = (uint32_t)all * (uint32_t)(p.num_kv_heads * g.splits);
+#pragma unroll 1
+  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int32_t split = item % (uint32_t)g.splits;
+    const int32_t h = item / (uint32_t)g.splits % (uint32_t)p.num_kv_heads;
+    const int64_t x = item / (uint32_t)(g.splits * p.num_kv_heads);
+    __syncthreads();  // the item before is done with shared memory
+    if (first <= x && x < first + mine) {
+      int64_t r = r_lo, at = first;
+      for (;; ++r) {
+        const int64_t n = row_tiles(p, r, group);
+        if (x < at + n) break;
+        at += n;
+      }
+      found_r = r;
+      found_tile = x - at;
+    }
+    __syncthreads();
+    const int64_t r = found_r;
+    TreeExtent e;
+    tree_extent(p, r, e);
+    // Rows and positions fit 32 bits (a context is at most 2^30 long); 64-bit
+    // divisions would cost microseconds before the first load.
+    const int32_t n_rows = (int32_t)(e.qe - e.qs) * group, row0 = (int32_t)found_tile * kRowTile;
+    const int32_t tiles = ((int32_t)(e.hi - e.lo) + kKeyTile - 1) / kKeyTile;
+    const int32_t share = (tiles + g.splits - 1) / g.splits;
+    const int32_t j0 = min(split * share, tiles), j1 = min(j0 + share, tiles);
+    const int64_t* trow = p.table + r * p.table_stride;
+
+    // Slots of tile j, by 64 threads; K or V of a tile, a warp taking every
+    // eighth key, asynchronously for fp32.
+    auto look_up = [&](int32_t j) {
+      const int32_t pos = (int32_t)e.lo + j * kKeyTile + tid, lb = pos / p.block_size;
       int64_t slot = -1;
-      if (pos < e.hi) {
+      if (j < j1 && pos < e.hi) {
         const int64_t blk = lb < p.table_width ? __ldg(trow + lb) : -1;
         if (blk >= 0 && blk < p.num_blocks)
           slot = ((blk * p.block_size + pos - lb * p.block_size) * p.num_kv_heads + h) * dim;
         else if (p.status != nullptr)
           atomicOr(p.status, MVB_STATUS_BLOCK_OUT_OF_RANGE);
       }
-      slot_sh[tid] = slot;
-    }
-    __syncthreads();
-    // A warp takes every eighth key.
-    bool odd = odd_q;
-    if constexpr (kVec) {
+      slots_sh[j & 1][tid] = slot;
+    };
+    auto load = [&](int32_t j, const T* from, float* to, int stride) {
+      if (j < j1) {
 #pragma unroll 4
-      for (int key = warp; key < kKeyTile; key += kThreads / 32) {
-        const int64_t slot = slot_sh[key];
+        for (int key = warp; key < kKeyTile; key += kThreads / 32) {
+          const int64_t slot = slots_sh[j & 1][key];
+          if constexpr (kVec) {
 #pragma unroll
-        for (int c = 0; c < (kDim + 127) / 128; ++c) {
-          const int d = 128 * c + 4 * lane;
-          if (d >= dim) continue;
-          float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-          if (slot >= 0) {
-            k = load4<T>(cache + slot + d);
-            v = load4<T>(cache + plane + slot + d);
+            for (int c = 0; c < (kDim + 127) / 128; ++c) {
+              const int d = 128 * c + 4 * lane;
+              if (d >= dim) continue;
+              if constexpr (kFp32)
+                copy16(to + key * stride + d, from + (slot >= 0 ? slot + d : 0), slot >= 0);
+              else
+                *reinterpret_cast<float4*>(to + key * stride + d) =
+                    slot >= 0 ? load4<T>(from + slot + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+          } else {
+            for (int d = lane; d < dim; d += 32)
+              to[key * stride + d] = slot >= 0 ? to_float(from[slot + d]) : 0.f;
           }
-          // A sum of differences is NaN where a term is not finite.
-          const float zero = (k.x - k.x) + (k.y - k.y) + (k.z - k.z) + (k.w - k.w) + (v.x - v.x) +
-                             (v.y - v.y) + (v.z - v.z) + (v.w - v.w);
-          odd |= zero != 0.f;
-          *reinterpret_cast<float4*>(k_sh + key * kQStride + d) = k;
-          *reinterpret_cast<float4*>(v_sh + key * kVStride + d) = v;
         }
       }
-    } else {
-      for (int key = warp; key < kKeyTile; key += kThreads / 32) {
-        const int64_t slot = slot_sh[key];
-        for (int d = lane; d < dim; d += 32) {
-          const float k = slot >= 0 ? to_float(cache[slot + d]) : 0.f;
-          const float v = slot >= 0 ? to_float(cache[plane + slot + d]) : 0.f;
-          odd |= !finite(k) || !finite(v);
-          k_sh[key * kQStride + d] = k;
-          v_sh[key * kVStride + d] = v;
-        }
-      }
-    }
-    odd = __syncthreads_or(odd) != 0;
+      copy_commit();  // a group for every call, so that the waits count alike
+    };
 
-    // Scores: 16 rows x 16 keys of this warp.
-    float s[2][4] = {};
-    const float* qa = q_sh + (r16 + fr) * kQStride + fc;
-    const float* kb = k_sh + (key16 + fr) * kQStride + fc;
-    if (!odd) {
+    if (tid < kKeyTile) look_up(j0);
+    const int32_t wrow = row0 + warp * kWarpRows;  // this warp's rows
+    for (int i = 0; i < kWarpRows; ++i) {
+      const int32_t row = wrow + i;
+      const T* src = row < n_rows ? static_cast<const T*>(p.query) + (e.qs + row / group) * p.q_st +
+                                        (int64_t)(h * group + row % group) * p.q_sh
+                                  : nullptr;
+      for (int d = lane; d < kDim; d += 32)
+        q_sh[(warp * kWarpRows + i) * kQStride + d] = src != nullptr && d < dim ? to_float(src[d]) : 0.f;
+    }
+    int64_t tok[kWarpRows], lo_row[kWarpRows];
+    int64_t lo_all = e.lo;
+#pragma unroll
+    for (int i = 0; i < kWarpRows; ++i) {
+      const bool ok = wrow + i < n_rows;
+      tok[i] = ok ? e.qs + (wrow + i) / group : -1;
+      lo_row[i] = ok ? min(max(e.lo, __ldg(p.qstart + tok[i])), e.committed) : e.lo;
+      lo_all = max(lo_all, lo_row[i]);
+    }
+    float m[kWarpRows], l[kWarpRows], acc[NT][4];
+#pragma unroll
+    for (int i = 0; i < kWarpRows; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+    }
+#pragma unroll
+    for (int c = 0; c < NT; ++c)
+#pragma unroll
+      for (int d = 0; d < 4; ++d) acc[c][d] = 0.f;
+    __syncthreads();
+    load(j0, keys, k_sh, kQStride);
+    load(j0, values, v_sh, kVStride);
+
+#pragma unroll 1
+    for (int32_t j = j0; j < j1; ++j) {
+      // K of the next tile comes in during this one's softmax and P.V, its V
+      // during the next q.k.
+      const int64_t k0 = e.lo + (int64_t)j * kKeyTile;
+      const int64_t* slot_sh = slots_sh[j & 1];
+      copy_wait_but_last();  // K of this tile
+      __syncthreads();
+      if (tid < kKeyTile) look_up(j + 1);
+
+      // Scores: 16 rows x 16 keys of this warp.
+      float s[2][4] = {};
+      const float* qa = q_sh + (r16 + fr) * kQStride + fc;
+      const float* kb = k_sh + (key16 + fr) * kQStride + fc;
 #pragma unroll 4
       for (int d = 0; d < kDim; d += 8) {
         const float a[4] = {qa[d], qa[8 * kQStride + d], qa[d + 4], qa[8 * kQStride + d + 4]};
@@ -278,79 +288,81 @@ __global__ void __launch_bounds__(kThreads) tree_attention_generic_kernel(const 
           uint32_t bh[2], bl[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) split_tf32(kb[8 * n * kQStride + d + 4 * i], bh[i], bl[i]);
-          if constexpr (kSplit) {
+          if constexpr (kFp32) {
             mma_tf32(s[n], al, bh[0], bh[1]);
             mma_tf32(s[n], ah, bl[0], bl[1]);
           }
           mma_tf32(s[n], ah, bh[0], bh[1]);
         }
       }
-    } else {
-      for (int n = 0; n < 2; ++n)
-        for (int i = 0; i < 4; ++i) {
-          const float* qr = q_sh + (r16 + fr + 8 * (i >> 1)) * kQStride;
-          const float* kr = k_sh + (key16 + 8 * n + 2 * fc + (i & 1)) * kQStride;
-          float dot = 0.f;
-          for (int d = 0; d < dim; ++d) dot = fmaf(qr[d], kr[d], dot);
-          s[n][i] = dot;
-        }
-    }
+      // A score that is not finite: q or K is not (or their sum), and the
+      // split product may have made NaN of an infinity.  Then plain sums.
+      bool odd = false;
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+      for (int i = 0; i < 8; ++i) odd |= !finite(s[i >> 2][i & 3]);
+      if (__syncthreads_or(odd)) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<float2*>(s_sh + (r16 + fr + 8 * i) * kSStride + key16 + 8 * n + 2 * fc) =
-            make_float2(s[n][2 * i], s[n][2 * i + 1]);
-    __syncthreads();
-
-    // Softmax of this warp's 4 rows, a lane at keys lane and lane + 32.
-    const bool whole = k0 >= lo_all && k0 + kKeyTile <= e.committed &&
-                       __all_sync(0xffffffffu, slot_sh[lane] >= 0 && slot_sh[lane + 32] >= 0);
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-    for (int i = 0; i < kWarpRows; ++i) {
-      float* row = s_sh + (warp * kWarpRows + i) * kSStride;
-      float x[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int64_t pos = k0 + 32 * u + lane;
-        bool seen = whole;
-        if (!whole && tok[i] >= 0 && slot_sh[32 * u + lane] >= 0) {
-          if (pos < e.committed) {
-            seen = pos >= lo_row[i];
-          } else {
-            const int64_t node = pos - e.committed;
-            seen = ((uint64_t)__ldg(p.mask + tok[i] * p.mask_words + (node >> 6)) >> (node & 63)) & 1u;
+          for (int i = 0; i < 4; ++i) {
+            const float* qr = q_sh + (r16 + fr + 8 * (i >> 1)) * kQStride;
+            const float* kr = k_sh + (key16 + 8 * n + 2 * fc + (i & 1)) * kQStride;
+            float dot = 0.f;
+#pragma unroll 1
+            for (int d = 0; d < dim; ++d) dot = fmaf(qr[d], kr[d], dot);
+            s[n][i] = dot;
           }
-        }
-        x[u] = seen ? row[32 * u + lane] * g.scale_log2 : -INFINITY;
       }
-      float top = fmaxf(x[0], x[1]);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float m_new = fmaxf(m[i], top), mu = m_new == -INFINITY ? 0.f : m_new;
-      const float corr = exp2f(m[i] - mu);
-      x[0] = exp2f(x[0] - mu);
-      x[1] = exp2f(x[1] - mu);
-      m[i] = m_new;
-      l[i] = l[i] * corr + warp_sum(x[0] + x[1]);
-      row[lane] = x[0];
-      row[32 + lane] = x[1];
-      if (lane == 0) corr_sh[warp * kWarpRows + i] = corr;
-    }
-    __syncthreads();
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          *reinterpret_cast<float2*>(s_sh + (r16 + fr + 8 * i) * kSStride + key16 + 8 * n + 2 * fc) =
+              make_float2(s[n][2 * i], s[n][2 * i + 1]);
+      __syncthreads();
+      load(j + 1, keys, k_sh, kQStride);
 
-    // O = O corr + P V: 16 rows x 8 NT columns of this warp.
-    const float corr_a = corr_sh[r16 + fr], corr_b = corr_sh[r16 + fr + 8];
+      // Softmax of this warp's 4 rows, a lane at keys lane and lane + 32.
+      const bool whole = k0 >= lo_all && k0 + kKeyTile <= e.committed &&
+                         __all_sync(0xffffffffu, slot_sh[lane] >= 0 && slot_sh[lane + 32] >= 0);
 #pragma unroll
-    for (int c = 0; c < NT; ++c) {
-      acc[c][0] *= corr_a;
-      acc[c][1] *= corr_a;
-      acc[c][2] *= corr_b;
-      acc[c][3] *= corr_b;
-    }
-    const float* pa = s_sh + (r16 + fr) * kSStride + fc;
-    const float* vb = v_sh + fc * kVStride + c0 + fr;
-    if (!odd) {
+      for (int i = 0; i < kWarpRows; ++i) {
+        float* row = s_sh + (warp * kWarpRows + i) * kSStride;
+        float y[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int64_t pos = k0 + 32 * u + lane;
+          bool seen = whole;
+          if (!whole && tok[i] >= 0 && slot_sh[32 * u + lane] >= 0) {
+            if (pos < e.committed) {
+              seen = pos >= lo_row[i];
+            } else {
+              const int64_t node = pos - e.committed;
+              seen = ((uint64_t)__ldg(p.mask + tok[i] * p.mask_words + (node >> 6)) >> (node & 63)) & 1u;
+            }
+          }
+          y[u] = seen ? row[32 * u + lane] * g.scale_log2 : -INFINITY;
+        }
+        float top = fmaxf(y[0], y[1]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float m_new = fmaxf(m[i], top), mu = m_new == -INFINITY ? 0.f : m_new;
+        const float corr = exp2f(m[i] - mu);
+        y[0] = exp2f(y[0] - mu);
+        y[1] = exp2f(y[1] - mu);
+        m[i] = m_new;
+        l[i] = l[i] * corr + warp_sum(y[0] + y[1]);
+        row[lane] = y[0];
+        row[32 + lane] = y[1];
+        if (lane == 0) corr_sh[warp * kWarpRows + i] = corr;
+      }
+      copy_wait_but_last();  // V of this tile
+      __syncthreads();
+
+      // O = O corr + P V: 16 rows x 8 NT columns of this warp.
+      const float* pa = s_sh + (r16 + fr) * kSStride + fc;
+      const float* vb = v_sh + fc * kVStride + c0 + fr;
+      float t[NT][4] = {};
 #pragma unroll 2
       for (int k = 0; k < kKeyTile; k += 8) {
         const float a[4] = {pa[k], pa[8 * kSStride + k], pa[k + 4], pa[8 * kSStride + k + 4]};
@@ -362,57 +374,72 @@ __global__ void __launch_bounds__(kThreads) tree_attention_generic_kernel(const 
           uint32_t bh[2], bl[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) split_tf32(vb[(k + 4 * i) * kVStride + 8 * c], bh[i], bl[i]);
-          mma_tf32(acc[c], al, bh[0], bh[1]);
-          if constexpr (kSplit) mma_tf32(acc[c], ah, bl[0], bl[1]);
-          mma_tf32(acc[c], ah, bh[0], bh[1]);
+          mma_tf32(t[c], al, bh[0], bh[1]);
+          if constexpr (kFp32) mma_tf32(t[c], ah, bl[0], bl[1]);
+          mma_tf32(t[c], ah, bh[0], bh[1]);
         }
       }
-    } else {
+      // A sum that is not finite: V holds such a value, of a key seen or not.
+      bool odd_v = false;
+#pragma unroll
+      for (int i = 0; i < 4 * NT; ++i) odd_v |= !finite(t[i >> 2][i & 3]);
+      if (__syncthreads_or(odd_v)) {
+#pragma unroll
+        for (int c = 0; c < NT; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float* pr = s_sh + (r16 + fr + 8 * (i >> 1)) * kSStride;
+            const float* vr = v_sh + c0 + 8 * c + 2 * fc + (i & 1);
+            float sum = 0.f;
+#pragma unroll 1
+            for (int k = 0; k < kKeyTile; ++k)
+              if (pr[k] != 0.f) sum = fmaf(pr[k], vr[k * kVStride], sum);  // 0: not seen
+            t[c][i] = sum;
+          }
+        __syncthreads();
+      }
+      const float corr_a = corr_sh[r16 + fr], corr_b = corr_sh[r16 + fr + 8];
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        acc[c][0] = fmaf(acc[c][0], corr_a, t[c][0]);
+        acc[c][1] = fmaf(acc[c][1], corr_a, t[c][1]);
+        acc[c][2] = fmaf(acc[c][2], corr_b, t[c][2]);
+        acc[c][3] = fmaf(acc[c][3], corr_b, t[c][3]);
+      }
+      load(j + 1, values, v_sh, kVStride);
+    }
+
+    // Each row's (max, sum) from the warp that owns it to the warps that hold
+    // its O.
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWarpRows; ++i)
+      if (lane == 0) {
+        s_sh[(warp * kWarpRows + i) * kSStride] = m[i];
+        s_sh[(warp * kWarpRows + i) * kSStride + 1] = l[i];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int in_tile = r16 + fr + 8 * i;
+      if (row0 + in_tile >= n_rows) continue;
+      const int64_t row =
+          (e.qs + (row0 + in_tile) / group) * p.num_q_heads + h * group + (row0 + in_tile) % group;
+      const float m_row = s_sh[in_tile * kSStride], l_row = s_sh[in_tile * kSStride + 1];
+      const float inv = l_row == 0.f ? 0.f : 1.f / l_row;
+      if (g.splits > 1 && c0 == 0 && fc == 0) g.part_ml[split * rows + row] = make_float2(m_row, l_row);
 #pragma unroll
       for (int c = 0; c < NT; ++c)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float* pr = s_sh + (r16 + fr + 8 * (i >> 1)) * kSStride;
-          const float* vr = v_sh + c0 + 8 * c + 2 * fc + (i & 1);
-          float sum = acc[c][i];
-#pragma unroll 1
-          for (int k = 0; k < kKeyTile; ++k)
-            if (pr[k] != 0.f) sum = fmaf(pr[k], vr[k * kVStride], sum);  // 0: not seen
-          acc[c][i] = sum;
+        for (int u = 0; u < 2; ++u) {
+          const int d = c0 + 8 * c + 2 * fc + u;
+          if (d >= dim) continue;
+          if (g.splits > 1)
+            g.part_o[(split * rows + row) * dim + d] = acc[c][2 * i + u];
+          else
+            out[row * dim + d] = from_float<T>(acc[c][2 * i + u] * inv);
         }
     }
-  }
-
-  // Each row's (max, sum) from the warp that owns it to the warps that hold its O.
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kWarpRows; ++i)
-    if (lane == 0) {
-      s_sh[(warp * kWarpRows + i) * kSStride] = m[i];
-      s_sh[(warp * kWarpRows + i) * kSStride + 1] = l[i];
-    }
-  __syncthreads();
-  const int64_t rows = p.num_tokens * p.num_q_heads;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int in_tile = r16 + fr + 8 * i;
-    if (row0 + in_tile >= n_rows) continue;
-    const int64_t row =
-        (e.qs + (row0 + in_tile) / group) * p.num_q_heads + h * group + (row0 + in_tile) % group;
-    const float m_row = s_sh[in_tile * kSStride], l_row = s_sh[in_tile * kSStride + 1];
-    const float inv = l_row == 0.f ? 0.f : 1.f / l_row;
-    if (g.splits > 1 && c0 == 0 && fc == 0) g.part_ml[split * rows + row] = make_float2(m_row, l_row);
-#pragma unroll
-    for (int c = 0; c < NT; ++c)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int d = c0 + 8 * c + 2 * fc + u;
-        if (d >= dim) continue;
-        if (g.splits > 1)
-          g.part_o[(split * rows + row) * dim + d] = acc[c][2 * i + u];
-        else
-          out[row * dim + d] = from_float<T>(acc[c][2 * i + u] * inv);
-      }
   }
 }
 
@@ -516,8 +543,7 @@ int launch_tree_attention_generic(const TreeProblem& p) {
   if (p.head_dim > 256) return MVB_ERR_UNSUPPORTED_SHAPE;
   const int32_t group = p.num_q_heads / p.num_kv_heads;
   const int64_t tiles = row_tile_bound(p.num_tokens, p.num_requests, group);
-  if (tiles > 0x7fffffffLL || p.num_kv_heads > 65535 ||
-      (p.num_tokens * p.num_q_heads + 7) / 8 > 0x7fffffffLL)
+  if (tiles > 0x7fffffffLL || (p.num_tokens * p.num_q_heads + 7) / 8 > 0x7fffffffLL)
     return MVB_ERR_UNSUPPORTED_SHAPE;
   GenericParams g;
   g.splits = splits_for(p.num_tokens, p.num_requests, p.num_q_heads, p.num_kv_heads);
@@ -531,7 +557,9 @@ int launch_tree_attention_generic(const TreeProblem& p) {
   }
   g.part_ml = static_cast<float2*>(p.workspace);
   g.part_o = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + ml);
-  const dim3 grid((unsigned)(tiles > 0 ? tiles : 1), (unsigned)p.num_kv_heads, (unsigned)g.splits);
+  const int64_t items = tiles * p.num_kv_heads * g.splits, most = 2 * (int64_t)num_sms();
+  if (items > 0x7fffffffLL) return MVB_ERR_UNSUPPORTED_SHAPE;
+  const dim3 grid((unsigned)(items < 1 ? 1 : items < most ? items : most));
   switch (p.dtype) {
     case MVB_DTYPE_F16:
       return launch_typed<__half>(p, g, grid);
