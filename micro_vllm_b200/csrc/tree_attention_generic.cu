@@ -6,8 +6,11 @@
 // head, and walks the request's keys in tiles of 64: K and V rows come into
 // shared memory once for the 32 rows, as fp32.  q.k and P.V run on the tensor
 // cores (mma.sync, TF32 operands, fp32 sums) with fp32 accuracy: a value is
-// hi + lo, both TF32 (21 bits), and a product hi hi + hi lo + lo hi.  fp16 and
-// bf16 values have no lo.  On the CUDA cores the same tiles are bound by
+// hi + lo, both TF32 (22 bits), and a product hi hi + hi lo + lo hi.  fp16 and
+// bf16 values have no lo.  The tensor cores cut off what a sum cannot hold, half
+// a last bit each time on average, so the hi products go round several sums (4
+// for q.k, 2 for P.V) and the small ones have their own: one sum for all was
+// 1.4e-6 off at 24 x 1.5K keys, against 5e-7 of a plain fp32 product.  On the CUDA cores the same tiles are bound by
 // shared memory (12-18 TFLOP/s; two operand loads for 32 FMA instructions).
 // The softmax is fp32, a warp owning 4 rows, their statistics in registers.
 // Tiles that hold infinities or NaN go through scalar loops: hi and lo of an
@@ -63,12 +66,11 @@ __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* at) 
   return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// x = hi + lo: hi is x rounded to TF32 (10 mantissa bits), lo the rest, of
-// which the MMA reads the upper 10 bits: 21 bits of x in all.  Integer
+// x = hi + lo, each rounded to TF32 (10 mantissa bits): 22 bits of x.  Integer
 // rounding, since conversions run at a quarter of the rate.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
-  lo = __float_as_uint(x - __uint_as_float(hi));
+  lo = (__float_as_uint(x - __uint_as_float(hi)) + 0x1000u) & 0xffffe000u;
 }
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -274,11 +276,12 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
       if (tid < kKeyTile) look_up(j + 1);
 
       // Scores: 16 rows x 16 keys of this warp.
-      float s[2][4] = {};
+      float big[4][2][4] = {}, s[2][4] = {};
       const float* qa = q_sh + (r16 + fr) * kQStride + fc;
       const float* kb = k_sh + (key16 + fr) * kQStride + fc;
 #pragma unroll 4
       for (int d = 0; d < kDim; d += 8) {
+        const int turn = (d >> 3) & 3;
         const float a[4] = {qa[d], qa[8 * kQStride + d], qa[d + 4], qa[8 * kQStride + d + 4]};
         uint32_t ah[4], al[4];
 #pragma unroll
@@ -292,9 +295,14 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
             mma_tf32(s[n], al, bh[0], bh[1]);
             mma_tf32(s[n], ah, bl[0], bl[1]);
           }
-          mma_tf32(s[n], ah, bh[0], bh[1]);
+          mma_tf32(big[turn][n], ah, bh[0], bh[1]);
         }
       }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          s[n][i] += (big[0][n][i] + big[1][n][i]) + (big[2][n][i] + big[3][n][i]);
       // A score that is not finite: q or K is not (or their sum), and the
       // split product may have made NaN of an infinity.  Then plain sums.
       bool odd = false;
@@ -362,9 +370,10 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
       // O = O corr + P V: 16 rows x 8 NT columns of this warp.
       const float* pa = s_sh + (r16 + fr) * kSStride + fc;
       const float* vb = v_sh + fc * kVStride + c0 + fr;
-      float t[NT][4] = {};
+      float big_t[2][NT][4] = {}, t[NT][4] = {};
 #pragma unroll 2
       for (int k = 0; k < kKeyTile; k += 8) {
+        const int turn = (k >> 3) & 1;
         const float a[4] = {pa[k], pa[8 * kSStride + k], pa[k + 4], pa[8 * kSStride + k + 4]};
         uint32_t ah[4], al[4];
 #pragma unroll
@@ -376,9 +385,13 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
           for (int i = 0; i < 2; ++i) split_tf32(vb[(k + 4 * i) * kVStride + 8 * c], bh[i], bl[i]);
           mma_tf32(t[c], al, bh[0], bh[1]);
           if constexpr (kFp32) mma_tf32(t[c], ah, bl[0], bl[1]);
-          mma_tf32(t[c], ah, bh[0], bh[1]);
+          mma_tf32(big_t[turn][c], ah, bh[0], bh[1]);
         }
       }
+#pragma unroll
+      for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[c][i] += big_t[0][c][i] + big_t[1][c][i];
       // A sum that is not finite: V holds such a value, of a key seen or not.
       bool odd_v = false;
 #pragma unroll
