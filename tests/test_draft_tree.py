@@ -97,9 +97,11 @@ def test_c_entries_refuse_before_touching_the_device(lib) -> None:
     assert tree(words=0) == tree(words=17) == tree(kind=7) == tree(kind=1, param=0) == tree(pointer=None) == bad
     assert tree(rows=0, requests=0) == ok
 
-    def attend(rows=4, requests=1, hq=4, hkv=2, d=128, words=1, dt=0, q=FAKE):
+    def attend(rows=4, requests=1, hq=4, hkv=2, d=128, words=1, dt=0, q=FAKE, scale=1.0):
         return lib.mvb_tree_attention(q, 512, 128, FAKE, FAKE, 4, 16, hkv, d, FAKE, FAKE, FAKE, FAKE, 8, 8, FAKE,
-                                      words, rows, requests, hq, 1.0, dt, None, 0, None, None)
+                                      words, rows, requests, hq, scale, dt, None, 0, None, None)
+
+    assert attend(scale=0.0) == attend(scale=-1.0) == attend(scale=float("nan")) == attend(scale=float("inf")) == bad
 
     assert attend(dt=5) == dtype and attend(hq=3) == shape and attend(rows=0) == ok
     assert attend(rows=-1) == attend(requests=-1) == attend(words=0) == attend(words=17) == attend(q=None) == bad

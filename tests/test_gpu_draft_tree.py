@@ -119,6 +119,11 @@ CASES = [
     ([200], [1000], 6, 2, 128, 64),
     ([3, 17], [250, 6000], 3, 3, 128, 16),
     ([40, 9], [900, 40], 16, 1, 128, 128),
+    ([2, 1], [20000, 9], 8, 1, 128, 16),
+    ([12, 3], [77, 400], 34, 2, 128, 16),
+    ([5], [300], 64, 1, 128, 32),
+    ([300, 1], [64, 700], 4, 2, 128, 256),
+    ([9, 70], [100, 33], 4, 2, 128, 48),
     ([5, 12], [30, 65], 4, 2, 64, 16),
     ([5, 12], [30, 65], 4, 2, 128, 7),
     ([5, 12], [30, 65], 4, 2, 80, 1),
@@ -133,8 +138,8 @@ def test_attention(case, dtype) -> None:
     nodes, committed, hq, hkv, dim, bs = case
     b = tree_batch(nodes, committed, q_heads=hq, kv_heads=hkv, dim=dim, block_size=bs, dtype=dtype, seed=len(nodes) + hq)
     operator, gpu = B200PagedAttentionOperator(), b.to(DEV)
-    out = operator.attend_tree(gpu.query, gpu.cache, build(gpu, max_nodes=200))
-    check_attention(out, b, plain_build(b, words=4))
+    out = operator.attend_tree(gpu.query, gpu.cache, build(gpu, max_nodes=300))
+    check_attention(out, b, plain_build(b, words=5))
     assert operator.read_status(DEV) == 0
 
 
@@ -178,6 +183,33 @@ def test_attention_rows_that_see_nothing_or_have_no_owner_are_zero(dtype) -> Non
     meta[4][4] &= ~(1 << 40)
     check_attention(out, b, meta)
     assert not out[1].any() and not out[rows:].any() and out[5].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
+def test_attention_of_requests_that_do_not_fit_is_zero(dtype) -> None:
+    """More nodes than mask bits, a context shorter than its nodes, rows that
+    run backwards or past the batch: zeros there, and the others unharmed."""
+
+    b = tree_batch([70, 5, 4, 6, 3], [40, 50, 60, 200, 70], dtype=dtype, seed=22)
+    gpu, operator = b.to(DEV), B200PagedAttentionOperator()
+    tree = build(gpu, max_nodes=128)
+    meta = list(plain_build(b, words=2))
+    lengths = tree.attention.context_lengths.clone()
+    lengths[2] = 3  # shorter than its 4 nodes
+    md = tree.attention
+    odd = AttentionMetadata(md.query_positions, md.query_context_start_positions, md.query_start_locations, lengths,
+                            md.block_table, md.slot_mapping, 16)
+    out = operator.attend_tree(gpu.query, gpu.cache, DraftTree(odd, tree.ancestor_mask[:, :1].contiguous()))
+    assert not out[:70].any() and not out[75:79].any()
+    rows = [*range(70, 75), *range(79, 88)]
+    check_attention(out, b, meta, only=rows)
+    starts = md.query_start_locations.clone()
+    starts[2], starts[5] = 60, 1000  # request 1 runs backwards, the last one past the rows
+    odd = AttentionMetadata(md.query_positions, md.query_context_start_positions, starts, md.context_lengths,
+                            md.block_table, md.slot_mapping, 16)
+    out = operator.attend_tree(gpu.query, gpu.cache, DraftTree(odd, tree.ancestor_mask))
+    torch.cuda.synchronize()
+    assert out.shape == gpu.query.shape
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32], ids=["fp16", "bf16", "fp32"])
