@@ -407,7 +407,7 @@ size_t mvb_tree_attention_workspace_size(int64_t max_num_tokens, int64_t max_num
       head_dim <= 0)
     return 0;
   const size_t tc = head_dim == 128 ? tree_workspace_bytes() : 0;
-  const size_t exact = tree_generic_workspace_bytes(max_num_tokens, num_q_heads, head_dim);
+  const size_t exact = tree_generic_workspace_bytes(head_dim);
   return tc > exact ? tc : exact;
 }
 

@@ -78,6 +78,42 @@ __device__ __forceinline__ bool tree_extent(const Problem& p, int64_t r, TreeExt
   return true;
 }
 
+// a / b for a >= 0, b > 0; a 64-bit division is ~800 cycles on the way to
+// the first load of a CTA.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+// Equal shares of a cost axis of `total` units for `ctas` CTAs (from 2^31
+// units on the next power of two's).
+__device__ __forceinline__ int64_t axis_share(int64_t total, uint32_t ctas) {
+  return total < ((int64_t)1 << 31) ? (int64_t)(((uint32_t)total + ctas - 1) / ctas)
+                                    : (total >> (31 - __clz((int)ctas))) + 1;
+}
+// Calls zero(t0, t1) by whole warps for the rows without an owner: before the
+// first request, behind the last, and those of requests that do not fit.
+template <typename Problem, typename Zero>
+__device__ __forceinline__ void for_unowned_rows(const Problem& p, int lane, int64_t warp0, int64_t warps,
+                                                 Zero zero) {
+  for (int64_t r0 = 32 * warp0; r0 < p.num_requests + 2; r0 += 32 * warps) {
+    const int64_t r = r0 + lane;
+    int64_t z0 = 0, z1 = 0;
+    if (r < p.num_requests) {
+      TreeExtent e;
+      if (!tree_extent(p, r, e)) z0 = e.qs, z1 = e.qe;
+    } else if (r == p.num_requests) {
+      z1 = p.num_requests > 0 ? __ldg(p.qsl) : p.num_tokens;
+    } else if (r == p.num_requests + 1 && p.num_requests > 0) {
+      z0 = __ldg(p.qsl + p.num_requests), z1 = p.num_tokens;
+    }
+    z0 = max(z0, (int64_t)0);
+    z1 = min(z1, p.num_tokens);
+    for (uint32_t todo = __ballot_sync(0xffffffffu, z0 < z1); todo != 0; todo &= todo - 1) {
+      const int src = __ffs(todo) - 1;
+      zero(__shfl_sync(0xffffffffu, z0, src), __shfl_sync(0xffffffffu, z1, src));
+    }
+  }
+}
+
 // Programmatic dependent launch (sm_90+): a kernel launched with
 // programmatic stream serialization may start while the kernel before it in
 // the stream still runs; grid_dependency_wait() returns once that kernel has

@@ -242,9 +242,9 @@ struct TreeProblem : AttentionProblem {
   int32_t mask_words;
 };
 int launch_tree_attention_generic(const TreeProblem& p);
-size_t tree_generic_workspace_bytes(int64_t num_tokens, int32_t num_q_heads, int32_t head_dim);
-// The tensor-core kernel: CTAs at most (one per SM; they size its workspace),
-// what it takes, and its launch.
+size_t tree_generic_workspace_bytes(int32_t head_dim);
+// SMs at most (they size the workspaces); what the tcgen05 kernel takes, and
+// its launch.
 constexpr int kMaxTreeCtas = 160;
 size_t tree_workspace_bytes();
 bool tree_tc_supported(const TreeProblem& p);

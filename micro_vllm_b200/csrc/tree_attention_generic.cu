@@ -16,9 +16,11 @@
 // Tiles that hold infinities or NaN go through scalar loops: hi and lo of an
 // infinity are no sum, and what a row does not see must not reach it as 0 x NaN.
 //
-// When there are fewer CTAs than the GPU holds, the key axis is cut into
-// `splits` equal parts, whose (max, sum, weighted V) partials a second launch
-// joins in order.
+// Split.  An item is (32 query rows, KV head); the key tiles of all items lie
+// on one axis with kItemCost for each item's fixed part, and every CTA takes an
+// equal share of it, which it finds itself from the metadata.  An item that
+// share borders cut leaves (max, sum, weighted V) partials, at most a head and a
+// tail per CTA, which the join launch behind adds up in order.
 #include <math.h>
 
 #include <mutex>
@@ -33,20 +35,35 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kRowTile = 32, kWarpRows = 4;
 constexpr int kKeyTile = 64;
-constexpr int kMaxSplits = 32;
+constexpr int kMaxCtas = 2 * kMaxTreeCtas;
+constexpr int kItemCost = 1;  // in key tiles
 
-struct GenericParams {
-  int32_t splits;
-  float scale_log2;
-  float* part_o;    // [splits][row][head_dim]
-  float2* part_ml;  // [splits][row] (max, sum)
+// What the join needs of the item that a CTA starts and does not finish.
+struct CutItem {
+  int64_t qs, cost0, share;  // the request's first token; the item's place on the axis
+  int32_t row0, n_rows, h, tiles, valid;
 };
 
-// Row tiles of request r (0 when it owns no node).
-__device__ __forceinline__ int64_t row_tiles(const TreeProblem& p, int64_t r, int32_t group) {
-  TreeExtent e;
-  if (!tree_extent(p, r, e)) return 0;
-  return ((int32_t)(e.qe - e.qs) * group + kRowTile - 1) / kRowTile;
+struct GenericParams {
+  float scale_log2;
+  float* part_o;    // [CTA][2][kRowTile][head_dim]
+  float2* part_ml;  // [CTA][2][kRowTile] (max, sum)
+  CutItem* cuts;    // [CTA]
+};
+
+// A request's place on the cost axis.
+struct RequestItems {
+  int32_t n_rows, row_tiles, tiles, items;
+  int64_t cost;  // of an item
+};
+__device__ __forceinline__ RequestItems items_of(const TreeProblem& p, const TreeExtent& e, int32_t group) {
+  RequestItems q;
+  q.n_rows = (int32_t)(e.qe - e.qs) * group;
+  q.row_tiles = (q.n_rows + kRowTile - 1) / kRowTile;
+  q.tiles = ((int32_t)(e.hi - e.lo) + kKeyTile - 1) / kKeyTile;
+  q.items = q.row_tiles * p.num_kv_heads;
+  q.cost = kItemCost + q.tiles;
+  return q;
 }
 
 template <typename T>
@@ -104,33 +121,24 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
   constexpr bool kFp32 = std::is_same<T, float>::value;    // q, k and v have a lo
   extern __shared__ __align__(16) float sm[];
   __shared__ int64_t warp_sum_sh[kThreads / 32];
-  __shared__ int64_t found_r, found_tile;
+  __shared__ int64_t start_r_sh, start_at_sh;
   __shared__ int64_t slots_sh[2][kKeyTile];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int32_t dim = p.head_dim, group = p.num_q_heads / p.num_kv_heads;
   T* out = static_cast<T*>(p.out);
+  allow_dependent_launch();  // the join waits for this grid's end before it reads
 
-  // Rows that no request owns, 32 tokens to a warp.
-  for (int64_t t0 = 32 * ((int64_t)warp * gridDim.x + blockIdx.x); t0 < p.num_tokens;
-       t0 += 32 * (int64_t)gridDim.x * (kThreads / 32)) {
-    const int64_t t = t0 + lane;
-    bool zero = false;
-    if (t < p.num_tokens) {
-      const int64_t r = find_request(p.qsl, p.num_requests, t);
-      TreeExtent e;
-      zero = r < 0 || !tree_extent(p, r, e);
-    }
-    for (uint32_t todo = __ballot_sync(0xffffffffu, zero); todo != 0; todo &= todo - 1)
-      for (int64_t d = lane; d < (int64_t)p.num_q_heads * dim; d += 32)
-        out[(t0 + __ffs(todo) - 1) * p.num_q_heads * dim + d] = from_float<T>(0.f);
-  }
-
-  // Row tiles of all requests, counted once; an item is (row tile, KV head,
-  // split), and a CTA takes every gridDim.x-th.
+  // This CTA's share of the cost axis.
   const int64_t per = (p.num_requests + kThreads - 1) / kThreads;
   const int64_t r_lo = min(tid * per, p.num_requests), r_hi = min(r_lo + per, p.num_requests);
+  auto cost_of = [&](int64_t r) -> int64_t {
+    TreeExtent e;
+    if (!tree_extent(p, r, e)) return 0;
+    const RequestItems q = items_of(p, e, group);
+    return q.items * q.cost;
+  };
   int64_t mine = 0;
-  for (int64_t r = r_lo; r < r_hi; ++r) mine += row_tiles(p, r, group);
+  for (int64_t r = r_lo; r < r_hi; ++r) mine += cost_of(r);
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -138,11 +146,27 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
     if (lane >= o) incl += u;
   }
   if (lane == 31) warp_sum_sh[warp] = incl;
+  if (tid == 0) g.cuts[blockIdx.x].valid = 0;
   __syncthreads();
-  int64_t first = incl - mine, all = 0;
+  int64_t before = incl - mine, total = 0;
+#pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) first += warp_sum_sh[w];
-    all += warp_sum_sh[w];
+    const int64_t v = warp_sum_sh[w];
+    if (w < warp) before += v;
+    total += v;
+  }
+  const int64_t share = axis_share(total, gridDim.x);
+  const int64_t my_lo = blockIdx.x * share, my_hi = min(my_lo + share, total);
+  if (my_lo >= total) return;
+  if (before <= my_lo && my_lo < before + mine) {
+    int64_t r = r_lo, at = before;
+    for (;; ++r) {
+      const int64_t c = cost_of(r);
+      if (my_lo < at + c) break;
+      at += c;
+    }
+    start_r_sh = r;
+    start_at_sh = at;
   }
 
   float* q_sh = sm;                          // [kRowTile][kQStride]
@@ -158,40 +182,42 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
   }
   const T* keys = static_cast<const T*>(p.cache);
   const T* values = keys + p.num_blocks * p.block_size * p.num_kv_heads * dim;
-  const int64_t rows = p.num_tokens * p.num_q_heads;
   // MMA fragments: 16 rows from r16, keys from key16, columns from c0; fr =
   // lane / 4 and fc = lane % 4 place a lane in a fragment.
   const int r16 = 16 * (warp & 1), key16 = 16 * (warp >> 1), c0 = (warp >> 1) * 8 * NT;
   const int fr = lane >> 2, fc = lane & 3;
 
-  const uint32_t items = (uint32_t)all * (uint32_t)(p.num_kv_heads * g.splits);
+  __syncthreads();
+  int64_t r = start_r_sh - 1, at = start_at_sh;  // request and its place on the axis
+  TreeExtent e;
+  RequestItems q{};
+  int32_t item = 0;
 #pragma unroll 1
-  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int32_t split = item % (uint32_t)g.splits;
-    const int32_t h = item / (uint32_t)g.splits % (uint32_t)p.num_kv_heads;
-    const int64_t x = item / (uint32_t)(g.splits * p.num_kv_heads);
-    __syncthreads();  // the item before is done with shared memory
-    if (first <= x && x < first + mine) {
-      int64_t r = r_lo, at = first;
-      for (;; ++r) {
-        const int64_t n = row_tiles(p, r, group);
-        if (x < at + n) break;
-        at += n;
-      }
-      found_r = r;
-      found_tile = x - at;
+  for (;; ++item) {
+    if (item >= q.items) {  // the next request with nodes
+      at += q.items * q.cost;
+      if (at >= my_hi) break;
+      do ++r;
+      while (r < p.num_requests && !tree_extent(p, r, e));
+      if (r >= p.num_requests) break;
+      q = items_of(p, e, group);
+      item = my_lo > at ? (int32_t)divide(my_lo - at, q.cost) : 0;
     }
-    __syncthreads();
-    const int64_t r = found_r;
-    TreeExtent e;
-    tree_extent(p, r, e);
+    const int64_t cost0 = at + item * q.cost;
+    if (cost0 >= my_hi) break;
+    const int32_t j0 = (int32_t)min(max(my_lo - cost0 - kItemCost, (int64_t)0), (int64_t)q.tiles);
+    const int32_t j1 = (int32_t)min(max(my_hi - cost0 - kItemCost, (int64_t)0), (int64_t)q.tiles);
+    if (j0 >= j1) continue;
+    __syncthreads();  // the item before is done with shared memory
     // Rows and positions fit 32 bits (a context is at most 2^30 long); 64-bit
     // divisions would cost microseconds before the first load.
-    const int32_t n_rows = (int32_t)(e.qe - e.qs) * group, row0 = (int32_t)found_tile * kRowTile;
-    const int32_t tiles = ((int32_t)(e.hi - e.lo) + kKeyTile - 1) / kKeyTile;
-    const int32_t share = (tiles + g.splits - 1) / g.splits;
-    const int32_t j0 = min(split * share, tiles), j1 = min(j0 + share, tiles);
+    const int32_t h = item / q.row_tiles, row0 = item % q.row_tiles * kRowTile, n_rows = q.n_rows;
+    const bool whole_item = j0 == 0 && j1 == q.tiles;
+    const int64_t part = 2 * (int64_t)blockIdx.x + (j0 == 0 ? 1 : 0);
+    if (j0 == 0 && !whole_item && tid == 0)
+      g.cuts[blockIdx.x] = {e.qs, cost0, share, row0, n_rows, h, q.tiles, 1};
     const int64_t* trow = p.table + r * p.table_stride;
+    const bool active = row0 + r16 < n_rows;  // this warp's MMA rows hold queries
 
     // Slots of tile j, by 64 threads; K or V of a tile, a warp taking every
     // eighth key, asynchronously for fp32.
@@ -234,13 +260,16 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
 
     if (tid < kKeyTile) look_up(j0);
     const int32_t wrow = row0 + warp * kWarpRows;  // this warp's rows
+#pragma unroll
     for (int i = 0; i < kWarpRows; ++i) {
       const int32_t row = wrow + i;
-      const T* src = row < n_rows ? static_cast<const T*>(p.query) + (e.qs + row / group) * p.q_st +
-                                        (int64_t)(h * group + row % group) * p.q_sh
-                                  : nullptr;
-      for (int d = lane; d < kDim; d += 32)
-        q_sh[(warp * kWarpRows + i) * kQStride + d] = src != nullptr && d < dim ? to_float(src[d]) : 0.f;
+      const T* src = static_cast<const T*>(p.query) + (e.qs + row / group) * p.q_st +
+                     (int64_t)(h * group + row % group) * p.q_sh;
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        const int d = 32 * c + lane;
+        q_sh[(warp * kWarpRows + i) * kQStride + d] = row < n_rows && d < dim ? to_float(src[d]) : 0.f;
+      }
     }
     int64_t tok[kWarpRows], lo_row[kWarpRows];
     int64_t lo_all = e.lo;
@@ -279,6 +308,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
       float big[4][2][4] = {}, s[2][4] = {};
       const float* qa = q_sh + (r16 + fr) * kQStride + fc;
       const float* kb = k_sh + (key16 + fr) * kQStride + fc;
+      if (active)
 #pragma unroll 4
       for (int d = 0; d < kDim; d += 8) {
         const int turn = (d >> 3) & 3;
@@ -371,6 +401,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
       const float* pa = s_sh + (r16 + fr) * kSStride + fc;
       const float* vb = v_sh + fc * kVStride + c0 + fr;
       float big_t[2][NT][4] = {}, t[NT][4] = {};
+      if (active)
 #pragma unroll 2
       for (int k = 0; k < kKeyTile; k += 8) {
         const int turn = (k >> 3) & 1;
@@ -440,15 +471,15 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
           (e.qs + (row0 + in_tile) / group) * p.num_q_heads + h * group + (row0 + in_tile) % group;
       const float m_row = s_sh[in_tile * kSStride], l_row = s_sh[in_tile * kSStride + 1];
       const float inv = l_row == 0.f ? 0.f : 1.f / l_row;
-      if (g.splits > 1 && c0 == 0 && fc == 0) g.part_ml[split * rows + row] = make_float2(m_row, l_row);
+      if (!whole_item && c0 == 0 && fc == 0) g.part_ml[part * kRowTile + in_tile] = make_float2(m_row, l_row);
 #pragma unroll
       for (int c = 0; c < NT; ++c)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int d = c0 + 8 * c + 2 * fc + u;
           if (d >= dim) continue;
-          if (g.splits > 1)
-            g.part_o[(split * rows + row) * dim + d] = acc[c][2 * i + u];
+          if (!whole_item)
+            g.part_o[(part * kRowTile + in_tile) * dim + d] = acc[c][2 * i + u];
           else
             out[row * dim + d] = from_float<T>(acc[c][2 * i + u] * inv);
         }
@@ -456,56 +487,70 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
   }
 }
 
-// One warp per owned row: joins the row's splits in order.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) tree_join_kernel(const TreeProblem p, const GenericParams g) {
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = p.num_tokens * p.num_q_heads;
-  const int64_t row = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  const int64_t r = find_request(p.qsl, p.num_requests, row / p.num_q_heads);
-  TreeExtent e;
-  if (r < 0 || !tree_extent(p, r, e)) return;  // written as 0 before
-  float2 ml = make_float2(-INFINITY, 0.f);
-  if (lane < g.splits) ml = __ldcg(g.part_ml + lane * rows + row);
-  float top = ml.x;
+// Joins the partials of the items that were cut, a warp per row, and writes 0
+// to the rows that no request owns.  One block per SM.
+constexpr int kJoinThreads = 1024;
+
+template <typename T, int kLaneCols>
+__global__ void __launch_bounds__(kJoinThreads, 1)
+    tree_join_kernel(const TreeProblem p, const GenericParams g, int32_t ctas) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t warp0 = (int64_t)warp * gridDim.x + blockIdx.x;  // neighbours on different SMs
+  const int64_t warps = (int64_t)gridDim.x * (kJoinThreads / 32);
+  const int32_t dim = p.head_dim, group = p.num_q_heads / p.num_kv_heads;
+  T* out = static_cast<T*>(p.out);
+  // The attention before does not write these rows, and its inputs were there
+  // before it began.
+  for_unowned_rows(p, lane, warp0, warps, [&](int64_t t0, int64_t t1) {
+    const int64_t first = t0 * p.num_q_heads * dim, last = t1 * p.num_q_heads * dim;
+    for (int64_t e = first + lane; e < last; e += 32) out[e] = from_float<T>(0.f);
+  });
+  grid_dependency_wait();
+  for (int64_t job = warp0; job < (int64_t)ctas * kRowTile; job += warps) {
+    const int32_t b0 = (int32_t)(job % ctas), in_tile = (int32_t)(job / ctas);
+    const CutItem c = g.cuts[b0];
+    const int32_t row = c.row0 + in_tile;
+    if (!c.valid || row >= c.n_rows) continue;
+    // Every share from the item's first tile to its last holds some.
+    const int32_t b_last = (int32_t)divide(c.cost0 + kItemCost + c.tiles - 1, c.share);
+    float m = -INFINITY, l = 0.f, o[kLaneCols] = {};
+#pragma unroll 2
+    for (int32_t b = b0; b <= b_last; ++b) {
+      const int64_t at = (2 * (int64_t)b + (b == b0 ? 1 : 0)) * kRowTile + in_tile;
+      const float2 ml = __ldcg(g.part_ml + at);
+      float add[kLaneCols];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float f = exp2f(ml.x - (top == -INFINITY ? 0.f : top));
-  const float l = warp_sum(ml.y * f);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  for (int d0 = 0; d0 < p.head_dim; d0 += 32) {
-    const int d = d0 + lane;
-    float acc = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < g.splits; ++s) {
-      const float fs = __shfl_sync(0xffffffffu, f, s), ls = __shfl_sync(0xffffffffu, ml.y, s);
-      if (d < p.head_dim && ls != 0.f) acc = fmaf(__ldcg(g.part_o + (s * rows + row) * p.head_dim + d), fs, acc);
+      for (int k = 0; k < kLaneCols; ++k)
+        add[k] = 32 * k + lane < dim ? __ldcg(g.part_o + at * dim + 32 * k + lane) : 0.f;
+      const float m_new = fmaxf(m, ml.x), mu = m_new == -INFINITY ? 0.f : m_new;
+      const float f0 = exp2f(m - mu), f1 = exp2f(ml.x - mu);
+      m = m_new;
+      l = l * f0 + ml.y * f1;
+#pragma unroll
+      for (int k = 0; k < kLaneCols; ++k) o[k] = o[k] * f0 + add[k] * f1;
     }
-    if (d < p.head_dim) static_cast<T*>(p.out)[row * p.head_dim + d] = from_float<T>(acc * inv);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* dst = out + ((c.qs + row / group) * p.num_q_heads + (int64_t)c.h * group + row % group) * dim;
+#pragma unroll
+    for (int k = 0; k < kLaneCols; ++k)
+      if (32 * k + lane < dim) dst[32 * k + lane] = from_float<T>(o[k] * inv);
   }
 }
 
-// Row tiles of a batch: at most T G / 32 and one more for each request with
-// a node.
-int64_t row_tile_bound(int64_t num_tokens, int64_t num_requests, int32_t group) {
-  const int64_t requests = num_requests < num_tokens ? num_requests : num_tokens;
-  return num_tokens * group / kRowTile + requests;
-}
-
-// Splits of the key axis: enough CTAs for two on each SM.  Measured in fp32: 2,
-// 4 and 8 CTAs an SM give 158, 192 and 187 us at 1 x 64 nodes x 8K keys and 46,
-// 50 and 60 us at 5 x 12 nodes x 1.5K keys.
-constexpr int64_t kWantCtas = 2 * 148;
-int32_t splits_for(int64_t num_tokens, int64_t num_requests, int32_t num_q_heads, int32_t num_kv_heads) {
-  const int64_t ctas = row_tile_bound(num_tokens, num_requests, num_q_heads / num_kv_heads) * num_kv_heads;
-  if (ctas == 0) return 1;
-  const int64_t want = (kWantCtas + ctas - 1) / ctas;
-  return (int32_t)(want < kMaxSplits ? want : kMaxSplits);
+size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+struct GenericLayout {
+  size_t ml, o, end;  // (the cut items come first)
+};
+GenericLayout generic_layout(int64_t ctas, int32_t head_dim) {
+  GenericLayout w;
+  w.ml = align256((size_t)ctas * sizeof(CutItem));
+  w.o = align256(w.ml + (size_t)ctas * 2 * kRowTile * sizeof(float2));
+  w.end = w.o + (size_t)ctas * 2 * kRowTile * head_dim * sizeof(float);
+  return w;
 }
 
 template <typename T, int NT, bool kVec>
-int launch(const TreeProblem& p, const GenericParams& g, dim3 grid) {
+int launch(const TreeProblem& p) {
   constexpr int kDim = 32 * NT;
   constexpr size_t kSmem = sizeof(float) * (kRowTile * (kDim + 4) + kKeyTile * (kDim + 4) + kKeyTile * (kDim + 8) +
                                             kRowTile * (kKeyTile + 4) + kRowTile);
@@ -525,63 +570,59 @@ int launch(const TreeProblem& p, const GenericParams& g, dim3 grid) {
       if (dev >= 0 && dev < kMaxDevices) configured[dev] = true;
     }
   }
-  tree_attention_generic_kernel<T, NT, kVec><<<grid, kThreads, kSmem, p.stream>>>(p, g);
-  int rc = check_launch();
-  if (rc != MVB_OK || g.splits == 1) return rc;
-  const int64_t rows = p.num_tokens * p.num_q_heads;
-  tree_join_kernel<T><<<(unsigned)((rows + 7) / 8), kThreads, 0, p.stream>>>(p, g);
+  // As many CTAs as the SMs hold (shared memory: two, or one of head_dim > 128).
+  const int sms = num_sms() < kMaxTreeCtas ? num_sms() : kMaxTreeCtas;
+  const int ctas = NT <= 4 ? 2 * sms : sms;
+  const GenericLayout w = generic_layout(ctas, p.head_dim);
+  if (p.workspace == nullptr || ((uintptr_t)p.workspace % 256) != 0) return MVB_ERR_INVALID_ARGUMENT;
+  if (p.workspace_bytes < w.end) return MVB_ERR_WORKSPACE_TOO_SMALL;
+  char* ws = static_cast<char*>(p.workspace);
+  GenericParams g;
+  g.scale_log2 = p.scale * 1.4426950408889634f;
+  g.cuts = reinterpret_cast<CutItem*>(ws);
+  g.part_ml = reinterpret_cast<float2*>(ws + w.ml);
+  g.part_o = reinterpret_cast<float*>(ws + w.o);
+  tree_attention_generic_kernel<T, NT, kVec><<<ctas, kThreads, kSmem, p.stream>>>(p, g);
+  const int rc = check_launch();
+  if (rc != MVB_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)sms);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = p.stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, tree_join_kernel<T, NT>, p, g, (int32_t)ctas);
+  if (err != cudaSuccess) {
+    set_last_cuda_error(err);
+    return MVB_ERR_CUDA;
+  }
   return check_launch();
 }
 
 template <typename T>
-int launch_typed(const TreeProblem& p, const GenericParams& g, dim3 grid) {
+int launch_typed(const TreeProblem& p) {
   const bool vec = p.head_dim % 4 == 0 && ((uintptr_t)p.cache % (4 * sizeof(T))) == 0;
-  if (p.head_dim <= 64) return vec ? launch<T, 2, true>(p, g, grid) : launch<T, 2, false>(p, g, grid);
-  if (p.head_dim <= 128) return vec ? launch<T, 4, true>(p, g, grid) : launch<T, 4, false>(p, g, grid);
-  return vec ? launch<T, 8, true>(p, g, grid) : launch<T, 8, false>(p, g, grid);
+  if (p.head_dim <= 64) return vec ? launch<T, 2, true>(p) : launch<T, 2, false>(p);
+  if (p.head_dim <= 128) return vec ? launch<T, 4, true>(p) : launch<T, 4, false>(p);
+  return vec ? launch<T, 8, true>(p) : launch<T, 8, false>(p);
 }
-
-size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 }  // namespace
 
-// splits x rows is largest for a batch that is split: rows <= 32 x CTAs (a
-// row tile holds 32 of them), so splits x rows <= (kWantCtas / CTAs + 1) rows
-// <= 32 kWantCtas + rows, with CTAs < kWantCtas.
-size_t tree_generic_workspace_bytes(int64_t num_tokens, int32_t num_q_heads, int32_t head_dim) {
-  const int64_t rows = num_tokens * num_q_heads, most = kRowTile * kWantCtas;
-  const size_t n = (size_t)(most + (rows < most ? rows : most));
-  return align256(n * sizeof(float2)) + n * head_dim * sizeof(float) + 256;
-}
+size_t tree_generic_workspace_bytes(int32_t head_dim) { return generic_layout(kMaxCtas, head_dim).end; }
 
 int launch_tree_attention_generic(const TreeProblem& p) {
   if (p.head_dim > 256) return MVB_ERR_UNSUPPORTED_SHAPE;
-  const int32_t group = p.num_q_heads / p.num_kv_heads;
-  const int64_t tiles = row_tile_bound(p.num_tokens, p.num_requests, group);
-  if (tiles > 0x7fffffffLL || (p.num_tokens * p.num_q_heads + 7) / 8 > 0x7fffffffLL)
-    return MVB_ERR_UNSUPPORTED_SHAPE;
-  GenericParams g;
-  g.splits = splits_for(p.num_tokens, p.num_requests, p.num_q_heads, p.num_kv_heads);
-  g.scale_log2 = p.scale * 1.4426950408889634f;
-  const int64_t rows = p.num_tokens * p.num_q_heads;
-  const size_t ml = align256((size_t)g.splits * rows * sizeof(float2));
-  const size_t need = ml + (size_t)g.splits * rows * p.head_dim * sizeof(float);
-  if (g.splits > 1) {
-    if (p.workspace == nullptr || ((uintptr_t)p.workspace % 256) != 0) return MVB_ERR_INVALID_ARGUMENT;
-    if (p.workspace_bytes < need) return MVB_ERR_WORKSPACE_TOO_SMALL;
-  }
-  g.part_ml = static_cast<float2*>(p.workspace);
-  g.part_o = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + ml);
-  const int64_t items = tiles * p.num_kv_heads * g.splits, most = 2 * (int64_t)num_sms();
-  if (items > 0x7fffffffLL) return MVB_ERR_UNSUPPORTED_SHAPE;
-  const dim3 grid((unsigned)(items < 1 ? 1 : items < most ? items : most));
   switch (p.dtype) {
     case MVB_DTYPE_F16:
-      return launch_typed<__half>(p, g, grid);
+      return launch_typed<__half>(p);
     case MVB_DTYPE_BF16:
-      return launch_typed<__nv_bfloat16>(p, g, grid);
+      return launch_typed<__nv_bfloat16>(p);
     case MVB_DTYPE_F32:
-      return launch_typed<float>(p, g, grid);
+      return launch_typed<float>(p);
     default:
       return MVB_ERR_UNSUPPORTED_DTYPE;
   }

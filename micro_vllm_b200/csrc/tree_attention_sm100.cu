@@ -231,12 +231,6 @@ __device__ __forceinline__ int32_t tile_at(int64_t x, int64_t cost0, bool two, i
   const int64_t j = two ? (d + kTileCost2 - 1) / kTileCost2 : (d + kTileCost1 - 1) / kTileCost1;
   return (int32_t)(j < tiles ? j : tiles);
 }
-// a / b for a >= 0, b > 0; a 64-bit division is ~800 cycles on the way to
-// the first load of a CTA.
-__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
-  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_attention_kernel(const __grid_constant__ CUtensorMap qmap,
@@ -283,11 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (w < warp) before += v;
     total += v;
   }
-  // (From 2^31 cost units on the share is the next power of two's.)
-  const int64_t share = max(total < ((int64_t)1 << 31)
-                                ? (int64_t)(((uint32_t)total + gridDim.x - 1) / gridDim.x)
-                                : (total >> (31 - __clz((int)gridDim.x))) + 1,
-                            (int64_t)kMinShare);
+  const int64_t share = max(axis_share(total, gridDim.x), (int64_t)kMinShare);
   const int64_t my_lo = blockIdx.x * share, my_hi = min(my_lo + share, total);
   if (my_lo >= total) return;
   if (before <= my_lo && my_lo < before + mine) {
@@ -1176,30 +1166,13 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t warp0 = (int64_t)warp * gridDim.x + blockIdx.x;  // neighbours on different SMs
   const int64_t warps = (int64_t)gridDim.x * (kMergeThreads / 32);
-  // Rows without an owner: before the first request, behind the last, and
-  // those of requests that do not fit.  The attention before does not write
-  // them, and its inputs were there before it began.
-  for (int64_t r0 = 32 * warp0; r0 < p.num_requests + 2; r0 += 32 * warps) {
-    const int64_t r = r0 + lane;
-    int64_t z0 = 0, z1 = 0;
-    if (r < p.num_requests) {
-      TreeExtent e;
-      if (!tree_extent(p, r, e)) z0 = e.qs, z1 = e.qe;
-    } else if (r == p.num_requests) {
-      z1 = p.num_requests > 0 ? __ldg(p.qsl) : p.num_tokens;
-    } else if (r == p.num_requests + 1 && p.num_requests > 0) {
-      z0 = __ldg(p.qsl + p.num_requests), z1 = p.num_tokens;
-    }
-    z0 = max(z0, (int64_t)0);
-    z1 = min(z1, p.num_tokens);
-    for (uint32_t todo = __ballot_sync(0xffffffffu, z0 < z1); todo != 0; todo &= todo - 1) {
-      const int src = __ffs(todo) - 1;
-      const int64_t first = __shfl_sync(0xffffffffu, z0, src) * p.num_q_heads * 16;
-      const int64_t last = __shfl_sync(0xffffffffu, z1, src) * p.num_q_heads * 16;
-      for (int64_t e = first + lane; e < last; e += 32)
-        reinterpret_cast<uint4*>(p.out)[e] = make_uint4(0, 0, 0, 0);
-    }
-  }
+  // The attention before does not write these rows, and its inputs were there
+  // before it began.
+  for_unowned_rows(p, lane, warp0, warps, [&](int64_t t0, int64_t t1) {
+    const int64_t first = t0 * p.num_q_heads * 16, last = t1 * p.num_q_heads * 16;
+    for (int64_t e = first + lane; e < last; e += 32)
+      reinterpret_cast<uint4*>(p.out)[e] = make_uint4(0, 0, 0, 0);
+  });
   grid_dependency_wait();
   if (tid < kMaxTreeCtas) {
     int32_t n = 0;

@@ -68,7 +68,7 @@ def launch(entry, device: torch.device, what: str, *args) -> None:
     """Calls a C entry whose last argument is the stream, with ``device``
     current and on its current stream, and raises for its status."""
 
-    if torch.cuda.current_device() == device.index:
+    if torch._C._cuda_getDevice() == device.index:
         rc = entry(*args, torch._C._cuda_getCurrentRawStream(device.index))
     else:
         with torch.cuda.device(device):
@@ -78,13 +78,15 @@ def launch(entry, device: torch.device, what: str, *args) -> None:
 
 
 def _vector(name: str, t: torch.Tensor, device: torch.device, size: int | None = None) -> torch.Tensor:
-    if t.dtype != torch.int64 or t.dim() != 1 or t.device != device or (size is not None and t.shape[0] != size):
+    if t.dtype is not torch.int64 or t.dim() != 1 or t.get_device() != device.index \
+            or (size is not None and t.shape[0] != size):
         raise ValueError(f"{name} must be torch.int64 [{'rows' if size is None else size}] on {device}")
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _table(table: torch.Tensor, device: torch.device, requests: int) -> torch.Tensor:
-    if table.dtype != torch.int64 or table.dim() != 2 or table.device != device or table.shape[0] != requests:
+    if table.dtype is not torch.int64 or table.dim() != 2 or table.get_device() != device.index \
+            or table.shape[0] != requests:
         raise ValueError(f"block_table must be torch.int64 [{requests}, width] on {device}")
     return table if table.shape[1] <= 1 or table.stride(1) == 1 else table.contiguous()
 
@@ -132,7 +134,7 @@ def build_draft_tree(
     starts = _vector("query_start_locations", query_start_locations, device, requests + 1)
     table = _table(block_table, device, requests)
     buffer = torch.empty(rows * (3 + words) + requests, dtype=torch.int64, device=device)
-    positions, context_starts, slots, mask, lengths = buffer.split((rows, rows, rows, rows * words, requests))
+    positions, context_starts, slots, mask, lengths = buffer.split_with_sizes((rows, rows, rows, rows * words, requests))
     launch(
         _lib.load().mvb_build_draft_tree, device, "b200_paged draft tree",
         parents.data_ptr(), starts.data_ptr(), committed.data_ptr(), table.data_ptr(),
@@ -181,7 +183,7 @@ def accept_draft_tree(
     starts = _vector("query_start_locations", query_start_locations, device, requests + 1)
     buffer = torch.empty(requests * (2 * max_accepted + 3), dtype=torch.int64, device=device)
     cells = requests * max_accepted
-    nodes, tokens, count, lengths, last = buffer.split((cells, cells, requests, requests, requests))
+    nodes, tokens, count, lengths, last = buffer.split_with_sizes((cells, cells, requests, requests, requests))
     launch(
         _lib.load().mvb_accept_draft_tree, device, "b200_paged draft acceptance",
         draft.data_ptr(), target.data_ptr(), parents.data_ptr(), starts.data_ptr(), committed.data_ptr(),
@@ -197,7 +199,7 @@ class DraftKVCompactor:
     block table).  Each cache is a contiguous [2, NB, bs, Hkv, D]; all have
     one shape, dtype and device."""
 
-    __slots__ = ("layer_kv_caches", "_device", "_dtype", "_sizes")
+    __slots__ = ("layer_kv_caches", "_device", "_dtype", "_sizes", "_pointers")
 
     def __init__(self, layer_kv_caches) -> None:
         caches = tuple(layer_kv_caches)
@@ -221,6 +223,7 @@ class DraftKVCompactor:
         self._device = first.device
         self._dtype = _CACHE_DTYPES[first.dtype]
         self._sizes = tuple(first.shape[1:])
+        self._pointers = ctypes.c_void_p * len(caches)
 
     def __call__(
         self,
@@ -248,7 +251,7 @@ class DraftKVCompactor:
         if not nodes.is_contiguous():
             nodes = nodes.contiguous()
         blocks, block_size, kv_heads, head_dim = self._sizes
-        pointers = (ctypes.c_void_p * len(self.layer_kv_caches))(*(t.data_ptr() for t in self.layer_kv_caches))
+        pointers = self._pointers(*map(torch.Tensor.data_ptr, self.layer_kv_caches))
         launch(
             _lib.load().mvb_compact_draft_kv, device, "b200_paged KV move",
             pointers, len(pointers), blocks, block_size, kv_heads, head_dim, self._dtype,

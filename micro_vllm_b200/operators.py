@@ -249,23 +249,25 @@ class B200PagedAttentionOperator(AttentionOperator):
     def _check_tree(self, query, layer_kv_cache, tree) -> int:
         """Checks that the cache and the tree fit the query; the MVB_DTYPE_*."""
 
-        if query.device.type != "cuda" or layer_kv_cache.device.type != "cuda":
+        if not query.is_cuda or not layer_kv_cache.is_cuda:
             raise RuntimeError("b200_paged attention requires CUDA tensors")
         dtype = _DTYPES.get(query.dtype)
-        if dtype is None or layer_kv_cache.dtype != query.dtype:
+        if dtype is None or layer_kv_cache.dtype is not query.dtype:
             raise ValueError("query and layer_kv_cache must share a float16/bfloat16/float32 dtype")
         if query.dim() != 3 or layer_kv_cache.dim() != 5 or not layer_kv_cache.is_contiguous():
             raise ValueError("expected query [T,H,D] and a contiguous layer_kv_cache [2,NB,bs,Hkv,D]")
+        num_tokens, num_q_heads, query_dim = query.shape
         planes, _, block_size, num_kv_heads, head_dim = layer_kv_cache.shape
-        if planes != 2 or head_dim != query.shape[2] or block_size != tree.attention.block_size:
+        if planes != 2 or head_dim != query_dim or block_size != tree.attention.block_size:
             raise ValueError("layer_kv_cache does not match the query / metadata")
-        if num_kv_heads == 0 or query.shape[1] % num_kv_heads != 0:
+        if num_kv_heads == 0 or num_q_heads % num_kv_heads != 0:
             raise ValueError("num_q_heads must be a multiple of num_kv_heads")
-        if layer_kv_cache.device != query.device:
+        index = query.get_device()
+        if layer_kv_cache.get_device() != index:
             raise ValueError("query and layer_kv_cache must be on one device")
         mask = tree.ancestor_mask
-        if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != query.shape[0] \
-                or not 1 <= mask.shape[1] <= _lib.MVB_MAX_TREE_NODES // 64 or mask.device != query.device:
+        if mask.dtype is not torch.int64 or mask.dim() != 2 or mask.shape[0] != num_tokens \
+                or not 1 <= mask.shape[1] <= _lib.MVB_MAX_TREE_NODES // 64 or mask.get_device() != index:
             raise ValueError("ancestor_mask must be torch.int64 [num_tokens, words] on the query's device")
         return dtype
 
@@ -291,11 +293,13 @@ class B200PagedAttentionOperator(AttentionOperator):
         md_ctx = _meta(md.context_lengths, device, "context_lengths")
         table = md.block_table
         num_requests = md_ctx.numel()
-        if table.dtype != torch.int64 or table.device != device or table.dim() != 2 or table.shape[0] != num_requests:
+        if table.dtype is not torch.int64 or table.get_device() != device.index or table.dim() != 2 \
+                or table.shape[0] != num_requests:
             raise ValueError("metadata.block_table must be torch.int64 [num_requests, width] on the query's device")
         if md_start.numel() != num_tokens or md_qsl.numel() != num_requests + 1:
             raise ValueError("metadata does not match the query")
-        if table.shape[1] > 1 and table.stride(1) != 1:
+        width = table.shape[1]
+        if width > 1 and table.stride(1) != 1:
             table = table.contiguous()
         output = torch.empty((num_tokens, num_q_heads, head_dim), dtype=query.dtype, device=device)
         nbytes = self._lib.mvb_tree_attention_workspace_size(num_tokens, num_requests, num_q_heads, num_kv_heads, head_dim)
@@ -305,7 +309,7 @@ class B200PagedAttentionOperator(AttentionOperator):
             query.data_ptr(), query.stride(0), query.stride(1), output.data_ptr(),
             layer_kv_cache.data_ptr(), num_blocks, block_size, num_kv_heads, head_dim,
             md_start.data_ptr(), md_qsl.data_ptr(), md_ctx.data_ptr(),
-            table.data_ptr(), table.stride(0), table.shape[1], mask.data_ptr(), mask.shape[1],
+            table.data_ptr(), table.stride(0), width, mask.data_ptr(), mask.shape[1],
             num_tokens, num_requests, num_q_heads, 1.0 / math.sqrt(head_dim), dtype,
             workspace.data_ptr(), nbytes, self._state(device).status.data_ptr(),
         )
