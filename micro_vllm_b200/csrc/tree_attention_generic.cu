@@ -83,11 +83,12 @@ __device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16* at) 
   return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// x = hi + lo, each rounded to TF32 (10 mantissa bits): 22 bits of x.  Integer
-// rounding, since conversions run at a quarter of the rate.
+// x = hi + lo, hi rounded to TF32 (10 mantissa bits; in integers, since
+// conversions run at a quarter of the rate).  The tensor cores take the upper
+// 19 bits of lo, so 21 bits of x count.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
   hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
-  lo = (__float_as_uint(x - __uint_as_float(hi)) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
 }
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -117,8 +118,10 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
     tree_attention_generic_kernel(const TreeProblem p, const GenericParams g) {
   constexpr int kDim = 32 * NT;                            // padded columns (zeros behind head_dim)
   constexpr int kQStride = kDim + 4, kVStride = kDim + 8;  // conflict-free fragment loads
+  constexpr int kKStride = kDim + 4;
   constexpr int kSStride = kKeyTile + 4;
   constexpr bool kFp32 = std::is_same<T, float>::value;    // q, k and v have a lo
+  constexpr int kQParts = kFp32 ? 2 : 1;
   extern __shared__ __align__(16) float sm[];
   __shared__ int64_t warp_sum_sh[kThreads / 32];
   __shared__ int64_t start_r_sh, start_at_sh;
@@ -169,15 +172,15 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
     start_at_sh = at;
   }
 
-  float* q_sh = sm;                          // [kRowTile][kQStride]
-  float* k_sh = q_sh + kRowTile * kQStride;  // [kKeyTile][kQStride]
-  float* v_sh = k_sh + kKeyTile * kQStride;  // [kKeyTile][kVStride]
+  float* q_sh = sm;  // [kRowTile][kQStride]; in fp32 (hi, lo): every tile takes it
+  float* k_sh = q_sh + kQParts * kRowTile * kQStride;  // [kKeyTile][kKStride]
+  float* v_sh = k_sh + kKeyTile * kKStride;            // [kKeyTile][kVStride]
   float* s_sh = v_sh + kKeyTile * kVStride;  // [kRowTile][kSStride]: scores, then P
   float* corr_sh = s_sh + kRowTile * kSStride;
   // Columns behind head_dim stay 0 in every tile.
   for (int i = tid; i < kKeyTile * (kDim - dim); i += kThreads) {
     const int key = i / (kDim - dim), d = dim + i % (kDim - dim);
-    k_sh[key * kQStride + d] = 0.f;
+    k_sh[key * kKStride + d] = 0.f;
     v_sh[key * kVStride + d] = 0.f;
   }
   const T* keys = static_cast<const T*>(p.cache);
@@ -268,7 +271,19 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
 #pragma unroll
       for (int c = 0; c < NT; ++c) {
         const int d = 32 * c + lane;
-        q_sh[(warp * kWarpRows + i) * kQStride + d] = row < n_rows && d < dim ? to_float(src[d]) : 0.f;
+        const float x = row < n_rows && d < dim ? to_float(src[d]) : 0.f;
+        const int at_q = (warp * kWarpRows + i) * kQStride + d;
+        if constexpr (kFp32) {
+          // (inf, x) where x has no hi + lo: its scores are not finite, and
+          // the scalar loop takes x.
+          uint32_t hi, lo;
+          split_tf32(x, hi, lo);
+          const bool odd_x = !finite(x) || !finite(__uint_as_float(hi));
+          reinterpret_cast<float2*>(q_sh)[at_q] =
+              make_float2(odd_x ? INFINITY : __uint_as_float(hi), odd_x ? x : __uint_as_float(lo));
+        } else {
+          q_sh[at_q] = x;
+        }
       }
     }
     int64_t tok[kWarpRows], lo_row[kWarpRows];
@@ -291,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
 #pragma unroll
       for (int d = 0; d < 4; ++d) acc[c][d] = 0.f;
     __syncthreads();
-    load(j0, keys, k_sh, kQStride);
+    load(j0, keys, k_sh, kKStride);
     load(j0, values, v_sh, kVStride);
 
 #pragma unroll 1
@@ -306,28 +321,42 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
 
       // Scores: 16 rows x 16 keys of this warp.
       float big[4][2][4] = {}, s[2][4] = {};
-      const float* qa = q_sh + (r16 + fr) * kQStride + fc;
-      const float* kb = k_sh + (key16 + fr) * kQStride + fc;
+      const int qa = (r16 + fr) * kQStride + fc;
+      const float* kb = k_sh + (key16 + fr) * kKStride + fc;
       if (active)
 #pragma unroll 4
-      for (int d = 0; d < kDim; d += 8) {
-        const int turn = (d >> 3) & 3;
-        const float a[4] = {qa[d], qa[8 * kQStride + d], qa[d + 4], qa[8 * kQStride + d + 4]};
-        uint32_t ah[4], al[4];
+        for (int d = 0; d < kDim; d += 8) {
+          const int turn = (d >> 3) & 3;
+          uint32_t ah[4], al[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split_tf32(a[i], ah[i], al[i]);
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          uint32_t bh[2], bl[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) split_tf32(kb[8 * n * kQStride + d + 4 * i], bh[i], bl[i]);
-          if constexpr (kFp32) {
-            mma_tf32(s[n], al, bh[0], bh[1]);
-            mma_tf32(s[n], ah, bl[0], bl[1]);
+          for (int i = 0; i < 4; ++i) {
+            const int at_q = qa + 8 * (i & 1) * kQStride + d + 4 * (i >> 1);
+            if constexpr (kFp32) {
+              const float2 x = reinterpret_cast<const float2*>(q_sh)[at_q];
+              ah[i] = __float_as_uint(x.x);
+              al[i] = __float_as_uint(x.y);
+            } else {
+              ah[i] = __float_as_uint(q_sh[at_q]);
+            }
           }
-          mma_tf32(big[turn][n], ah, bh[0], bh[1]);
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            uint32_t bh[2], bl[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float x = kb[8 * n * kKStride + d + 4 * i];
+              if constexpr (kFp32)
+                split_tf32(x, bh[i], bl[i]);
+              else
+                bh[i] = __float_as_uint(x);
+            }
+            if constexpr (kFp32) {
+              mma_tf32(s[n], al, bh[0], bh[1]);
+              mma_tf32(s[n], ah, bl[0], bl[1]);
+            }
+            mma_tf32(big[turn][n], ah, bh[0], bh[1]);
+          }
         }
-      }
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -343,11 +372,18 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float* qr = q_sh + (r16 + fr + 8 * (i >> 1)) * kQStride;
-            const float* kr = k_sh + (key16 + 8 * n + 2 * fc + (i & 1)) * kQStride;
+            const int qr = (r16 + fr + 8 * (i >> 1)) * kQStride;
+            const float* kr = k_sh + (key16 + 8 * n + 2 * fc + (i & 1)) * kKStride;
             float dot = 0.f;
 #pragma unroll 1
-            for (int d = 0; d < dim; ++d) dot = fmaf(qr[d], kr[d], dot);
+            for (int d = 0; d < dim; ++d) {
+              float x = q_sh[kQParts * (qr + d)];
+              if constexpr (kFp32) {
+                const float lo = q_sh[2 * (qr + d) + 1];
+                x = finite(x) ? x + lo : lo;
+              }
+              dot = fmaf(x, kr[d], dot);
+            }
             s[n][i] = dot;
           }
       }
@@ -358,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
           *reinterpret_cast<float2*>(s_sh + (r16 + fr + 8 * i) * kSStride + key16 + 8 * n + 2 * fc) =
               make_float2(s[n][2 * i], s[n][2 * i + 1]);
       __syncthreads();
-      load(j + 1, keys, k_sh, kQStride);
+      load(j + 1, keys, k_sh, kKStride);
 
       // Softmax of this warp's 4 rows, a lane at keys lane and lane + 32.
       const bool whole = k0 >= lo_all && k0 + kKeyTile <= e.committed &&
@@ -403,22 +439,28 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
       float big_t[2][NT][4] = {}, t[NT][4] = {};
       if (active)
 #pragma unroll 2
-      for (int k = 0; k < kKeyTile; k += 8) {
-        const int turn = (k >> 3) & 1;
-        const float a[4] = {pa[k], pa[8 * kSStride + k], pa[k + 4], pa[8 * kSStride + k + 4]};
-        uint32_t ah[4], al[4];
+        for (int k = 0; k < kKeyTile; k += 8) {
+          const int turn = (k >> 3) & 1;
+          const float a[4] = {pa[k], pa[8 * kSStride + k], pa[k + 4], pa[8 * kSStride + k + 4]};
+          uint32_t ah[4], al[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split_tf32(a[i], ah[i], al[i]);
+          for (int i = 0; i < 4; ++i) split_tf32(a[i], ah[i], al[i]);
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
-          uint32_t bh[2], bl[2];
+          for (int c = 0; c < NT; ++c) {
+            uint32_t bh[2], bl[2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) split_tf32(vb[(k + 4 * i) * kVStride + 8 * c], bh[i], bl[i]);
-          mma_tf32(t[c], al, bh[0], bh[1]);
-          if constexpr (kFp32) mma_tf32(t[c], ah, bl[0], bl[1]);
-          mma_tf32(big_t[turn][c], ah, bh[0], bh[1]);
+            for (int i = 0; i < 2; ++i) {
+              const float x = vb[(k + 4 * i) * kVStride + 8 * c];
+              if constexpr (kFp32)
+                split_tf32(x, bh[i], bl[i]);
+              else
+                bh[i] = __float_as_uint(x);
+            }
+            mma_tf32(t[c], al, bh[0], bh[1]);
+            if constexpr (kFp32) mma_tf32(t[c], ah, bl[0], bl[1]);
+            mma_tf32(big_t[turn][c], ah, bh[0], bh[1]);
+          }
         }
-      }
 #pragma unroll
       for (int c = 0; c < NT; ++c)
 #pragma unroll
@@ -552,7 +594,8 @@ GenericLayout generic_layout(int64_t ctas, int32_t head_dim) {
 template <typename T, int NT, bool kVec>
 int launch(const TreeProblem& p) {
   constexpr int kDim = 32 * NT;
-  constexpr size_t kSmem = sizeof(float) * (kRowTile * (kDim + 4) + kKeyTile * (kDim + 4) + kKeyTile * (kDim + 8) +
+  constexpr int kQParts = std::is_same<T, float>::value ? 2 : 1;
+  constexpr size_t kSmem = sizeof(float) * (kQParts * kRowTile * (kDim + 4) + kKeyTile * (kDim + 4) + kKeyTile * (kDim + 8) +
                                             kRowTile * (kKeyTile + 4) + kRowTile);
   static std::mutex lock;
   static bool configured[kMaxDevices] = {};
