@@ -224,13 +224,17 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
 
     // Slots of tile j, by 64 threads; K or V of a tile, a warp taking every
     // eighth key, asynchronously for fp32.
-    auto look_up = [&](int32_t j) {
+    auto block_of = [&](int32_t j) -> int64_t {
       const int32_t pos = (int32_t)e.lo + j * kKeyTile + tid, lb = pos / p.block_size;
+      return tid < kKeyTile && j < j1 && pos < e.hi && lb < p.table_width ? __ldg(trow + lb) : -1;
+    };
+    auto put_slot = [&](int32_t j, int64_t blk) {
+      if (tid >= kKeyTile) return;
+      const int32_t pos = (int32_t)e.lo + j * kKeyTile + tid;
       int64_t slot = -1;
       if (j < j1 && pos < e.hi) {
-        const int64_t blk = lb < p.table_width ? __ldg(trow + lb) : -1;
         if (blk >= 0 && blk < p.num_blocks)
-          slot = ((blk * p.block_size + pos - lb * p.block_size) * p.num_kv_heads + h) * dim;
+          slot = ((blk * p.block_size + pos % p.block_size) * p.num_kv_heads + h) * dim;
         else if (p.status != nullptr)
           atomicOr(p.status, MVB_STATUS_BLOCK_OUT_OF_RANGE);
       }
@@ -261,17 +265,36 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
       copy_commit();  // a group for every call, so that the waits count alike
     };
 
-    if (tid < kKeyTile) look_up(j0);
+    // The first block ids, the windows and the query rows come in together.
+    const int64_t first_block = block_of(j0);
     const int32_t wrow = row0 + warp * kWarpRows;  // this warp's rows
+    const int32_t lo = (int32_t)e.lo, committed = (int32_t)e.committed;
+    int32_t node_of[kWarpRows], lo_row[kWarpRows];  // -1: no row
+    int32_t lo_all = lo;
+#pragma unroll
+    for (int i = 0; i < kWarpRows; ++i) {
+      const bool ok = wrow + i < n_rows;
+      node_of[i] = ok ? (wrow + i) / group : -1;
+      lo_row[i] = ok ? (int32_t)min(max(e.lo, __ldg(p.qstart + e.qs + node_of[i])), e.committed) : lo;
+      lo_all = max(lo_all, lo_row[i]);
+    }
+    float q_in[kWarpRows][NT];
 #pragma unroll
     for (int i = 0; i < kWarpRows; ++i) {
       const int32_t row = wrow + i;
       const T* src = static_cast<const T*>(p.query) + (e.qs + row / group) * p.q_st +
                      (int64_t)(h * group + row % group) * p.q_sh;
 #pragma unroll
+      for (int c = 0; c < NT; ++c)
+        q_in[i][c] = row < n_rows && 32 * c + lane < dim ? to_float(src[32 * c + lane]) : 0.f;
+    }
+    put_slot(j0, first_block);
+#pragma unroll
+    for (int i = 0; i < kWarpRows; ++i)
+#pragma unroll
       for (int c = 0; c < NT; ++c) {
         const int d = 32 * c + lane;
-        const float x = row < n_rows && d < dim ? to_float(src[d]) : 0.f;
+        const float x = q_in[i][c];
         const int at_q = (warp * kWarpRows + i) * kQStride + d;
         if constexpr (kFp32) {
           // (inf, x) where x has no hi + lo: its scores are not finite, and
@@ -285,16 +308,6 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
           q_sh[at_q] = x;
         }
       }
-    }
-    int64_t tok[kWarpRows], lo_row[kWarpRows];
-    int64_t lo_all = e.lo;
-#pragma unroll
-    for (int i = 0; i < kWarpRows; ++i) {
-      const bool ok = wrow + i < n_rows;
-      tok[i] = ok ? e.qs + (wrow + i) / group : -1;
-      lo_row[i] = ok ? min(max(e.lo, __ldg(p.qstart + tok[i])), e.committed) : e.lo;
-      lo_all = max(lo_all, lo_row[i]);
-    }
     float m[kWarpRows], l[kWarpRows], acc[NT][4];
 #pragma unroll
     for (int i = 0; i < kWarpRows; ++i) {
@@ -313,11 +326,11 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
     for (int32_t j = j0; j < j1; ++j) {
       // K of the next tile comes in during this one's softmax and P.V, its V
       // during the next q.k.
-      const int64_t k0 = e.lo + (int64_t)j * kKeyTile;
+      const int32_t k0 = lo + j * kKeyTile;
       const int64_t* slot_sh = slots_sh[j & 1];
       copy_wait_but_last();  // K of this tile
       __syncthreads();
-      if (tid < kKeyTile) look_up(j + 1);
+      const int64_t next_block = block_of(j + 1);  // in flight during q.k
 
       // Scores: 16 rows x 16 keys of this warp.
       float big[4][2][4] = {}, s[2][4] = {};
@@ -393,41 +406,52 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
         for (int i = 0; i < 2; ++i)
           *reinterpret_cast<float2*>(s_sh + (r16 + fr + 8 * i) * kSStride + key16 + 8 * n + 2 * fc) =
               make_float2(s[n][2 * i], s[n][2 * i + 1]);
+      put_slot(j + 1, next_block);
       __syncthreads();
       load(j + 1, keys, k_sh, kKStride);
 
       // Softmax of this warp's 4 rows, a lane at keys lane and lane + 32.
-      const bool whole = k0 >= lo_all && k0 + kKeyTile <= e.committed &&
+      const bool whole = k0 >= lo_all && k0 + kKeyTile <= committed &&
                          __all_sync(0xffffffffu, slot_sh[lane] >= 0 && slot_sh[lane + 32] >= 0);
+      float* const rows_sh = s_sh + warp * kWarpRows * kSStride + lane;
+      float y[kWarpRows][2], top[kWarpRows];
+#pragma unroll
+      for (int i = 0; i < kWarpRows; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) y[i][u] = rows_sh[i * kSStride + 32 * u] * g.scale_log2;
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < kWarpRows; ++i)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int32_t pos = k0 + 32 * u + lane, key_node = pos - committed;
+            bool seen = false;
+            if (node_of[i] >= 0 && slot_sh[32 * u + lane] >= 0) {
+              if (key_node < 0)
+                seen = pos >= lo_row[i];
+              else
+                seen = ((uint64_t)__ldg(p.mask + (e.qs + node_of[i]) * p.mask_words + (key_node >> 6)) >>
+                        (key_node & 63)) & 1u;
+            }
+            if (!seen) y[i][u] = -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < kWarpRows; ++i) top[i] = fmaxf(y[i][0], y[i][1]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < kWarpRows; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
 #pragma unroll
       for (int i = 0; i < kWarpRows; ++i) {
-        float* row = s_sh + (warp * kWarpRows + i) * kSStride;
-        float y[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int64_t pos = k0 + 32 * u + lane;
-          bool seen = whole;
-          if (!whole && tok[i] >= 0 && slot_sh[32 * u + lane] >= 0) {
-            if (pos < e.committed) {
-              seen = pos >= lo_row[i];
-            } else {
-              const int64_t node = pos - e.committed;
-              seen = ((uint64_t)__ldg(p.mask + tok[i] * p.mask_words + (node >> 6)) >> (node & 63)) & 1u;
-            }
-          }
-          y[u] = seen ? row[32 * u + lane] * g.scale_log2 : -INFINITY;
-        }
-        float top = fmaxf(y[0], y[1]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float m_new = fmaxf(m[i], top), mu = m_new == -INFINITY ? 0.f : m_new;
+        const float m_new = fmaxf(m[i], top[i]), mu = m_new == -INFINITY ? 0.f : m_new;
         const float corr = exp2f(m[i] - mu);
-        y[0] = exp2f(y[0] - mu);
-        y[1] = exp2f(y[1] - mu);
+        y[i][0] = exp2f(y[i][0] - mu);
+        y[i][1] = exp2f(y[i][1] - mu);
         m[i] = m_new;
-        l[i] = l[i] * corr + warp_sum(y[0] + y[1]);
-        row[lane] = y[0];
-        row[32 + lane] = y[1];
+        l[i] = fmaf(l[i], corr, y[i][0] + y[i][1]);  // this lane's keys
+        rows_sh[i * kSStride] = y[i][0];
+        rows_sh[i * kSStride + 32] = y[i][1];
         if (lane == 0) corr_sh[warp * kWarpRows + i] = corr;
       }
       copy_wait_but_last();  // V of this tile
@@ -498,6 +522,8 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
     // Each row's (max, sum) from the warp that owns it to the warps that hold
     // its O.
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWarpRows; ++i) l[i] = warp_sum(l[i]);
 #pragma unroll
     for (int i = 0; i < kWarpRows; ++i)
       if (lane == 0) {
