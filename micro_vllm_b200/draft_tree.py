@@ -133,7 +133,7 @@ def build_draft_tree(
     rows, requests, words = parents.shape[0], committed.shape[0], (max_nodes + 63) // 64
     starts = _vector("query_start_locations", query_start_locations, device, requests + 1)
     table = _table(block_table, device, requests)
-    buffer = torch.empty(rows * (3 + words) + requests, dtype=torch.int64, device=device)
+    buffer = parents.new_empty(rows * (3 + words) + requests)
     positions, context_starts, slots, mask, lengths = buffer.split_with_sizes((rows, rows, rows, rows * words, requests))
     launch(
         _lib.load().mvb_build_draft_tree, device, "b200_paged draft tree",
@@ -181,7 +181,7 @@ def accept_draft_tree(
     committed = _vector("committed_lengths", committed_lengths, device)
     requests = committed.shape[0]
     starts = _vector("query_start_locations", query_start_locations, device, requests + 1)
-    buffer = torch.empty(requests * (2 * max_accepted + 3), dtype=torch.int64, device=device)
+    buffer = parents.new_empty(requests * (2 * max_accepted + 3))
     cells = requests * max_accepted
     nodes, tokens, count, lengths, last = buffer.split_with_sizes((cells, cells, requests, requests, requests))
     launch(

@@ -301,7 +301,7 @@ class B200PagedAttentionOperator(AttentionOperator):
         width = table.shape[1]
         if width > 1 and table.stride(1) != 1:
             table = table.contiguous()
-        output = torch.empty((num_tokens, num_q_heads, head_dim), dtype=query.dtype, device=device)
+        output = query.new_empty((num_tokens, num_q_heads, head_dim))
         nbytes = self._lib.mvb_tree_attention_workspace_size(num_tokens, num_requests, num_q_heads, num_kv_heads, head_dim)
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
         launch(
