@@ -460,7 +460,7 @@ int mvb_tree_attention(const void* query, int64_t query_token_stride, int64_t qu
   p.status = status;
   p.stream = static_cast<cudaStream_t>(stream);
   // 32 requests x 32 rows x 2.3K keys in fp16: 72 us with pages of 16 on the
-  // tcgen05 kernel, 416 us with pages of 48 on the other.
+  // tcgen05 kernel, 408 us with pages of 48 on the other.
   return tree_tc_supported(p) ? launch_tree_attention(p) : launch_tree_attention_generic(p);
 }
 

@@ -17,12 +17,12 @@
 // infinity are no sum, and what a row does not see must not reach it as 0 x NaN.
 //
 // Measured (B200, fp32, captured launches): 5 requests x 48 rows x up to 1.5K
-// keys 40 us, 64 x 32 x 1.5K keys 369 us and 200 x 128 x 1K keys 3.1 ms (34
-// TFLOP/s of useful products), 1 x 128 x 8K keys 131 us, 1 x 16 x 64 keys 15 us.
-// A tile takes two CTAs of an SM 18K cycles: a quarter q.k, a fifth P.V, the rest
+// keys 40 us, 64 x 32 x 1.5K keys 362 us and 200 x 128 x 1K keys 3.1 ms (34
+// TFLOP/s of useful products), 1 x 128 x 8K keys 129 us, 1 x 16 x 64 keys 15 us.
+// A tile takes two CTAs of an SM 17K cycles: a quarter q.k, a fifth P.V, the rest
 // softmax, copies and barriers; the tensor pipe is active for a third of it and
 // every second cycle issues, so that what bounds it are the latencies between
-// the four barriers of a tile, with 16 warps an SM to cover them.  K and V rows
+// the barriers of a tile, with 16 warps an SM to cover them.  K and V rows
 // by bulk copies of one warp instead of cp.async by all took 516 against 369 us
 // at 64 x 32 x 1.5K keys.  On the CUDA cores the same tiles are bound by shared
 // memory (12-18 TFLOP/s; two operand loads for 32 FMA instructions).
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
     };
     auto load = [&](int32_t j, const T* from, float* to, int stride) {
       if (j < j1) {
-#pragma unroll 4
+#pragma unroll
         for (int key = warp; key < kKeyTile; key += kThreads / 32) {
           const int64_t slot = slots_sh[j & 1][key];
           if constexpr (kVec) {
@@ -388,6 +388,16 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           s[n][i] += (big[0][n][i] + big[1][n][i]) + (big[2][n][i] + big[3][n][i]);
+      auto store_scores = [&]() {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<float2*>(s_sh + (r16 + fr + 8 * i) * kSStride + key16 + 8 * n + 2 * fc) =
+                make_float2(s[n][2 * i], s[n][2 * i + 1]);
+      };
+      store_scores();
+      put_slot(j + 1, next_block);
       // A score that is not finite: q or K is not (or their sum), and the
       // split product may have made NaN of an infinity.  Then plain sums.
       bool odd = false;
@@ -412,15 +422,9 @@ __global__ void __launch_bounds__(kThreads, NT <= 4 ? 2 : 1)
             }
             s[n][i] = dot;
           }
+        store_scores();
+        __syncthreads();
       }
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          *reinterpret_cast<float2*>(s_sh + (r16 + fr + 8 * i) * kSStride + key16 + 8 * n + 2 * fc) =
-              make_float2(s[n][2 * i], s[n][2 * i + 1]);
-      put_slot(j + 1, next_block);
-      __syncthreads();
       load(j + 1, keys, k_sh, kKStride);
 
       // Softmax of this warp's 4 rows, a lane at keys lane and lane + 32.

@@ -368,6 +368,69 @@ def test_attention_on_two_streams_and_in_two_graphs() -> None:
     assert torch.equal(results[0], want)
 
 
+@pytest.mark.parametrize("dtype, block_size", [(torch.float32, 16), (torch.float16, 48), (torch.bfloat16, 32)],
+                         ids=["fp32", "odd-pages", "bf16"])
+def test_attention_overlapped_and_replayed_on_other_trees(dtype, block_size) -> None:
+    """Calls on three streams at once, and one captured graph replayed on
+    lengths, parents and queries that the capture did not see."""
+
+    operator = B200PagedAttentionOperator()
+    make = lambda seed, committed: tree_batch([16, 40, 9], committed, q_heads=8, kv_heads=2, dtype=dtype, seed=seed,  # noqa: E731
+                                              block_size=block_size)
+    b = make(40, [900, 300, 70])
+    gpu = b.to(DEV)
+    tree = build(gpu)
+    want = operator.attend_tree(gpu.query, gpu.cache, tree)
+    check_attention(want, b, plain_build(b))
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(20):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(operator.attend_tree(gpu.query, gpu.cache, tree))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = operator.attend_tree(gpu.query, gpu.cache, build(gpu))
+    for seed, committed in ((41, [1, 299, 0]), (42, [900, 2, 70])):
+        other = make(seed, committed)
+        b.parents, b.committed, b.query = other.parents, other.committed, other.query
+        for name in ("parents", "committed", "query"):
+            getattr(gpu, name).copy_(getattr(b, name))
+        graph.replay()
+        check_attention(out, b, plain_build(b))
+
+
+@pytest.mark.parametrize("dtype, code", [(torch.float16, _lib.MVB_DTYPE_F16), (torch.float32, _lib.MVB_DTYPE_F32)],
+                         ids=["fp16", "fp32"])
+def test_attention_refuses_a_workspace_that_is_missing_or_too_small(dtype, code) -> None:
+    b = tree_batch([6, 9], [77, 30], dtype=dtype, seed=11)
+    gpu, lib = b.to(DEV), _lib.load()
+    tree = build(gpu)
+    md, out = tree.attention, torch.full_like(gpu.query, 3)
+    rows, q_heads, dim = gpu.query.shape
+    _, blocks, block_size, kv_heads, _ = gpu.cache.shape
+    need = lib.mvb_tree_attention_workspace_size(rows, 2, q_heads, kv_heads, dim)
+    room = torch.empty(need, dtype=torch.uint8, device=DEV)
+
+    def call(workspace, size):
+        return lib.mvb_tree_attention(
+            gpu.query.data_ptr(), gpu.query.stride(0), gpu.query.stride(1), out.data_ptr(), gpu.cache.data_ptr(),
+            blocks, block_size, kv_heads, dim, md.query_context_start_positions.data_ptr(), gpu.starts.data_ptr(),
+            md.context_lengths.data_ptr(), gpu.table.data_ptr(), gpu.table.stride(0), gpu.table.shape[1],
+            tree.ancestor_mask.data_ptr(), 1, rows, 2, q_heads, dim ** -0.5, code, workspace, size, None,
+            torch.cuda.current_stream().cuda_stream)
+
+    assert call(room.data_ptr(), 4096) == _lib.MVB_ERR_WORKSPACE_TOO_SMALL
+    assert call(None, need) == _lib.MVB_ERR_INVALID_ARGUMENT
+    assert call(room.data_ptr() + 16, need - 16) == _lib.MVB_ERR_INVALID_ARGUMENT
+    assert (out == 3).all()
+    assert call(room.data_ptr(), need) == _lib.MVB_OK
+    check_attention(out, b, plain_build(b))
+
+
 def test_attention_past_32_bit_offsets() -> None:
     """Pages whose element offset in the cache is past 2^31."""
 
