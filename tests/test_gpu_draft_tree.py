@@ -192,6 +192,33 @@ def test_attention_of_many_requests_of_mixed_length(dtype) -> None:
     check_attention(out, b, plain_build(b))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_attention_of_more_requests_than_threads(dtype) -> None:
+    gen = np.random.default_rng(9)
+    nodes, committed = gen.integers(0, 3, 1300).tolist(), gen.integers(0, 25, 1300).tolist()
+    nodes[:100] = [0] * 100  # no work where the first threads look
+    b = tree_batch(nodes, committed, q_heads=2, kv_heads=2, dtype=dtype, seed=23)
+    gpu = b.to(DEV)
+    out = B200PagedAttentionOperator().attend_tree(gpu.query, gpu.cache, build(gpu))
+    check_attention(out, b, plain_build(b))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32], ids=["fp16", "bf16", "fp32"])
+def test_queries_that_are_not_finite_spoil_their_rows_alone(dtype) -> None:
+    b = tree_batch([40, 7], [300, 90], q_heads=4, kv_heads=2, dtype=dtype, seed=24)
+    as_bits = torch.int32 if dtype == torch.float32 else torch.int16
+    b.query.view(as_bits)[3, 1, 5] = torch.iinfo(as_bits).max  # NaN with every bit of its payload
+    b.query[9, 2, 0] = torch.inf
+    b.query[44, 0, 127] = -torch.inf
+    gpu = b.to(DEV)
+    out = B200PagedAttentionOperator().attend_tree(gpu.query, gpu.cache, build(gpu))
+    for t, h in ((3, 1), (9, 2), (44, 0)):
+        assert torch.isnan(out[t, h]).all()
+        b.query[t, h], gpu.query[t, h] = 0, 0
+        out[t, h] = B200PagedAttentionOperator().attend_tree(gpu.query, gpu.cache, build(gpu))[t, h]
+    check_attention(out, b, plain_build(b))
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
 def test_attention_rows_that_see_nothing_or_have_no_owner_are_zero(dtype) -> None:
     b = tree_batch([4, 3, 2], [0, 20, 40], dtype=dtype, seed=5)
