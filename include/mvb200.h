@@ -423,8 +423,9 @@ MVB_API int mvb_build_draft_tree(const int64_t* parents, const int64_t* query_st
  * more nodes than mask bits, or a context shorter than their nodes, get 0.
  * scale is positive.  head_dim <= 256; fp16 and bf16 with head_dim 128, a GQA
  * ratio up to 64, pages of a power of two from 16 tokens on and 16-byte
- * aligned rows run on tcgen05 tiles (P rounded once to the dtype), everything
- * else, fp32 among it, on split-TF32 tiles with fp32 accuracy.  The workspace
+ * aligned rows run on tcgen05 tiles (P keeps 11 bits in fp16 and 16 in bf16, as
+ * in mvb_paged_attention), everything else, fp32 among it, on split-TF32 tiles
+ * with fp32 accuracy.  The workspace
  * (mvb_tree_attention_workspace_size, 256-byte aligned, no initialisation)
  * belongs to the call until it has run: calls that may overlap need one each.
  */

@@ -249,6 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int32_t q_issued;
 
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kParts = kBf16 ? 2 : 1;  // of P
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   allow_dependent_launch();  // the merge waits for this grid's end before it reads
 
@@ -696,17 +697,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint64_t dv = dv0 + (uint64_t)((stage * kTileBytes) >> 4);
           const uint32_t d_tmem = tmem + col_o(x), p_tmem = tmem + col_s(x);
           const int32_t k0 = d.kbase + (d.n - 1 - j) * kKeys;
+          auto step = [&](int k, int part, bool add) {
+            umma_f16_ts(d_tmem, p_tmem + 32 * (k >> 1) + 8 * (k & 1) + 16 * part,
+                        dv + (uint64_t)(k * (2 * kGroupBytes >> 4)), idesc_pv, add);
+          };
           if (k0 >= d.kv_lo && k0 + kKeys <= d.kv_hi) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              umma_f16_ts(d_tmem, p_tmem + 32 * (k >> 1) + 8 * (k & 1),
-                          dv + (uint64_t)(k * (2 * kGroupBytes >> 4)), idesc_pv, acc || k > 0);
+            for (int part = 0; part < kParts; ++part)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) step(k, part, acc || k > 0 || part > 0);
           } else {
             const int lo = max(d.kv_lo - k0, 0) >> 4, hi = (min(d.kv_hi - k0, kKeys) + 15) >> 4;
 #pragma unroll 1
             for (int k = lo; k < hi; ++k)
-              umma_f16_ts(d_tmem, p_tmem + 32 * (k >> 1) + 8 * (k & 1),
-                          dv + (uint64_t)(k * (2 * kGroupBytes >> 4)), idesc_pv, acc || k > lo);
+#pragma unroll
+              for (int part = 0; part < kParts; ++part) step(k, part, acc || k > lo || part > 0);
           }
           umma_commit(bar(kPvDone + x));
         };
@@ -1068,32 +1073,60 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           // P = 2^(s*scale - m), over S as packed 16-bit pairs (keys 32ch..+31
-          // in columns 32ch..+15), summed before it is rounded.  bf16 P is
-          // rounded once too: its half step of 2^-8 is that of the output,
-          // and keeping 16 bits of it (a second product) measured 378 -> 518
-          // us at 64 requests x 128 rows x 6K keys.
+          // in columns 32ch..+15), summed before it is rounded.  A bf16 P goes
+          // in two parts (the second in columns 32ch+16..+31) and two
+          // products, as in the paged kernels: its first 8 bits, cut off, and
+          // the rest rounded to 8 more.  2^-24 P on top keeps the rest above 0,
+          // so that an infinity of V times it is no NaN.  With one part 64 x 128
+          // rows x 4K keys take 199 us against 236, 3 x 244 rows x 48K 162
+          // against 212.  The two parts' loop is rolled and reads its scores
+          // from TMEM again, since code and registers count here: unrolled it
+          // takes 330 instead of 270 us at 256 x 16 rows x 1K keys.
           const float mu = m_ref == -INFINITY ? 0.f : m_ref;
           const uint64_t scale2 = f32x2_pack(p.scale_log2, p.scale_log2);
           const uint64_t negmu2 = f32x2_pack(-mu, -mu);
+          [[maybe_unused]] const uint64_t tiny2 = f32x2_pack(0x1p-24f, 0x1p-24f);
           uint64_t ps2[2] = {f32x2_pack(0.f, 0.f), f32x2_pack(0.f, 0.f)};
-#pragma unroll
+#pragma unroll(kBf16 ? 1 : 4)
           for (int ch = 0; ch < 4; ++ch) {
+            uint32_t again[32];
+            if constexpr (kBf16) {
+              __syncwarp();
+              tmem_ld32_raw(s_cols + 32 * ch, again);
+              tmem_wait_ld();
+              reg_fence(again);
+            }
+            auto score = [&](int k) -> float {
+              if constexpr (kBf16)
+                return __uint_as_float(again[k]);
+              else
+                return __uint_as_float(sc[ch][k]);
+            };
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
-              uint32_t pk[8];
+              uint32_t pk[8], rest[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 const int k = 16 * hh + 2 * e;
                 float xa, xb;
-                f32x2_unpack(f32x2_fma(f32x2_pack(__uint_as_float(sc[ch][k]),
-                                                  __uint_as_float(sc[ch][k + 1])),
-                                       scale2, negmu2),
-                             xa, xb);
+                f32x2_unpack(f32x2_fma(f32x2_pack(score(k), score(k + 1)), scale2, negmu2), xa, xb);
                 const float pa = ex2(xa), pb = ex2(xb);
-                ps2[e & 1] = f32x2_add(ps2[e & 1], f32x2_pack(pa, pb));
-                pk[e] = pack2<T>(pa, pb);
+                const uint64_t p2 = f32x2_pack(pa, pb);
+                ps2[e & 1] = f32x2_add(ps2[e & 1], p2);
+                if constexpr (kBf16) {
+                  const uint32_t ua = __float_as_uint(pa), ub = __float_as_uint(pb);
+                  pk[e] = __byte_perm(ua, ub, 0x7632);
+                  const uint64_t first2 = f32x2_pack(__uint_as_float(ua & 0xffff0000u),
+                                                     __uint_as_float(ub & 0xffff0000u));
+                  float ra, rb;
+                  f32x2_unpack(f32x2_fma(p2, tiny2, f32x2_sub(p2, first2)), ra, rb);
+                  rest[e] = pack2<T>(ra, rb);
+                } else {
+                  pk[e] = pack2<T>(pa, pb);
+                }
               }
               tmem_st8(s_cols + 32 * ch + 8 * hh, pk);
+              if constexpr (kBf16) tmem_st8(s_cols + 32 * ch + 16 + 8 * hh, rest);
             }
           }
           tmem_wait_st();
