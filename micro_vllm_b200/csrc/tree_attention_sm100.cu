@@ -98,6 +98,8 @@ static_assert(2 * 128 * kSoftmaxRegs + 128 * kEpiRegs + 128 * kOtherRegs <= kThr
 constexpr uint32_t kTmemCols = 512;
 __device__ __forceinline__ uint32_t col_s(int x) { return 128u * (uint32_t)x; }
 __device__ __forceinline__ uint32_t col_o(int x) { return 256u + 128u * (uint32_t)x; }
+// A row's reference moves to where its largest P is 2^kTop, once a P would pass
+// 2^(kTop + kRescaleLog2).
 constexpr float kRescaleLog2 = 8.f;
 
 // Cost axis: a KV tile of an item with one or two query tiles, an item's
@@ -1050,13 +1052,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], __uint_as_float(sc[e >> 5][e & 31]),
                                      __uint_as_float(sc[e >> 5][(e & 31) + 1]));
           const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-          // The reference moves only when a score exceeds it by 2^8: O / l is
-          // exact whatever it is, and P <= 2^8 stays well inside fp16 / bf16.
+          // O / l is exact whatever the reference is.  fp16 holds [2^-14, 2^16)
+          // in full: with P up to 2^15 a long tail of small weights comes
+          // through (a weight is off by 2^-32 of the row's largest at most).
+          // bf16 has fp32's exponents, and O less room for large values.
+          constexpr float kTop = kBf16 ? 0.f : 7.f;
           float corr = 1.f;
-          if (tmax > m_ref + kRescaleLog2) {
-            corr = ex2(m_ref - tmax);  // 0 when m_ref is -inf
+          if (tmax > m_ref + (kTop + kRescaleLog2)) {
+            const float m_new = tmax - kTop;
+            corr = ex2(m_ref - m_new);  // 0 when m_ref is -inf
             l *= corr;
-            m_ref = tmax;
+            m_ref = m_new;
           }
           // O holds P.V of the stream's tile before, complete because this S
           // (issued behind it) is.

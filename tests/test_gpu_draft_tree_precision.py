@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import oracle.draft_tree as plain
-from _draft_trees import attention_tolerance, tree_batch
+from _draft_trees import TreeBatch, attention_tolerance, tree_batch
 from micro_vllm_b200 import B200PagedAttentionOperator, FullAttentionSpec, build_draft_tree
 
 pytestmark = pytest.mark.gpu
@@ -40,4 +40,38 @@ def test_bf16_weights_keep_sixteen_bits(nodes, committed, q_heads, kv_heads) -> 
     rounded = torch.finfo(torch.bfloat16).eps / 2
     sums = attention_tolerance(size, reach, exact, torch.float32, keys, 128, 0.0)
     allowed = rounded * np.abs(exact) + (1 + rounded) * (sums + (2.0 ** -16 + 2.0 ** -23) * size)
+    assert (np.abs(got - exact) <= allowed).all(), (np.abs(got - exact) / allowed).max()
+
+
+@pytest.mark.parametrize("nodes, q_heads", [(1, 8), (20, 8), (80, 4)])
+@pytest.mark.parametrize("bits", [15.5, 21.5, 25.5])
+def test_fp16_keeps_the_weights_of_a_long_tail(nodes, q_heads, bits) -> None:
+    """Each node's own key outweighs every committed one by 2^bits, and only
+    those have a value: what they add up to comes through.  The path scales
+    weights so that a row's largest is at least 2^7; below 2^-14 an fp16
+    number is off by at most 2^-25, so a weight by 2^-32 of the largest.
+    A score is a product of few terms, exact up to its rounding to fp32.  320
+    requests over the same pages: items stay whole, long runs of tiles."""
+
+    keys, requests = 4000, 320
+    b = tree_batch([nodes], [keys], q_heads=q_heads, kv_heads=1, seed=32, shape="star")
+    b.cache.zero_()
+    b.query.zero_()
+    flat = b.cache.view(2, -1, 1, 128)
+    at = lambda p: int(b.table[0, p // 16] * 16 + p % 16)  # noqa: E731
+    rise = bits * np.log(2) * 128 ** 0.5 / 16
+    for p in range(keys):
+        flat[1, at(p)] = 1 + p % 2
+    for i in range(nodes):
+        flat[0, at(keys + i), 0, i] = 16
+        b.query[i, :, i] = rise
+    _, exact, size, _, _ = attend(b, 2)
+    many = TreeBatch(b.parents.repeat(requests), torch.arange(requests + 1) * nodes, b.committed.repeat(requests),
+                     b.table.repeat(requests, 1), b.cache, b.query.repeat(requests, 1, 1), 16).to(DEV)
+    tree = build_draft_tree(many.parents, many.starts, many.committed, many.table, 16, max_nodes=128)
+    out = B200PagedAttentionOperator().attend_tree(many.query, many.cache, tree)
+    got = out.float().cpu().numpy().astype(np.float64).reshape(requests, *exact.shape)
+    # Scores: rise in fp16 times 16, scaled in fp32 and cut in ex2 at 2^-20.
+    allowed = 2.0 ** -11 * np.abs(exact) + (2.0 ** -11 + 2 * keys * 2.0 ** -23 + 2.0 ** -18) * size
+    allowed += 2.0 ** -25 + keys * 2.0 ** -32 * 2
     assert (np.abs(got - exact) <= allowed).all(), (np.abs(got - exact) / allowed).max()
