@@ -241,13 +241,17 @@ class B200PagedAttentionOperator(AttentionOperator):
             raise ValueError("key/value must be [num_tokens, num_kv_heads, head_dim]")
         if key.device != query.device or value.device != query.device:
             raise ValueError("query, key, value and layer_kv_cache must be on one device")
-        self._check_tree(query, layer_kv_cache, tree)
+        checked = self._check_tree(query, layer_kv_cache, tree)
+        slots = tree.attention.slot_mapping
+        if slots.dtype is not torch.int64 or slots.numel() != query.shape[0] or slots.device != query.device:
+            raise ValueError("metadata.slot_mapping must be torch.int64 [num_tokens] on the query's device")
         with torch.cuda.device(query.device):
             write_kv_cache(key, value, layer_kv_cache, tree.attention)
-        return self.attend_tree(query, layer_kv_cache, tree)
+        return self._attend_tree(query, layer_kv_cache, checked)
 
-    def _check_tree(self, query, layer_kv_cache, tree) -> int:
-        """Checks that the cache and the tree fit the query; the MVB_DTYPE_*."""
+    def _check_tree(self, query, layer_kv_cache, tree):
+        """Refuses a cache or a tree that does not fit the query, before
+        anything is written; the MVB_DTYPE_* and the metadata for the launch."""
 
         if not query.is_cuda or not layer_kv_cache.is_cuda:
             raise RuntimeError("b200_paged attention requires CUDA tensors")
@@ -260,8 +264,10 @@ class B200PagedAttentionOperator(AttentionOperator):
         planes, _, block_size, num_kv_heads, head_dim = layer_kv_cache.shape
         if planes != 2 or head_dim != query_dim or block_size != tree.attention.block_size:
             raise ValueError("layer_kv_cache does not match the query / metadata")
-        if num_kv_heads == 0 or num_q_heads % num_kv_heads != 0:
+        if num_kv_heads == 0 or num_q_heads == 0 or num_q_heads % num_kv_heads != 0:
             raise ValueError("num_q_heads must be a multiple of num_kv_heads")
+        if not 1 <= head_dim <= 256:
+            raise ValueError("head_dim must be 1 .. 256")
         index = query.get_device()
         if layer_kv_cache.get_device() != index:
             raise ValueError("query and layer_kv_cache must be on one device")
@@ -269,7 +275,19 @@ class B200PagedAttentionOperator(AttentionOperator):
         if mask.dtype is not torch.int64 or mask.dim() != 2 or mask.shape[0] != num_tokens \
                 or not 1 <= mask.shape[1] <= _lib.MVB_MAX_TREE_NODES // 64 or mask.get_device() != index:
             raise ValueError("ancestor_mask must be torch.int64 [num_tokens, words] on the query's device")
-        return dtype
+        md, device = tree.attention, query.device
+        md_start = _meta(md.query_context_start_positions, device, "query_context_start_positions")
+        md_qsl = _meta(md.query_start_locations, device, "query_start_locations")
+        md_ctx = _meta(md.context_lengths, device, "context_lengths")
+        table, num_requests = md.block_table, md_ctx.numel()
+        if table.dtype is not torch.int64 or table.get_device() != index or table.dim() != 2 \
+                or table.shape[0] != num_requests:
+            raise ValueError("metadata.block_table must be torch.int64 [num_requests, width] on the query's device")
+        if md_start.numel() != num_tokens or md_qsl.numel() != num_requests + 1:
+            raise ValueError("metadata does not match the query")
+        if table.shape[1] > 1 and table.stride(1) != 1:
+            table = table.contiguous()
+        return dtype, md_start, md_qsl, md_ctx, table, mask if mask.is_contiguous() else mask.contiguous()
 
     def attend_tree(self, query, layer_kv_cache, tree) -> torch.Tensor:
         """Attention of draft trees (``build_draft_tree``) over a cache that
@@ -279,28 +297,15 @@ class B200PagedAttentionOperator(AttentionOperator):
         allocator, so calls on several streams, and several captured graphs,
         have one each."""
 
-        dtype = self._check_tree(query, layer_kv_cache, tree)
+        return self._attend_tree(query, layer_kv_cache, self._check_tree(query, layer_kv_cache, tree))
+
+    def _attend_tree(self, query, layer_kv_cache, checked) -> torch.Tensor:
+        dtype, md_start, md_qsl, md_ctx, table, mask = checked
         num_tokens, num_q_heads, head_dim = query.shape
         _, num_blocks, block_size, num_kv_heads, _ = layer_kv_cache.shape
-        device = query.device
+        device, num_requests = query.device, md_ctx.numel()
         if query.stride(2) != 1:
             query = query.contiguous()
-        md, mask = tree.attention, tree.ancestor_mask
-        if not mask.is_contiguous():
-            mask = mask.contiguous()
-        md_start = _meta(md.query_context_start_positions, device, "query_context_start_positions")
-        md_qsl = _meta(md.query_start_locations, device, "query_start_locations")
-        md_ctx = _meta(md.context_lengths, device, "context_lengths")
-        table = md.block_table
-        num_requests = md_ctx.numel()
-        if table.dtype is not torch.int64 or table.get_device() != device.index or table.dim() != 2 \
-                or table.shape[0] != num_requests:
-            raise ValueError("metadata.block_table must be torch.int64 [num_requests, width] on the query's device")
-        if md_start.numel() != num_tokens or md_qsl.numel() != num_requests + 1:
-            raise ValueError("metadata does not match the query")
-        width = table.shape[1]
-        if width > 1 and table.stride(1) != 1:
-            table = table.contiguous()
         output = query.new_empty((num_tokens, num_q_heads, head_dim))
         nbytes = self._lib.mvb_tree_attention_workspace_size(num_tokens, num_requests, num_q_heads, num_kv_heads, head_dim)
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
@@ -309,7 +314,7 @@ class B200PagedAttentionOperator(AttentionOperator):
             query.data_ptr(), query.stride(0), query.stride(1), output.data_ptr(),
             layer_kv_cache.data_ptr(), num_blocks, block_size, num_kv_heads, head_dim,
             md_start.data_ptr(), md_qsl.data_ptr(), md_ctx.data_ptr(),
-            table.data_ptr(), table.stride(0), width, mask.data_ptr(), mask.shape[1],
+            table.data_ptr(), table.stride(0), table.shape[1], mask.data_ptr(), mask.shape[1],
             num_tokens, num_requests, num_q_heads, 1.0 / math.sqrt(head_dim), dtype,
             workspace.data_ptr(), nbytes, self._state(device).status.data_ptr(),
         )

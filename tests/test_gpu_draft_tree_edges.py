@@ -1,0 +1,90 @@
+"""Draft trees where one mechanism meets another: values that are not finite
+in items of many tiles, first calls inside a capture, windows with missing
+pages, far offsets, the layer's prologue, several cache groups."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import oracle.draft_tree as plain
+from _draft_trees import attention_tolerance, tree_batch
+from micro_vllm_b200 import (
+    B200PagedAttentionOperator,
+    ChunkedLocalSpec,
+    DraftTree,
+    AttentionMetadata,
+    FullAttentionSpec,
+    SlidingWindowSpec,
+    _lib,
+    build_draft_tree,
+)
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+FULL = FullAttentionSpec()
+DTYPES = pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32], ids=["fp16", "bf16", "fp32"])
+
+
+def build(b, spec=FULL, max_nodes=64):
+    return build_draft_tree(b.parents, b.starts, b.committed, b.table, b.block_size, spec=spec, max_nodes=max_nodes)
+
+
+def plain_build(b, spec=FULL, words=1):
+    return plain.build_draft_tree(b.parents.numpy(), b.starts.numpy(), b.committed.numpy(), b.table.numpy(),
+                                  b.block_size, spec.context_start, words)
+
+
+def check(out, b, meta, *, only=slice(None)) -> None:
+    """``out`` against the 64-bit loops, infinities and NaN among it."""
+
+    _, begin, lengths, _, mask = meta
+    dim, values = b.query.shape[2], b.cache.float().numpy()
+    with np.errstate(all="ignore"):
+        exact, size, reach = plain.tree_attention(b.query.float().numpy(), values, begin, b.starts.numpy(), lengths,
+                                                  b.table.numpy(), mask, dim ** -0.5)
+    finite = np.abs(np.nan_to_num(values[1], nan=0.0, posinf=0.0, neginf=0.0)).max()
+    allowed = attention_tolerance(size, reach, exact, out.dtype, int(max(lengths)), dim, float(finite))[only]
+    got, exact = out.float().cpu().numpy().astype(np.float64)[only], exact[only]
+    np.testing.assert_array_equal(np.isnan(got), np.isnan(exact))
+    odd = ~np.isfinite(exact)
+    np.testing.assert_array_equal(got[odd], exact[odd])
+    assert np.isfinite(got[~odd]).all()
+    assert (np.abs(got[~odd] - exact[~odd]) <= allowed[~odd]).all()
+
+
+def spoil(b, r: int, position: int, value: float, *, plane=1, column=slice(None), head=slice(None)) -> None:
+    page = int(b.table[r, position // b.block_size])
+    b.cache[plane, page, position % b.block_size, head, column] = value
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
+def test_forward_tree_refuses_before_it_writes(dtype) -> None:
+    b = tree_batch([6, 9], [77, 30], dtype=dtype, seed=56)
+    gpu, operator = b.to(DEV), B200PagedAttentionOperator()
+    tree = build(gpu)
+    md, rows = tree.attention, b.query.shape[0]
+    key = torch.ones(rows, 2, 128, dtype=dtype, device=DEV)
+
+    def refused(match, *, mask=tree.ancestor_mask, query=gpu.query, key=key, **fields):
+        other = AttentionMetadata(**{**{f: getattr(md, f) for f in md.__dataclass_fields__}, **fields})
+        with pytest.raises(ValueError, match=match):
+            operator.forward_tree(query, key, key, gpu.cache, DraftTree(other, mask))
+
+    for slots in (md.slot_mapping[:-1], torch.cat([md.slot_mapping, md.slot_mapping]), md.slot_mapping.int(),
+                  md.slot_mapping.cpu(), md.slot_mapping[:0]):
+        refused("slot_mapping", slot_mapping=slots)
+    refused("block_table", block_table=md.block_table[:1])
+    refused("match the query", query_start_locations=md.query_start_locations[:-1])
+    refused("match the query", query_context_start_positions=md.query_context_start_positions[1:])
+    refused("context_lengths", context_lengths=md.context_lengths.int())
+    refused("ancestor_mask", mask=tree.ancestor_mask[1:])
+    refused("key/value", key=key[1:])
+    refused("multiple", query=gpu.query[:, :0])
+    assert torch.equal(gpu.cache.cpu(), b.cache)
+    wide = torch.zeros(2, 4, 16, 2, 264, dtype=dtype, device=DEV)
+    with pytest.raises(ValueError, match="head_dim"):
+        operator.attend_tree(wide.new_zeros(rows, 4, 264), wide, tree)
+    with pytest.raises(ValueError, match="head_dim"):
+        operator.attend_tree(gpu.query[..., :0], wide[..., :0].contiguous(), tree)
