@@ -64,13 +64,27 @@ class B200PagedAttentionOperator(AttentionOperator):
     def __init__(self) -> None:
         self._lib = _lib.load()
         self._devices: dict[int, _DeviceState] = {}
+        # The status word of the device in use, ahead of a first call that is captured.
+        if torch.cuda.is_initialized() and not torch.cuda.is_current_stream_capturing():
+            self._state(torch.device("cuda"))
 
     # -- workspace -------------------------------------------------------
     def _state(self, device: torch.device) -> _DeviceState:
         idx = device.index if device.index is not None else torch.cuda.current_device()
         st = self._devices.get(idx)
         if st is None:
-            st = self._devices[idx] = _DeviceState(torch.device("cuda", idx))
+            device = torch.device("cuda", idx)
+            with torch.cuda.device(device):
+                # A captured zero-fill would run with every replay, and clear
+                # what other calls set.
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError(
+                        f"b200_paged has no status word on {device} yet: call reserve(), or attention once, before "
+                        "a CUDA-graph capture"
+                    )
+                st = _DeviceState(device)
+                torch.cuda.current_stream().synchronize()  # the word is 0 for every stream
+            st = self._devices.setdefault(idx, st)
         return st
 
     def reserve(

@@ -60,6 +60,36 @@ def spoil(b, r: int, position: int, value: float, *, plane=1, column=slice(None)
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
+def test_a_status_word_keeps_its_bits_over_captured_calls(dtype) -> None:
+    """An operator whose first call is captured: nothing is set before the
+    graph runs, and a replay or a call that is clean clears nothing."""
+
+    b = tree_batch([7, 5], [200, 64], dtype=dtype, seed=55)
+    gpu, operator = b.to(DEV), B200PagedAttentionOperator()
+    tree = build(gpu)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = operator.attend_tree(gpu.query, gpu.cache, tree)
+    assert operator.read_status(DEV) == 0
+    whole = gpu.table.clone()
+    gpu.table[0, 3] = -1
+    graph.replay()
+    gpu.table.copy_(whole)
+    graph.replay()
+    operator.attend_tree(gpu.query, gpu.cache, tree)
+    assert operator.read_status(DEV) == _lib.MVB_STATUS_BLOCK_OUT_OF_RANGE
+    assert operator.read_status(DEV) == 0
+    check(out, b, plain_build(b))
+    late = B200PagedAttentionOperator()
+    late._devices.clear()  # as one made before CUDA is in use, or for another device
+    with pytest.raises(RuntimeError, match="no status word"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            late.attend_tree(gpu.query, gpu.cache, tree)
+    assert not late._devices
+    assert late.read_status(DEV) == 0 and torch.equal(late.attend_tree(gpu.query, gpu.cache, tree), out)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
 def test_forward_tree_refuses_before_it_writes(dtype) -> None:
     b = tree_batch([6, 9], [77, 30], dtype=dtype, seed=56)
     gpu, operator = b.to(DEV), B200PagedAttentionOperator()
