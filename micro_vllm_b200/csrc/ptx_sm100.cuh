@@ -79,6 +79,25 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int lim
   return false;
 }
 
+// Of `issued` loads into a ring of `stages`, those from the result on may be in
+// flight, in any order; the ones before have landed, since their stages were
+// taken again.
+__host__ __device__ constexpr int32_t first_in_flight(int32_t issued, int32_t stages) {
+  return issued > stages ? issued - stages : 0;
+}
+constexpr bool drain_reaches_every_stage(int32_t stages) {
+  for (int32_t issued = 0; issued < 4 * stages; ++issued) {
+    int32_t last[8] = {-1, -1, -1, -1, -1, -1, -1, -1}, waited = 0;
+    for (int32_t c = 0; c < issued; ++c) last[c % stages] = c;
+    for (int32_t c = first_in_flight(issued, stages); c < issued; ++c) {
+      if (last[c % stages] != c) return false;  // its barrier is in a later phase
+      ++waited;
+    }
+    if (waited != (issued < stages ? issued : stages)) return false;
+  }
+  return true;
+}
+
 // ---------------------------------------------------------------- TMA
 // Brings a kernel argument's tensor map into the descriptor cache.
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {

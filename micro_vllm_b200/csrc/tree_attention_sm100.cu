@@ -111,6 +111,10 @@ constexpr int kTileCost1 = 4, kTileCost2 = 6, kItemCost = 20, kMinShare = 8;
 static_assert(kMinShare >= kTileCost1 && kMinShare >= kTileCost2,
               "a share between an item's first and last holds a tile of it");
 
+static_assert(drain_reaches_every_stage(kKStages) && drain_reaches_every_stage(kVStages) &&
+                  drain_reaches_every_stage(kQStages),
+              "an aborted CTA waits for every load it has in flight");
+
 constexpr int kPartRows = 2 * kRows;  // rows of one partial
 
 enum Bar : int {
@@ -247,8 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int32_t bad_v_sh[kFlagSlots];
   __shared__ uint32_t tmem_base_sh;
   __shared__ int32_t abort_sh;
-  __shared__ int32_t last_issued[2];
-  __shared__ int32_t q_issued;
+  __shared__ int32_t k_issued, v_issued, q_issued;  // TMA loads of tiles
 
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int kParts = kBf16 ? 2 : 1;  // of P
@@ -317,8 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init_fence();
     abort_sh = 0;
-    last_issued[0] = last_issued[1] = -1;
-    q_issued = 0;
+    k_issued = v_issued = q_issued = 0;
   }
   if (warp == kMmaWarp) tmem_alloc(smem_addr(&tmem_base_sh), kTmemCols);
   tc_fence_before();
@@ -934,7 +936,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
               }
               if (lane == 0) {
-                last_issued[is_k ? 0 : 1] = (int32_t)c;
+                (is_k ? k_issued : v_issued) = (int32_t)c + 1;
                 mbar_expect_tx(full, kTileBytes);
               }
               __syncwarp();
@@ -1172,16 +1174,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (abort_sh && tid == 0) {
     if (p.status != nullptr) atomicOr(p.status, kStatusWaitTimeout);
-    if (last_issued[0] >= 0) {
-      const uint32_t c = (uint32_t)last_issued[0];
-      bar_wait(bar(kKFull + kslot(c)), kphase(c));
-    }
-    if (last_issued[1] >= 0) {
-      const uint32_t c = (uint32_t)last_issued[1];
-      bar_wait(bar(kVFull + vslot(c)), vphase(c));
-    }
 #pragma unroll 1
-    for (int32_t c = max(q_issued - kQStages, 0); c < q_issued; ++c)
+    for (int32_t c = first_in_flight(k_issued, kKStages); c < k_issued; ++c)
+      bar_wait(bar(kKFull + kslot((uint32_t)c)), kphase((uint32_t)c));
+#pragma unroll 1
+    for (int32_t c = first_in_flight(v_issued, kVStages); c < v_issued; ++c)
+      bar_wait(bar(kVFull + vslot((uint32_t)c)), vphase((uint32_t)c));
+#pragma unroll 1
+    for (int32_t c = first_in_flight(q_issued, kQStages); c < q_issued; ++c)
       bar_wait(bar(kQFull + c % kQStages), (c / kQStages) & 1);
   }
   tc_fence_before();
