@@ -118,6 +118,8 @@ enum Bar : int {
   kFinal = kItemEmpty + kItemSlots,     // last MMA commit before TMEM is released
   kNumBars = kFinal + 1,
 };
+static_assert(drain_reaches_every_stage(kKStages) && drain_reaches_every_stage(kVStages),
+              "an aborted CTA waits for every load it has in flight");
 static_assert(kNumBars == 4 + 2 * kKStages + 3 * kVStages + 4 * 2 + 2 * kItemSlots + 1,
               "mbarrier layout");
 
@@ -192,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t tmem_base_sh;
   __shared__ int32_t first_claim;
   __shared__ int32_t abort_sh;
-  __shared__ int32_t last_issued[2];  // last K and last V tile index issued
+  __shared__ int32_t kv_issued[2];  // K and V tiles issued
   __shared__ int32_t q_issued[2];     // Q loads issued per tile (phases of kQFull)
 
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -241,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(bar(kFinal), 1);
     mbar_init_fence();
     abort_sh = 0;
-    last_issued[0] = last_issued[1] = -1;
+    kv_issued[0] = kv_issued[1] = 0;
     q_issued[0] = q_issued[1] = 0;
   }
   if (warp == kMmaWarp) tmem_alloc(smem_addr(&tmem_base_sh), kTmemCols);
@@ -526,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             int64_t blk = -1;
             if (lane < 8) blk = page_of(p, trow, pos);
             if (lane == 0) {
-              last_issued[is_k ? 0 : 1] = (int32_t)c;
+              kv_issued[is_k ? 0 : 1] = (int32_t)c + 1;
               mbar_expect_tx(full, kTileBytes);
             }
             __syncwarp();
@@ -831,7 +833,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // Everything this CTA issued lands before TMEM and shared memory go away
   // (each wait bounded): the MMA thread waits on a final commit; after an
-  // abort, the producers also wait for their last TMA loads.
+  // abort, for every TMA load that may be in flight too.
   if (warp == kMmaWarp && lane == 0) {
     umma_commit(bar(kFinal));
     mbar_wait(bar(kFinal), 0);
@@ -839,15 +841,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (abort_sh && tid == 0) {
     if (p.status != nullptr) atomicOr(p.status, kStatusWaitTimeout);
-    // The last K and V loads issued complete after every earlier one.
-    if (last_issued[0] >= 0) {
-      const uint32_t c = (uint32_t)last_issued[0];
-      mbar_wait(bar(kKFull + kslot(c)), kphase(c));
-    }
-    if (last_issued[1] >= 0) {
-      const uint32_t c = (uint32_t)last_issued[1];
-      mbar_wait(bar(kVFull + vslot(c)), vphase(c));
-    }
+#pragma unroll 1
+    for (int32_t c = first_in_flight(kv_issued[0], kKStages); c < kv_issued[0]; ++c)
+      mbar_wait(bar(kKFull + kslot((uint32_t)c)), kphase((uint32_t)c));
+#pragma unroll 1
+    for (int32_t c = first_in_flight(kv_issued[1], kVStages); c < kv_issued[1]; ++c)
+      mbar_wait(bar(kVFull + vslot((uint32_t)c)), vphase((uint32_t)c));
     for (int t = 0; t < 2; ++t)
       if (q_issued[t] > 0) mbar_wait(bar(kQFull + t), (q_issued[t] - 1) & 1);
   }
