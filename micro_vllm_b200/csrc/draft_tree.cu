@@ -12,6 +12,8 @@ namespace mvb {
 namespace {
 
 constexpr int kTreeThreads = 128;
+// Block ids from here on are no pages (their slots could wrap to a real one).
+constexpr int64_t kMaxBlockId = (int64_t)1 << 32;
 
 __device__ __forceinline__ int64_t tree_context_start(int64_t pos, int32_t kind, int64_t param) {
   if (kind == MVB_SPEC_SLIDING_WINDOW) return max(pos - param + 1, (int64_t)0);
@@ -78,7 +80,7 @@ __global__ void __launch_bounds__(kTreeThreads) build_draft_tree_kernel(const Dr
     int64_t slot = -1;
     if (page < a.table_width) {
       const int64_t blk = a.block_table[r * a.table_stride + page];
-      if (blk >= 0) slot = blk * a.block_size + logical % a.block_size;
+      if (blk >= 0 && blk < kMaxBlockId) slot = blk * a.block_size + logical % a.block_size;
     } else if (a.status) {
       atomicOr(a.status, MVB_STATUS_POSITION_PAST_TABLE);
     }

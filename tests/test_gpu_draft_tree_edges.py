@@ -59,6 +59,19 @@ def spoil(b, r: int, position: int, value: float, *, plane=1, column=slice(None)
     b.cache[plane, page, position % b.block_size, head, column] = value
 
 
+def test_slots_of_pages_that_cannot_be_do_not_wrap() -> None:
+    """16 times 2^60 is 0 in 64 bits: a node on such a page has no slot."""
+
+    b = tree_batch([3, 2], [14, 30], q_heads=1, kv_heads=1, dim=8)
+    b.table[0, 1], b.table[1, 1] = 1 << 60, (1 << 63) - 1
+    gpu = b.to(DEV)
+    slots = build(gpu).attention.slot_mapping.tolist()
+    want = plain_build(b)[3].tolist()
+    assert slots == [want[0], want[1], -1, -1, -1]
+    gpu.table[1, 1] = (1 << 32) - 1
+    assert build(gpu).attention.slot_mapping.tolist()[3] == ((1 << 32) - 1) * 16 + 14
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
 def test_a_status_word_keeps_its_bits_over_captured_calls(dtype) -> None:
     """An operator whose first call is captured: nothing is set before the
