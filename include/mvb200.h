@@ -443,6 +443,16 @@ MVB_API int mvb_tree_attention(const void* query, int64_t query_token_stride,
                                int64_t num_tokens, int64_t num_requests, int32_t num_q_heads,
                                float scale, int32_t dtype, void* workspace, size_t workspace_bytes,
                                int32_t* status, void* stream);
+/* Which kernel mvb_tree_attention runs for these arguments on the current
+ * device: 1 the tcgen05 tiles, 0 the split-TF32 ones (or a refusal).  Reads no
+ * device memory. */
+MVB_API int mvb_tree_attention_uses_tcgen05(const void* query, int64_t query_token_stride,
+                                            int64_t query_head_stride, const void* output,
+                                            const void* kv_cache, int64_t num_blocks,
+                                            int32_t block_size, int32_t num_kv_heads,
+                                            int32_t head_dim, int64_t num_tokens,
+                                            int64_t num_requests, int32_t num_q_heads,
+                                            int32_t dtype);
 
 /*
  * The path of each draft tree that the target model keeps.

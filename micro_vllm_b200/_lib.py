@@ -130,6 +130,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _P, _SZ, _P, _P,  # workspace, bytes, status, stream
         ],
     ),
+    "mvb_tree_attention_uses_tcgen05": (
+        ctypes.c_int,
+        [_P, _I64, _I64, _P, _P, _I64, _I32, _I32, _I32, _I64, _I64, _I32, _I32],
+    ),
     "mvb_accept_draft_tree": (
         ctypes.c_int,
         [_P, _P, _P, _P, _P, _I64, _I64, _I32, _P, _P, _P, _P, _P, _P, _P],

@@ -464,6 +464,31 @@ int mvb_tree_attention(const void* query, int64_t query_token_stride, int64_t qu
   return tree_tc_supported(p) ? launch_tree_attention(p) : launch_tree_attention_generic(p);
 }
 
+int mvb_tree_attention_uses_tcgen05(const void* query, int64_t query_token_stride,
+                                    int64_t query_head_stride, const void* output,
+                                    const void* kv_cache, int64_t num_blocks, int32_t block_size,
+                                    int32_t num_kv_heads, int32_t head_dim, int64_t num_tokens,
+                                    int64_t num_requests, int32_t num_q_heads, int32_t dtype) {
+  if (elem_bytes_of(dtype) == 0 || num_blocks <= 0 || block_size <= 0 || num_kv_heads <= 0 ||
+      num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 || num_tokens <= 0 || num_requests < 0)
+    return 0;
+  TreeProblem p{};
+  p.query = query;
+  p.q_st = query_token_stride;
+  p.q_sh = query_head_stride;
+  p.out = const_cast<void*>(output);
+  p.cache = kv_cache;
+  p.num_blocks = num_blocks;
+  p.block_size = block_size;
+  p.num_kv_heads = num_kv_heads;
+  p.head_dim = head_dim;
+  p.num_tokens = num_tokens;
+  p.num_requests = num_requests;
+  p.num_q_heads = num_q_heads;
+  p.dtype = dtype;
+  return tree_tc_supported(p) ? 1 : 0;
+}
+
 int mvb_accept_draft_tree(const int64_t* draft_tokens, const int64_t* target_tokens,
                           const int64_t* parents, const int64_t* query_start_locations,
                           const int64_t* committed_lengths, int64_t num_tokens,

@@ -129,6 +129,15 @@ def test_c_entries_refuse_before_touching_the_device(lib) -> None:
     assert move(caches=(ctypes.c_void_p * 2)(256, None)) == move(caches=(ctypes.c_void_p * 2)(256, 257)) == bad
 
 
+def test_the_path_query_takes_any_arguments(lib) -> None:
+    def path(bs=16, hkv=2, d=128, rows=4, requests=1, hq=4, dt=0, blocks=4, q=FAKE):
+        return lib.mvb_tree_attention_uses_tcgen05(q, 512, 128, FAKE, FAKE, blocks, bs, hkv, d, rows, requests, hq, dt)
+
+    assert path(bs=0) == path(hkv=0) == path(hq=0) == path(hq=3) == path(d=0) == path(rows=0) == path(rows=-1) == 0
+    assert path(requests=-1) == path(blocks=0) == path(dt=2) == path(dt=7) == path(bs=48) == path(hq=130) == 0
+    assert path(q=ctypes.c_void_p(264)) == path(blocks=1 << 30) == 0
+
+
 def test_entry_points_refuse_cpu_tensors() -> None:
     b = tree_batch([3, 2], [4, 5])
     with pytest.raises(RuntimeError, match="require CUDA tensors"):

@@ -59,14 +59,45 @@ def spoil(b, r: int, position: int, value: float, *, plane=1, column=slice(None)
     b.cache[plane, page, position % b.block_size, head, column] = value
 
 
+def on_tensor_tiles(query, out, cache) -> int:
+    rows, q_heads, dim = query.shape
+    _, blocks, block_size, kv_heads, _ = cache.shape
+    code = {torch.float16: _lib.MVB_DTYPE_F16, torch.bfloat16: _lib.MVB_DTYPE_BF16, torch.float32: _lib.MVB_DTYPE_F32}
+    return _lib.load().mvb_tree_attention_uses_tcgen05(
+        query.data_ptr(), query.stride(0), query.stride(1), out.data_ptr(), cache.data_ptr(), blocks, block_size,
+        kv_heads, dim, rows, 4, q_heads, code[query.dtype])
+
+
+@DTYPES
+def test_which_kernel_runs(dtype) -> None:
+    """The 16-bit tests of the tensor tiles run on them: a build whose
+    register count does not fit the kernel's split would fail here."""
+
+    def path(q_heads=16, kv_heads=8, dim=128, block_size=16, rows=24, cut=0):
+        query = torch.zeros(rows * (q_heads * dim + cut) + cut, dtype=dtype, device=DEV)
+        query = query[cut:].view(rows, -1)[:, :q_heads * dim].view(rows, q_heads, dim)
+        cache = torch.zeros(2, 5, block_size, kv_heads, dim, dtype=dtype, device=DEV)
+        return on_tensor_tiles(query, torch.empty_like(query), cache)
+
+    tiles = int(dtype != torch.float32)
+    for block_size in (16, 32, 64, 128, 256, 512):
+        assert path(block_size=block_size) == tiles
+    for q_heads, kv_heads in ((1, 1), (8, 8), (6, 2), (10, 2), (32, 8), (64, 1)):
+        assert path(q_heads, kv_heads) == path(q_heads, kv_heads, rows=1) == tiles
+    assert path(cut=8) == tiles
+    # Just outside: pages of no power of two or below 16, wider groups, other
+    # head sizes, rows that are not 16-byte aligned.
+    assert path(block_size=48) == path(block_size=8) == path(130, 2) == path(dim=64) == path(dim=136) == path(cut=4) == 0
+
+
 def test_slots_of_pages_that_cannot_be_do_not_wrap() -> None:
     """16 times 2^60 is 0 in 64 bits: a node on such a page has no slot."""
 
     b = tree_batch([3, 2], [14, 30], q_heads=1, kv_heads=1, dim=8)
+    want = plain_build(b)[3].tolist()
     b.table[0, 1], b.table[1, 1] = 1 << 60, (1 << 63) - 1
     gpu = b.to(DEV)
     slots = build(gpu).attention.slot_mapping.tolist()
-    want = plain_build(b)[3].tolist()
     assert slots == [want[0], want[1], -1, -1, -1]
     gpu.table[1, 1] = (1 << 32) - 1
     assert build(gpu).attention.slot_mapping.tolist()[3] == ((1 << 32) - 1) * 16 + 14
