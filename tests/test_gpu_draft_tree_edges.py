@@ -10,16 +10,22 @@ import torch
 
 import oracle.draft_tree as plain
 from _draft_trees import attention_tolerance, tree_batch
+from _golden import within_ulps
 from micro_vllm_b200 import (
+    AttentionMetadata,
     B200PagedAttentionOperator,
     ChunkedLocalSpec,
+    DraftKVCompactor,
     DraftTree,
-    AttentionMetadata,
     FullAttentionSpec,
+    Qwen3AttentionPrologue,
     SlidingWindowSpec,
     _lib,
+    accept_draft_tree,
     build_draft_tree,
+    rotary_inverse_frequencies,
 )
+from oracle.qk_prologue import qk_norm_rope_and_cache
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -103,6 +109,85 @@ def test_slots_of_pages_that_cannot_be_do_not_wrap() -> None:
     assert build(gpu).attention.slot_mapping.tolist()[3] == ((1 << 32) - 1) * 16 + 14
 
 
+# Requests x heads against the GPU's CTAs: a few long requests are cut into
+# shares of a tile or two, many middling ones leave whole items of several tiles.
+FEW = ([40, 7, 150, 0, 260], [3000, 901, 1290, 77, 2000])
+MANY = ([5, 12, 3, 9] * 12, [700, 391, 600, 515] * 12)
+
+
+@DTYPES
+@pytest.mark.parametrize("heads", [(4, 2), (16, 8)], ids=["4x2", "16x8"])
+@pytest.mark.parametrize("sizes", [FEW, MANY], ids=["few", "many"])
+@pytest.mark.parametrize("spec", [FULL, SlidingWindowSpec(333)], ids=["full", "window"])
+def test_values_that_are_not_finite_in_items_of_many_tiles(sizes, heads, spec, dtype) -> None:
+    nodes, committed = sizes
+    b = tree_batch(nodes, committed, q_heads=heads[0], kv_heads=heads[1], dtype=dtype, seed=51)
+    gen = np.random.default_rng(52)
+    bad = [torch.nan, torch.inf, -torch.inf]
+    for r, (n, c) in enumerate(zip(nodes, committed)):
+        if n == 0 or r % 4 == 3:
+            continue  # some requests stay clean
+        for i in range(0, n, 3):  # drafted branches, in every one of their tiles
+            if gen.random() < 0.4:
+                spoil(b, r, c + i, bad[i % 3], column=int(gen.integers(0, 128)), head=int(gen.integers(0, heads[1])))
+        if spec is not FULL:
+            for d in range(6):  # the window's edge: seen by the nodes near the root
+                spoil(b, r, c - 333 + 1 + d, bad[d % 3], column=5 * d)
+            spoil(b, r, c - 334, torch.nan)  # seen by none
+            spoil(b, r, c - 334, torch.nan, plane=0)
+        for p in range(c + n, -(-(c + n) // 16) * 16):  # behind the last node
+            spoil(b, r, p, torch.nan)
+            spoil(b, r, p, torch.nan, plane=0)
+    gpu = b.to(DEV)
+    operator = B200PagedAttentionOperator()
+    out = operator.attend_tree(gpu.query, gpu.cache, build(gpu, spec, 320))
+    check(out, b, plain_build(b, spec, 5))
+    assert operator.read_status(DEV) == 0
+
+
+@DTYPES
+@pytest.mark.parametrize("sizes", [FEW, MANY], ids=["few", "many"])
+def test_infinite_values_that_every_row_sees(sizes, dtype) -> None:
+    nodes, committed = sizes
+    b = tree_batch(nodes, committed, q_heads=4, kv_heads=2, dtype=dtype, seed=53)
+    for r, c in enumerate(committed):
+        spoil(b, r, c // 2, torch.inf, column=3)
+        spoil(b, r, c // 3, -torch.inf, column=9, head=1)
+        spoil(b, r, c // 5, torch.nan, column=100)
+    gpu = b.to(DEV)
+    out = B200PagedAttentionOperator().attend_tree(gpu.query, gpu.cache, build(gpu, max_nodes=320))
+    check(out, b, plain_build(b, words=5))
+
+
+@DTYPES
+@pytest.mark.parametrize("spec", [SlidingWindowSpec(1), SlidingWindowSpec(130), ChunkedLocalSpec(256)])
+def test_windows_with_missing_pages(spec, dtype) -> None:
+    b = tree_batch([20, 1, 64, 30], [250, 300, 45, 1021], q_heads=4, kv_heads=2, dtype=dtype, seed=54)
+    b.table[0, 13], b.table[0, 15], b.table[3, 60], b.table[3, 61] = -1, 1 << 40, b.cache.shape[1], -5
+    gpu = b.to(DEV)
+    operator = B200PagedAttentionOperator()
+    out = operator.attend_tree(gpu.query, gpu.cache, build(gpu, spec))
+    check(out, b, plain_build(b, spec))
+    assert operator.read_status(DEV) == _lib.MVB_STATUS_BLOCK_OUT_OF_RANGE
+
+
+@DTYPES
+def test_requests_that_run_backwards_leave_the_others_unharmed(dtype) -> None:
+    """Rows that two requests claim are undefined; all others are theirs."""
+
+    b = tree_batch([70, 5, 4, 6, 3], [40, 50, 60, 200, 70], dtype=dtype, seed=22)
+    gpu, operator = b.to(DEV), B200PagedAttentionOperator()
+    tree = build(gpu, max_nodes=128)
+    md = tree.attention
+    starts = md.query_start_locations.clone()
+    starts[2], starts[5] = 60, 1000  # request 1 runs backwards, the last one past the rows
+    odd = AttentionMetadata(md.query_positions, md.query_context_start_positions, starts, md.context_lengths,
+                            md.block_table, md.slot_mapping, 16)
+    out = operator.attend_tree(gpu.query, gpu.cache, DraftTree(odd, tree.ancestor_mask))
+    check(out, b, plain_build(b, words=2), only=[*range(60), *range(79, 85)])
+    assert not out[85:].any()
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32], ids=["fp16", "fp32"])
 def test_a_status_word_keeps_its_bits_over_captured_calls(dtype) -> None:
     """An operator whose first call is captured: nothing is set before the
@@ -162,3 +247,91 @@ def test_forward_tree_refuses_before_it_writes(dtype) -> None:
         operator.attend_tree(wide.new_zeros(rows, 4, 264), wide, tree)
     with pytest.raises(ValueError, match="head_dim"):
         operator.attend_tree(gpu.query[..., :0], wide[..., :0].contiguous(), tree)
+
+
+@pytest.mark.parametrize("block_size", [16, 48], ids=["pages", "odd-pages"])
+def test_attention_past_32_bit_offsets_off_the_tensor_tiles(block_size) -> None:
+    """fp32, and 16 bits with pages that are no power of two, at element
+    offsets past 2^31."""
+
+    dtype = torch.float32 if block_size == 16 else torch.bfloat16
+    blocks = (1 << 31) // (block_size * 8 * 128) + 64
+    b = tree_batch([12], [150], q_heads=16, kv_heads=8, seed=12, dtype=dtype, block_size=block_size)
+    cache = torch.zeros((2, blocks, block_size, 8, 128), dtype=dtype, device=DEV)
+    gpu = b.to(DEV)
+    pages = b.table.shape[1] - 1
+    far = torch.arange(blocks - pages, blocks, device=DEV)
+    cache[:, far] = gpu.cache[:, gpu.table[0, :pages]]
+    gpu.table[0, :pages] = far
+    check(B200PagedAttentionOperator().attend_tree(gpu.query, cache, build(gpu)), b, plain_build(b))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("spec", [FULL, SlidingWindowSpec(20)], ids=["full", "window"])
+def test_a_layer_through_the_prologue(spec, dtype) -> None:
+    """Projections, the fused prologue with the tree's metadata, attend_tree:
+    siblings share a rotary position and no slot."""
+
+    name = {torch.float16: "f16", torch.bfloat16: "bf16"}[dtype]
+    b = tree_batch([12, 1, 0, 30], [40, 3, 9, 130], q_heads=16, kv_heads=8, dtype=dtype, seed=57)
+    rows, normal = b.query.shape[0], torch.Generator().manual_seed(58)
+    fused = (torch.randn((rows, 32 * 128), generator=normal) * 2).to(dtype).to(DEV)
+    q, k, v = (part.unflatten(1, (-1, 128)) for part in fused.split([16 * 128, 8 * 128, 8 * 128], 1))
+    weights = (0.5 + torch.rand(2, 128, generator=normal)).to(dtype).to(DEV)
+    gpu, operator = b.to(DEV), B200PagedAttentionOperator()
+    tree, meta = build(gpu, spec), plain_build(b, spec)
+    md = tree.attention
+    prologue = Qwen3AttentionPrologue(weights[0], weights[1], 1e-6, 1e6)
+    rotated = prologue(md.query_positions, q, k, v, gpu.cache, md)
+    out = operator.attend_tree(rotated, gpu.cache, tree)
+
+    want_cache = b.cache.float().numpy().copy()
+    inverse = rotary_inverse_frequencies(128, 1e6, DEV).cpu().numpy()
+    want_q = qk_norm_rope_and_cache(
+        *(t.float().cpu().numpy() for t in (q, k, v)), meta[0], weights[0].float().cpu().numpy(),
+        weights[1].float().cpu().numpy(), 1e-6, inverse, want_cache, meta[3], name)
+    got_cache = gpu.cache.float().cpu().numpy()
+    assert within_ulps(rotated.float().cpu().numpy(), want_q, name, 2, rotated=True).all()
+    assert within_ulps(got_cache[0], want_cache[0], name, 2, rotated=True).all()
+    np.testing.assert_array_equal(got_cache[1], want_cache[1])
+    b.query, b.cache = rotated.cpu(), gpu.cache.cpu()
+    check(out, b, meta)
+
+
+@DTYPES
+def test_two_cache_groups_in_one_step(dtype) -> None:
+    """Layers of full attention and layers of a sliding window keep tables,
+    trees and moves of their own; the accepted path is one."""
+
+    nodes, committed, most = [12, 1, 30], [40, 3, 130], 6
+    room = [c + n for c, n in zip(committed, nodes)]
+    specs = [FULL, SlidingWindowSpec(25)]
+    groups = [tree_batch(nodes, room, q_heads=4, kv_heads=2, dtype=dtype, seed=60 + i) for i in range(2)]
+    for b in groups:
+        b.committed, b.parents = torch.tensor(committed), groups[0].parents
+    rows, normal = groups[0].query.shape[0], torch.Generator().manual_seed(62)
+    target = torch.randint(0, 4, (rows,), generator=normal)
+    drafts = torch.randint(0, 4, (rows,), generator=normal)
+    on_gpu = [b.to(DEV) for b in groups]
+    operator = B200PagedAttentionOperator()
+    keys, values = (torch.randn((2, rows, 2, 128), generator=normal).to(dtype) for _ in range(2))
+    outs = [operator.forward_tree(g.query, k.to(DEV), v.to(DEV), g.cache, build(g, spec))
+            for g, spec, k, v in zip(on_gpu, specs, keys, values)]
+    first = on_gpu[0]
+    kept = accept_draft_tree(drafts.to(DEV), target.to(DEV), first.parents, first.starts, first.committed, max_accepted=most)
+    for g in on_gpu:
+        DraftKVCompactor([g.cache])(g.table, g.committed, kept.nodes, kept.num_accepted)
+    want = plain.accept_draft_tree(drafts.numpy(), target.numpy(), groups[0].parents.numpy(), groups[0].starts.numpy(),
+                                   groups[0].committed.numpy(), most)
+    np.testing.assert_array_equal(kept.nodes.cpu().numpy(), want[0])
+    bits = torch.int32 if dtype == torch.float32 else torch.int16
+    for b, g, spec, out, k, v in zip(groups, on_gpu, specs, outs, keys, values):
+        meta = plain_build(b, spec)
+        flat = b.cache.view(2, -1, 2, 128)
+        flat[0, torch.from_numpy(meta[3])], flat[1, torch.from_numpy(meta[3])] = k, v
+        check(out, b, meta)
+        moved = plain.compact_draft_kv(b.cache.view(bits).numpy(), b.table.numpy(), b.committed.numpy(), want[0], want[1])
+        np.testing.assert_array_equal(g.cache.view(bits).cpu().numpy(), moved)
+        for r, c in enumerate(committed):  # a kept node lies where its rotary position says
+            path = want[0][r, :want[1][r]]
+            np.testing.assert_array_equal(meta[0][int(b.starts[r]) + path], c + np.arange(len(path)))

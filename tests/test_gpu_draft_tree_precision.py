@@ -75,3 +75,46 @@ def test_fp16_keeps_the_weights_of_a_long_tail(nodes, q_heads, bits) -> None:
     allowed = 2.0 ** -11 * np.abs(exact) + (2.0 ** -11 + 2 * keys * 2.0 ** -23 + 2.0 ** -18) * size
     allowed += 2.0 ** -25 + keys * 2.0 ** -32 * 2
     assert (np.abs(got - exact) <= allowed).all(), (np.abs(got - exact) / allowed).max()
+
+
+def plain_fp32(b, begin, lengths, mask):
+    """The attention of one batch in plain fp32 products and sums."""
+
+    out = torch.zeros(b.query.shape)
+    group, dim = b.query.shape[1] // b.cache.shape[3], b.query.shape[2]
+    words = mask.view(np.uint64)
+    for r, length in enumerate(lengths.tolist()):
+        first, n = int(b.starts[r]), int(b.starts[r + 1] - b.starts[r])
+        at = torch.arange(length)
+        k, v = (plane[b.table[r, at // b.block_size], at % b.block_size].repeat_interleave(group, 1) for plane in b.cache)
+        seen = torch.zeros(n, length, dtype=torch.bool)
+        for i in range(n):
+            seen[i, int(begin[first + i]): length - n] = True
+            for j in range(n):
+                seen[i, length - n + j] = bool((int(words[first + i, j // 64]) >> (j % 64)) & 1)
+        score = (b.query[first: first + n].transpose(0, 1) @ k.permute(1, 2, 0)) * dim ** -0.5
+        weight = torch.softmax(score.masked_fill(~seen, -torch.inf), 2)
+        out[first: first + n] = (weight @ v.transpose(0, 1)).transpose(0, 1)
+    return out.numpy().astype(np.float64)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("nodes, committed", [([24, 9], [100, 17]), ([24, 40], [1500, 700]), ([8], [12000])])
+def test_fp32_is_as_exact_as_plain_fp32(nodes, committed, dim) -> None:
+    """Two parts of 10 and 11 bits keep a factor to 2^-21 (the second is cut
+    off: 2^-23 of the factor in the mean square, no sign preferred), so a
+    product is off by 2^-22.5 and a sum of ``dim`` of them by sqrt(dim)
+    2^-22.5 of a term; plain fp32 rounds every partial sum, dim 2^-25.5 of a
+    term for a sequential sum: 8 / sqrt(dim) of it, 1 at 64.  With as much for
+    P.V and the sums cut off, twice plain fp32's error in the mean square is
+    what the path may have, and as it is spread alike, three times its largest.
+    Without the second parts the error is 2^10 times as large."""
+
+    b = tree_batch(nodes, committed, q_heads=4, kv_heads=2, dim=dim, dtype=torch.float32, seed=33)
+    got, exact, _, _, _ = attend(b, 1)
+    meta = plain.build_draft_tree(b.parents.numpy(), b.starts.numpy(), b.committed.numpy(), b.table.numpy(), b.block_size,
+                                  FULL.context_start, 1)
+    near = plain_fp32(b, meta[1], meta[2], meta[4])
+    rms = lambda x: float(np.sqrt(np.mean(np.square(x - exact))))  # noqa: E731
+    assert rms(got) <= 2 * rms(near), (rms(got), rms(near))
+    assert np.abs(got - exact).max() <= 3 * np.abs(near - exact).max()
