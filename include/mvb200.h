@@ -482,7 +482,8 @@ MVB_API int mvb_accept_draft_tree(const int64_t* draft_tokens, const int64_t* ta
  * Moves the kept nodes' K/V rows behind the committed ones, in place and bit
  * for bit: for every layer cache, plane and k < num_accepted[r], the row at
  * logical position C + nodes[r, k] goes to C + k.  layer_caches is a host
- * array of num_layers distinct device pointers, each a kv_cache of these sizes.
+ * array of num_layers device pointers, each a kv_cache of these sizes, without
+ * common memory.
  * nodes[r] must increase (as mvb_accept_draft_tree writes them); a request
  * whose entries do not, or whose positions or pages are out of range, is left
  * as it was in every layer and sets a status bit

@@ -539,9 +539,13 @@ int mvb_compact_draft_kv(void* const* layer_caches, int32_t num_layers, int64_t 
     return MVB_ERR_INVALID_ARGUMENT;
   for (int32_t i = 0; i < num_layers; ++i)
     if (!layer_caches[i] || ((uintptr_t)layer_caches[i] % eb) != 0) return MVB_ERR_INVALID_ARGUMENT;
-  for (int32_t i = 0; i < num_layers; ++i)  // a cache given twice would move twice
-    for (int32_t j = 0; j < i; ++j)
-      if (layer_caches[i] == layer_caches[j]) return MVB_ERR_INVALID_ARGUMENT;
+  // Rows of a cache given twice, or of two that overlap, would move twice.
+  const uint64_t bytes = 2 * (uint64_t)num_blocks * block_size * num_kv_heads * head_dim * eb;
+  for (int32_t i = 0; i < num_layers; ++i)
+    for (int32_t j = 0; j < i; ++j) {
+      const uintptr_t a = (uintptr_t)layer_caches[i], b = (uintptr_t)layer_caches[j];
+      if (a == b || (a > b ? a - b : b - a) < bytes) return MVB_ERR_INVALID_ARGUMENT;
+    }
   for (int32_t first = 0; first < num_layers; first += kMaxCompactLayers) {
     CompactArgs a;
     a.num_layers = num_layers - first < kMaxCompactLayers ? num_layers - first : kMaxCompactLayers;

@@ -217,8 +217,10 @@ class DraftKVCompactor:
                 raise ValueError("layer caches must share one shape, dtype and device")
         if first.numel() == 0:
             raise ValueError("layer caches must not be empty")
-        if len({t.data_ptr() for t in caches}) != len(caches):
-            raise ValueError("layer caches must be distinct: a row would move twice")
+        begins = sorted(t.data_ptr() for t in caches)
+        nbytes = first.numel() * first.element_size()
+        if any(b - a < nbytes for a, b in zip(begins, begins[1:])):
+            raise ValueError("layer caches must be distinct, without common memory: a row would move twice")
         self.layer_kv_caches = caches
         self._device = first.device
         self._dtype = _CACHE_DTYPES[first.dtype]

@@ -138,6 +138,17 @@ def test_the_path_query_takes_any_arguments(lib) -> None:
     assert path(q=ctypes.c_void_p(264)) == path(blocks=1 << 30) == 0
 
 
+def test_the_kv_move_refuses_caches_that_overlap(lib) -> None:
+    """2 x 4 x 16 x 2 x 8 fp16 values are 4096 bytes."""
+
+    def move(*at):
+        caches = (ctypes.c_void_p * len(at))(*at)
+        return lib.mvb_compact_draft_kv(caches, len(at), 4, 16, 2, 8, 0, FAKE, 8, 8, FAKE, FAKE, FAKE, 0, 4, None, None), \
+            lib.mvb_compact_draft_kv(caches, len(at), 4, 16, 2, 8, 0, FAKE, 8, 8, FAKE, FAKE, FAKE, 1, 4, None, None)
+
+    assert move(4096, 4096 + 4094) == move(8192, 256, 4608) == (_lib.MVB_OK, _lib.MVB_ERR_INVALID_ARGUMENT)
+
+
 def test_entry_points_refuse_cpu_tensors() -> None:
     b = tree_batch([3, 2], [4, 5])
     with pytest.raises(RuntimeError, match="require CUDA tensors"):

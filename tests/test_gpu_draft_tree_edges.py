@@ -109,6 +109,16 @@ def test_slots_of_pages_that_cannot_be_do_not_wrap() -> None:
     assert build(gpu).attention.slot_mapping.tolist()[3] == ((1 << 32) - 1) * 16 + 14
 
 
+def test_kv_move_refuses_caches_that_overlap() -> None:
+    flat = torch.zeros(3 * 2 * 4 * 16 * 2 * 8, dtype=torch.float16, device=DEV)
+    size = flat.numel() // 3
+    cut = lambda at: flat[at: at + size].view(2, 4, 16, 2, 8)  # noqa: E731
+    DraftKVCompactor([cut(2 * size), cut(0), cut(size)])
+    for at in (0, 8, size // 2, size - 8):
+        with pytest.raises(ValueError, match="distinct"):
+            DraftKVCompactor([cut(2 * size), cut(0), cut(at)])
+
+
 # Requests x heads against the GPU's CTAs: a few long requests are cut into
 # shares of a tile or two, many middling ones leave whole items of several tiles.
 FEW = ([40, 7, 150, 0, 260], [3000, 901, 1290, 77, 2000])
