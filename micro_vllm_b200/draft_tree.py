@@ -125,8 +125,8 @@ def build_draft_tree(
         raise RuntimeError("b200_paged draft trees require CUDA tensors")
     if not 1 <= max_nodes <= MAX_TREE_NODES:
         raise ValueError(f"max_nodes must be 1 .. {MAX_TREE_NODES}")
-    if block_size <= 0:
-        raise ValueError("block_size must be positive")
+    if not 1 <= block_size < 1 << 31:
+        raise ValueError("block_size must be positive and fit 32 bits")
     kind, param = spec_code(spec)
     parents = _vector("parents", parents, device)
     committed = _vector("committed_lengths", committed_lengths, device)

@@ -109,6 +109,16 @@ def test_slots_of_pages_that_cannot_be_do_not_wrap() -> None:
     assert build(gpu).attention.slot_mapping.tolist()[3] == ((1 << 32) - 1) * 16 + 14
 
 
+def test_metadata_refuses_sizes_that_do_not_fit() -> None:
+    gpu = tree_batch([3, 2], [14, 30], q_heads=1, kv_heads=1, dim=8).to(DEV)
+    for block_size in (0, -16, 1 << 31, (1 << 32) + 16):  # the last is 16 in 32 bits
+        with pytest.raises(ValueError, match="block_size"):
+            build_draft_tree(gpu.parents, gpu.starts, gpu.committed, gpu.table, block_size)
+    for max_nodes in (0, -1, 1025, (1 << 32) + 64):
+        with pytest.raises(ValueError, match="max_nodes"):
+            build_draft_tree(gpu.parents, gpu.starts, gpu.committed, gpu.table, 16, max_nodes=max_nodes)
+
+
 def test_kv_move_refuses_caches_that_overlap() -> None:
     flat = torch.zeros(3 * 2 * 4 * 16 * 2 * 8, dtype=torch.float16, device=DEV)
     size = flat.numel() // 3
