@@ -11,18 +11,21 @@
 // a last bit each time on average, so the hi products go round several sums (4
 // for q.k, 2 for P.V) and the small ones have their own: one sum for all was
 // 1.4e-6 off at 24 x 1.5K keys, against 5e-7 of a plain fp32 product; this is
-// 2.4e-7 off.
+// 2.4e-7 off and costs 3 % (200 x 128 x 1K keys 2.97 -> 3.06 ms, 64 x 32 x 1.5K
+// 350 -> 362 us).
 // The softmax is fp32, a warp owning 4 rows, their statistics in registers.
 // Tiles that hold infinities or NaN go through scalar loops: hi and lo of an
 // infinity are no sum, and what a row does not see must not reach it as 0 x NaN.
 //
 // Measured (B200, fp32, captured launches): 5 requests x 48 rows x up to 1.5K
-// keys 40 us, 64 x 32 x 1.5K keys 362 us and 200 x 128 x 1K keys 3.1 ms (34
+// keys 39 us, 64 x 32 x 1.5K keys 362 us and 200 x 128 x 1K keys 3.06 ms (34
 // TFLOP/s of useful products), 1 x 128 x 8K keys 129 us, 1 x 16 x 64 keys 15 us.
-// A tile takes two CTAs of an SM 17K cycles: a quarter q.k, a fifth P.V, the rest
-// softmax, copies and barriers; the tensor pipe is active for a third of it and
-// every second cycle issues, so that what bounds it are the latencies between
-// the barriers of a tile, with 16 warps an SM to cover them.  K and V rows
+// A tile takes a CTA 14K cycles beside the SM's other CTA: a third q.k, a third
+// P.V, a sixth the copies' instructions, a twelfth each the softmax and the
+// checks for infinities.  The tensor pipe is active for 40 % of the time and 55 %
+// of the cycles issue (2114 instructions per warp and tile, 192 of them tensor:
+// fragments are loaded as single words, and K and V cut into hi and lo by each
+// warp that reads them), with 16 warps an SM to cover latencies.  K and V rows
 // by bulk copies of one warp instead of cp.async by all took 516 against 369 us
 // at 64 x 32 x 1.5K keys.  On the CUDA cores the same tiles are bound by shared
 // memory (12-18 TFLOP/s; two operand loads for 32 FMA instructions).

@@ -21,13 +21,16 @@
 // CTA), which the merge launch behind joins in a fixed order.
 //
 // Measured (B200, 6549 GB/s and 1624 bf16 TFLOP/s measured peaks, captured
-// launches): 32 requests x 32 rows x 2.3K keys 68 us = 4255 GB/s; 64 x up to
-// 128 rows x 4K keys 192 us = 5451 GB/s; 64 x 256 rows x 6K keys 472 us = 867
-// TFLOP/s; 1 x 16 rows x 265 keys 17 us.  A call has a fixed part of about 17
-// us (8 until the first scores: metadata, block ids, first tiles; 9 for the
-// last epilogue and the join).  In between, the HBM reads bound up to 128
-// rows, and two query tiles are bound by the exponentials (2048 cycles per
-// key tile, as many as the MMAs) and the hand-overs around them.
+// launches; fp16, then bf16 with its two products): 32 requests x 32 rows x
+// 2.3K keys 72 us = 4235 GB/s and 76; 64 x 128 rows x 4K keys 209 us = 5123 GB/s
+// and 245; 64 x 256 rows x 6K keys 479 us = 862 TFLOP/s and 602; 1 x 16 rows x
+// 265 keys 17 and 18 us.  A call has a fixed part of about 17 us (8 until the
+// first scores: metadata, block ids, first tiles; 9 for the last epilogue and
+// the join).  In between, the HBM reads bound up to 128 rows of fp16.  What
+// bounds two query tiles and bf16 is the chain scores, softmax, P.V of each
+// stream, which two streams cover in part (P lies over S, so a stream's next
+// scores wait for its P.V): per key tile of two query tiles 2048 cycles of MMA
+// (3072 in bf16) and 2048 of exponentials.
 //
 // Inside a CTA (16 warps, roles without a block-wide barrier between items):
 //   warp 11   scheduler: describes items in a 4-slot ring, loads their Q tiles
