@@ -1056,14 +1056,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < kKeys; e += 2)
             mx[(e >> 1) & 3] = fmax3(mx[(e >> 1) & 3], __uint_as_float(sc[e >> 5][e & 31]),
                                      __uint_as_float(sc[e >> 5][(e & 31) + 1]));
-          const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+          // Rounded up, and compared by a difference: no P passes 2^(kTop + 8)
+          // however large the scores are.
+          const float tmax = __fmul_ru(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), p.scale_log2);
           // O / l is exact whatever the reference is.  fp16 holds [2^-14, 2^16)
           // in full: with P up to 2^15 a long tail of small weights comes
           // through (a weight is off by 2^-32 of the row's largest at most).
           // bf16 has fp32's exponents, and O less room for large values.
           constexpr float kTop = kBf16 ? 0.f : 7.f;
           float corr = 1.f;
-          if (tmax > m_ref + (kTop + kRescaleLog2)) {
+          if (tmax - m_ref > kTop + kRescaleLog2) {  // (two infinities: no)
             const float m_new = tmax - kTop;
             corr = ex2(m_ref - m_new);  // 0 when m_ref is -inf
             l *= corr;

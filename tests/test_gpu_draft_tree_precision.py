@@ -77,6 +77,31 @@ def test_fp16_keeps_the_weights_of_a_long_tail(nodes, q_heads, bits) -> None:
     assert (np.abs(got - exact) <= allowed).all(), (np.abs(got - exact) / allowed).max()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32], ids=["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("size", [1, 64, 1024, 2048])
+@pytest.mark.parametrize("nodes, committed", [([20], [900]), ([1, 90], [300, 2000])])
+def test_large_scores_pick_their_key(nodes, committed, size, dtype) -> None:
+    """Queries and keys of +-size: sums of 128 products are exact, scores go
+    up to 2^26 in powers of two.  From 64 on, other sums weigh nothing beside a
+    row's largest: the output is the mean of the values that have it."""
+
+    b = tree_batch(nodes, committed, q_heads=8, kv_heads=2, dtype=dtype, seed=34)
+    b.cache[0] = torch.sign(b.cache[0]) * size
+    b.query.copy_(torch.sign(b.query) * size)
+    flat = b.cache.view(2, -1, 2, 128)
+    for r, c in enumerate(committed):  # a key alike each query of some nodes
+        for i in range(0, nodes[r], 7):
+            p = (97 * i + 5) % c
+            flat[0, int(b.table[r, p // 16] * 16 + p % 16), 0] = b.query[int(b.starts[r]) + i, 1]
+    got, exact, weighted, _, keys = attend(b, 2)
+    rounded = torch.finfo(dtype).eps / 2
+    # The scores' own factor, scale, is rounded to fp32 alike in all of a row's.
+    score = 2.0 ** -22 * size * size * 128 ** 0.5 if size == 1 else 0.0
+    allowed = 2 * rounded * (np.abs(exact) + weighted) + (score + 2 * keys * 2.0 ** -23 + 2.0 ** -18) * weighted + 2.0 ** -20
+    assert np.isfinite(got).all()
+    assert (np.abs(got - exact) <= allowed).all(), (np.abs(got - exact) / allowed).max()
+
+
 def plain_fp32(b, begin, lengths, mask):
     """The attention of one batch in plain fp32 products and sums."""
 
