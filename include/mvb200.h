@@ -73,6 +73,13 @@ MVB_API const char* mvb_status_string(int status);
 MVB_API int mvb_last_cuda_error(void);
 
 /*
+ * Sets this host thread's stream-capture mode (cudaStreamCaptureMode) to *mode
+ * and *mode to the one before: a host that allocates or waits beside a capture
+ * of its own, and no part of it, does so in the relaxed mode.
+ */
+MVB_API int mvb_exchange_capture_mode(int32_t* mode);
+
+/*
  * KV-cache scatter ("reshape_and_cache").
  *
  * Replaces write_kv_cache (src/micro_vllm/attention/operators/reference.py:84-98)

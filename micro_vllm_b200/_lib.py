@@ -32,6 +32,8 @@ MVB_STATUS_BAD_PARENT = 32
 
 MVB_MAX_TREE_NODES = 1024
 
+CAPTURE_MODE_RELAXED = 2  # cudaStreamCaptureModeRelaxed
+
 MVB_SPEC_FULL = 0
 MVB_SPEC_SLIDING_WINDOW = 1
 MVB_SPEC_CHUNKED_LOCAL = 2
@@ -46,6 +48,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mvb_version": (ctypes.c_int, []),
     "mvb_status_string": (ctypes.c_char_p, [ctypes.c_int]),
     "mvb_last_cuda_error": (ctypes.c_int, []),
+    "mvb_exchange_capture_mode": (ctypes.c_int, [_P]),
     "mvb_reshape_and_cache": (
         ctypes.c_int,
         [_P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _I64, _I32, _P, _P],

@@ -64,6 +64,19 @@ const char* mvb_status_string(int status) {
 
 int mvb_last_cuda_error(void) { return g_last_cuda_error; }
 
+int mvb_exchange_capture_mode(int32_t* mode) {
+  if (!mode || *mode < cudaStreamCaptureModeGlobal || *mode > cudaStreamCaptureModeRelaxed)
+    return MVB_ERR_INVALID_ARGUMENT;
+  cudaStreamCaptureMode exchanged = static_cast<cudaStreamCaptureMode>(*mode);
+  const cudaError_t err = cudaThreadExchangeStreamCaptureMode(&exchanged);
+  if (err != cudaSuccess) {
+    set_last_cuda_error(err);
+    return MVB_ERR_CUDA;
+  }
+  *mode = exchanged;
+  return MVB_OK;
+}
+
 int mvb_debug_arm_decode_stall(int32_t cta, int32_t tile, int32_t wait_limit) {
   return arm_decode_stall(cta, tile, wait_limit);
 }

@@ -10,6 +10,7 @@ workspace exists (see ``reserve``).
 
 from __future__ import annotations
 
+import ctypes
 import math
 from abc import ABC, abstractmethod
 
@@ -47,7 +48,30 @@ class _DeviceState:
     def __init__(self, device: torch.device) -> None:
         self.workspace: torch.Tensor | None = None
         self.capacity = (0, 0, 0, 0, 0)  # tokens, requests, Hq, Hkv, D
-        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self.status = _zeroed_word(device)
+
+
+_status_words: list[torch.Tensor] = []  # kept: a graph may outlive the operator that it calls
+
+
+def _zeroed_word(device: torch.device) -> torch.Tensor:
+    """An int32 0 on ``device``, there for every stream.  It is made on a
+    stream of its own, so that an operator's first call may be captured: a
+    zero-fill in the graph would run with every replay, and the graph's memory
+    is written by its other nodes."""
+
+    lib, mode = _lib.load(), ctypes.c_int32(_lib.CAPTURE_MODE_RELAXED)
+    with torch.cuda.device(device):
+        _lib.check(lib.mvb_exchange_capture_mode(ctypes.byref(mode)), "b200_paged status word")
+        try:  # allocating and waiting would end a capture in any other mode
+            own = torch.cuda.Stream(device)
+            with torch.cuda.stream(own):
+                word = torch.zeros(1, dtype=torch.int32, device=device)
+            own.synchronize()
+        finally:
+            _lib.check(lib.mvb_exchange_capture_mode(ctypes.byref(mode)), "b200_paged status word")
+    _status_words.append(word)
+    return word
 
 
 def _meta(t: torch.Tensor, device: torch.device, name: str) -> torch.Tensor:
@@ -64,27 +88,13 @@ class B200PagedAttentionOperator(AttentionOperator):
     def __init__(self) -> None:
         self._lib = _lib.load()
         self._devices: dict[int, _DeviceState] = {}
-        # The status word of the device in use, ahead of a first call that is captured.
-        if torch.cuda.is_initialized() and not torch.cuda.is_current_stream_capturing():
-            self._state(torch.device("cuda"))
 
     # -- workspace -------------------------------------------------------
     def _state(self, device: torch.device) -> _DeviceState:
         idx = device.index if device.index is not None else torch.cuda.current_device()
         st = self._devices.get(idx)
         if st is None:
-            device = torch.device("cuda", idx)
-            with torch.cuda.device(device):
-                # A captured zero-fill would run with every replay, and clear
-                # what other calls set.
-                if torch.cuda.is_current_stream_capturing():
-                    raise RuntimeError(
-                        f"b200_paged has no status word on {device} yet: call reserve(), or attention once, before "
-                        "a CUDA-graph capture"
-                    )
-                st = _DeviceState(device)
-                torch.cuda.current_stream().synchronize()  # the word is 0 for every stream
-            st = self._devices.setdefault(idx, st)
+            st = self._devices.setdefault(idx, _DeviceState(torch.device("cuda", idx)))
         return st
 
     def reserve(

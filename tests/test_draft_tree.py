@@ -129,6 +129,12 @@ def test_c_entries_refuse_before_touching_the_device(lib) -> None:
     assert move(caches=(ctypes.c_void_p * 2)(256, None)) == move(caches=(ctypes.c_void_p * 2)(256, 257)) == bad
 
 
+def test_the_capture_mode_is_one_of_three(lib) -> None:
+    for mode in (-1, 3, 1 << 30):
+        assert lib.mvb_exchange_capture_mode(ctypes.byref(ctypes.c_int32(mode))) == _lib.MVB_ERR_INVALID_ARGUMENT
+    assert lib.mvb_exchange_capture_mode(None) == _lib.MVB_ERR_INVALID_ARGUMENT
+
+
 def test_the_path_query_takes_any_arguments(lib) -> None:
     def path(bs=16, hkv=2, d=128, rows=4, requests=1, hq=4, dt=0, blocks=4, q=FAKE):
         return lib.mvb_tree_attention_uses_tcgen05(q, 512, 128, FAKE, FAKE, blocks, bs, hkv, d, rows, requests, hq, dt)
