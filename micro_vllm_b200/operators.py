@@ -65,7 +65,7 @@ def _zeroed_word(device: torch.device) -> torch.Tensor:
         _lib.check(lib.mvb_exchange_capture_mode(ctypes.byref(mode)), "b200_paged status word")
         try:  # allocating and waiting would end a capture in any other mode
             own = torch.cuda.Stream(device)
-            with torch.cuda.stream(own):
+            with torch.cuda.stream(own), torch.inference_mode(False):  # read_status writes it anywhere
                 word = torch.zeros(1, dtype=torch.int32, device=device)
             own.synchronize()
         finally:

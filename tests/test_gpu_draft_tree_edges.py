@@ -109,6 +109,18 @@ def test_slots_of_pages_that_cannot_be_do_not_wrap() -> None:
     assert build(gpu).attention.slot_mapping.tolist()[3] == ((1 << 32) - 1) * 16 + 14
 
 
+@pytest.mark.parametrize("inside", [True, False])
+def test_the_status_is_read_in_and_out_of_inference_mode(inside) -> None:
+    b = tree_batch([7, 5], [200, 64], seed=55)
+    b.table[0, 3] = -1
+    gpu, operator = b.to(DEV), B200PagedAttentionOperator()
+    with torch.inference_mode(inside):
+        operator.attend_tree(gpu.query, gpu.cache, build(gpu))
+    with torch.inference_mode(not inside):
+        assert operator.read_status(DEV) == _lib.MVB_STATUS_BLOCK_OUT_OF_RANGE
+    assert operator.read_status(DEV) == 0
+
+
 def test_metadata_refuses_sizes_that_do_not_fit() -> None:
     gpu = tree_batch([3, 2], [14, 30], q_heads=1, kv_heads=1, dim=8).to(DEV)
     for block_size in (0, -16, 1 << 31, (1 << 32) + 16):  # the last is 16 in 32 bits
