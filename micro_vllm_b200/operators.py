@@ -54,9 +54,21 @@ class _DeviceState:
 _status_words: list[torch.Tensor] = []  # kept: a graph may outlive the operator that it calls
 
 
+def _stream_beside(device: torch.device) -> torch.cuda.Stream:
+    """A stream that no capture is on: torch hands its streams out in turn, the
+    captured one among them."""
+
+    for _ in range(64):
+        stream = torch.cuda.Stream(device)
+        with torch.cuda.stream(stream):
+            if not torch.cuda.is_current_stream_capturing():
+                return stream
+    raise RuntimeError("b200_paged: every stream is being captured")
+
+
 def _zeroed_word(device: torch.device) -> torch.Tensor:
-    """An int32 0 on ``device``, there for every stream.  It is made on a
-    stream of its own, so that an operator's first call may be captured: a
+    """An int32 0 on ``device``, there for every stream.  It is made on another
+    stream, so that an operator's first call may be captured: a
     zero-fill in the graph would run with every replay, and the graph's memory
     is written by its other nodes."""
 
@@ -64,7 +76,7 @@ def _zeroed_word(device: torch.device) -> torch.Tensor:
     with torch.cuda.device(device):
         _lib.check(lib.mvb_exchange_capture_mode(ctypes.byref(mode)), "b200_paged status word")
         try:  # allocating and waiting would end a capture in any other mode
-            own = torch.cuda.Stream(device)
+            own = _stream_beside(device)
             with torch.cuda.stream(own), torch.inference_mode(False):  # read_status writes it anywhere
                 word = torch.zeros(1, dtype=torch.int32, device=device)
             own.synchronize()

@@ -109,6 +109,22 @@ def test_slots_of_pages_that_cannot_be_do_not_wrap() -> None:
     assert build(gpu).attention.slot_mapping.tolist()[3] == ((1 << 32) - 1) * 16 + 14
 
 
+def test_many_operators_are_first_called_in_one_capture() -> None:
+    """More of them than torch has streams, the captured one among these."""
+
+    b = tree_batch([7], [40], seed=55)
+    gpu = b.to(DEV)
+    tree = build(gpu)
+    want = B200PagedAttentionOperator().attend_tree(gpu.query, gpu.cache, tree)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        operators = [B200PagedAttentionOperator() for _ in range(70)]
+        outs = [operator.attend_tree(gpu.query, gpu.cache, tree) for operator in operators]
+    graph.replay()
+    assert all(torch.equal(out, want) for out in outs)
+    assert [operator.read_status(DEV) for operator in operators] == [0] * 70
+
+
 @pytest.mark.parametrize("inside", [True, False])
 def test_the_status_is_read_in_and_out_of_inference_mode(inside) -> None:
     b = tree_batch([7, 5], [200, 64], seed=55)
